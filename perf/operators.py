@@ -1,0 +1,359 @@
+"""Cases of the 8-bit operators of the acoustic model (vosk.ops): quantised
+frames, the maps that say which cached frames an output row reads, and the
+matrix product over them.
+
+The three operators, as a program that runs layers in 8 bits uses them:
+
+  map     frame_map      which rows of a paged frame cache every output row of
+                         a step reads, from the streams' lengths and tables
+  rows    quantize_rows  rows of floats to 8-bit codes with a scale for each
+                         row, packed or scattered into a frame cache
+  linear  linear_int8    float rows in: quantised and multiplied in one call
+  splice  linear_int8    the product over a frame cache through a row map
+
+Codes are whole numbers and the definition fixes every one of them: the scale
+is the 32-bit rounding of max|x| / 127, a code is x / scale rounded half to
+even, decided by the exact quotient.
+"""
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+PAD = 64  # codes are kept in rows of a multiple of 64 bytes
+UNLIMITED = 1 << 29
+
+
+def listed():
+    return [
+        # one recognizer's chunk of 51 frames, the splice of one TDNN-F layer
+        {"name": "map one stream", "kind": "map", "streams": 1, "frames": 51, "ragged": False, "taps": 3, "step": 1,
+         "page": 512, "pages": 1, "limits": True, "clamp": True},
+        # a batch lane: 256 streams x 51 frames, one output row for three frames
+        {"name": "map 256 streams", "kind": "map", "streams": 256, "frames": 51, "ragged": False, "taps": 3, "step": 3,
+         "page": 512, "pages": 1, "limits": True, "clamp": True},
+        # thousands of streams of very different lengths, pages of 64 frames
+        {"name": "map ragged pages", "kind": "map", "streams": 4001, "frames": 200, "ragged": True, "taps": 5, "step": 1,
+         "page": 64, "pages": 8, "limits": True, "clamp": False},
+        # one frame of one stream
+        {"name": "rows one", "kind": "rows", "rows": 1, "k": 512, "type": "fp32", "scatter": False},
+        # a batch lane's chunk of a hidden layer into its frame cache
+        {"name": "rows 256x51 cache", "kind": "rows", "rows": 13056, "k": 512, "type": "fp32", "scatter": True},
+        # odd width, wide rows of a larger model in half precision
+        {"name": "rows odd bf16", "kind": "rows", "rows": 9001, "k": 2047, "type": "bf16", "scatter": False},
+        # a single token through a large layer
+        {"name": "linear one row", "kind": "linear", "rows": 1, "k": 4096, "n": 4096, "type": "bf16", "out": "bf16",
+         "relu": False, "affine": False, "residual": False},
+        # one stream's chunk through the output layer
+        {"name": "linear one chunk", "kind": "linear", "rows": 17, "k": 192, "n": 2000, "type": "fp32", "out": "fp32",
+         "relu": False, "affine": False, "residual": False},
+        # odd everything, the whole epilogue
+        {"name": "linear odd fp16", "kind": "linear", "rows": 1999, "k": 1001, "n": 777, "type": "fp16", "out": "fp16",
+         "relu": True, "affine": True, "residual": True},
+        # large: a prompt-sized batch through a wide layer
+        {"name": "linear large bf16", "kind": "linear", "rows": 8192, "k": 4096, "n": 4096, "type": "bf16", "out": "bf16",
+         "relu": False, "affine": False, "residual": False},
+        # TDNN-F layer of a batch lane, ragged: hidden -> bottleneck over two spliced frames
+        {"name": "splice to bottleneck", "kind": "splice", "streams": 256, "frames": 51, "ragged": True, "taps": 2,
+         "k": 512, "n": 96, "out": "fp32", "relu": False, "affine": False, "residual": False},
+        # ... and bottleneck -> hidden with ReLU, BatchNorm and the bypass
+        {"name": "splice to hidden", "kind": "splice", "streams": 256, "frames": 51, "ragged": False, "taps": 2,
+         "k": 96, "n": 512, "out": "fp32", "relu": True, "affine": True, "residual": True},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["map", "rows", "linear", "linear", "splice", "splice"])
+    if kind == "map":
+        while True:
+            c = {"kind": kind, "streams": _log(rng, 1, 5000), "frames": _log(rng, 1, 400), "ragged": rng.random() < 0.7,
+                 "taps": rng.randint(1, 5), "step": rng.choice([1, 1, 2, 3]), "page": rng.choice([16, 64, 100, 512]),
+                 "pages": rng.randint(1, 8), "limits": rng.random() < 0.7, "clamp": rng.random() < 0.5}
+            if c["streams"] * c["frames"] * c["taps"] <= 4001 * 200 * 5:
+                return c
+    if kind == "rows":
+        while True:
+            c = {"kind": kind, "rows": _log(rng, 1, 20000), "k": _log(rng, 8, 8192), "type": rng.choice(sorted(DTYPES)),
+                 "scatter": rng.random() < 0.5}
+            if c["rows"] * c["k"] <= 9001 * 2047:
+                return c
+    relu, affine, residual = (rng.random() < 0.5 for _ in range(3))
+    if kind == "linear":
+        while True:
+            c = {"kind": kind, "rows": _log(rng, 1, 8192), "k": _log(rng, 16, 4096), "n": _log(rng, 16, 4096),
+                 "type": rng.choice(sorted(DTYPES)), "out": rng.choice(sorted(DTYPES)), "relu": relu, "affine": affine,
+                 "residual": residual}
+            if c["rows"] * c["k"] * c["n"] <= 1 << 36:
+                return c
+    while True:
+        c = {"kind": kind, "streams": _log(rng, 1, 600), "frames": _log(rng, 1, 150), "ragged": rng.random() < 0.7,
+             "taps": rng.randint(1, 4), "k": _log(rng, 16, 1536), "n": _log(rng, 16, 2000), "out": rng.choice(sorted(DTYPES)),
+             "relu": relu, "affine": affine, "residual": residual}
+        if c["streams"] * c["frames"] * (c["taps"] * c["k"] + c["n"]) <= 1 << 26:
+            return c
+
+
+# ---- the plain forms
+
+
+def _padded(k):
+    return -(-k // PAD) * PAD
+
+
+def _plain_map(lengths, first, table, page, offsets, step, low, high, clamp, rows):
+    n = (lengths.clamp(min=0).long() + step - 1) // step
+    ends = n.cumsum(0)
+    starts = torch.cat([ends.new_zeros(1), ends])
+    row = torch.arange(rows.shape[0], device=rows.device)
+    r = torch.searchsorted(ends, row, right=True).clamp(max=len(lengths) - 1)
+    inside = row < ends[-1]
+    off = torch.tensor(offsets, device=rows.device)
+    lo = low.long() if low is not None else torch.full_like(ends, -UNLIMITED * 4)
+    hi = high.long() if high is not None else torch.full_like(ends, UNLIMITED * 4)
+    newest = torch.minimum(first.long() + step * (n - 1) + max(offsets), hi)
+    t = (first.long()[r] + step * (row - starts[r]))[:, None] + off
+    if clamp:
+        t = torch.minimum(torch.maximum(t, lo[r][:, None]), hi[r][:, None])
+    ring = page * table.shape[1]
+    held = (t >= lo[r][:, None]) & (t <= hi[r][:, None]) & (t > (newest - ring)[r][:, None])
+    at = t % ring
+    pg = table.long()[r[:, None], at // page]
+    out = torch.where(held & (pg >= 0), pg * page + at % page, torch.full_like(pg, -1))
+    return starts.to(torch.int32), torch.where(inside[:, None], out.to(torch.int32), rows)
+
+
+def _plain_codes(x):
+    """codes [M, padded K] and scales of the rows of x."""
+    m, k = x.shape
+    x = x.double()
+    top = x.abs().amax(1)
+    fine = torch.isfinite(x).all(1)
+    s = torch.where(fine, (top / 127).float(), torch.full_like(top, math.nan).float())
+    usable = (fine & (s > 0))[:, None]
+    q = torch.round(x / torch.where(usable, s.double()[:, None], torch.ones_like(x[:, :1])))
+    q = torch.where(usable, q.clamp(-127, 127), torch.zeros_like(q)).to(torch.int8)
+    codes = torch.zeros(m, _padded(k), dtype=torch.int8, device=x.device)
+    codes[:, :k] = q
+    return codes, s
+
+
+def _plain_epilogue(v, s):
+    if s["bias"] is not None:
+        v = v + s["bias"]
+    if s["relu"]:
+        v = v.clamp(min=0)
+    if s["gain"] is not None:
+        v = v * s["gain"] + s["shift"]
+    if s["residual"] is not None:
+        v = v + s["residual_scale"] * s["residual"].float()
+    return v.to(s["out_type"])
+
+
+def _plain_linear(codes, scales, s):
+    values = codes.float() * scales[:, None]
+    return _plain_epilogue((values @ s["weight"].float().t()) * s["weight_scale"], s)
+
+
+def _plain_splice(s):
+    rows = s["map"].long()
+    there = rows >= 0
+    at = rows.clamp(min=0)
+    values = s["codes"][at].float() * s["scales"][at][..., None] * there[..., None]
+    v = (values.flatten(1) @ s["weight"].float().t()) * s["weight_scale"]
+    v = _plain_epilogue(v, s)
+    inside = torch.arange(len(rows), device=rows.device) < s["count"]
+    return torch.where(inside[:, None], v, s["into"])
+
+
+# ---- states
+
+
+def _streams(c, g):
+    """lengths and first frames of the streams of a step, on the GPU, and the most rows that they can give."""
+    n, f = c["streams"], c["frames"]
+    if c["ragged"]:
+        lengths = torch.randint(0, f + 1, (n,), generator=g, device="cuda", dtype=torch.int32)
+    else:
+        lengths = torch.full((n,), f, dtype=torch.int32, device="cuda")
+    first = torch.randint(0, 2000, (n,), generator=g, device="cuda", dtype=torch.int32)
+    return lengths, first
+
+
+def _offsets(c):
+    return [3 * j - 3 * (c["taps"] // 2) for j in range(c["taps"])]
+
+
+def _epilogue_state(c, g, m, s):
+    n = c["n"]
+    gauss = lambda *shape: torch.randn(*shape, generator=g, device="cuda")  # noqa: E731
+    s["out_type"] = DTYPES[c["out"]]
+    s["bias"] = gauss(n) if c["affine"] else None
+    s["relu"] = c["relu"]
+    s["gain"] = 0.5 + torch.rand(n, generator=g, device="cuda") if c["affine"] else None
+    s["shift"] = 0.1 * gauss(n) if c["affine"] else None
+    s["residual"] = gauss(m, n).to(s["out_type"]) if c["residual"] else None
+    s["residual_scale"] = 0.75 if c["residual"] else 1.0
+
+
+def _weights(n, k, taps, g, s):
+    """int8 weights in the layout of the codes: each tap's k columns padded to a multiple of 64."""
+    w = torch.randn(n, taps, k, generator=g, device="cuda") / math.sqrt(taps * k)
+    top = w.abs().amax((1, 2))
+    s["weight_scale"] = top / 127
+    q = torch.round(w / s["weight_scale"][:, None, None]).clamp(-127, 127)
+    full = torch.zeros(n, taps, _padded(k), device="cuda")
+    full[:, :, :k] = q
+    s["weight"] = full.flatten(1).to(torch.int8)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    c, s = case, {"kind": case["kind"]}
+    if c["kind"] in ("map", "splice"):
+        lengths, first = _streams(c, g)
+        step, page, pages = c.get("step", 1), c.get("page", 256), c.get("pages", 1)
+        n = c["streams"]
+        table = torch.randperm(n * pages, generator=g, device="cuda").to(torch.int32).view(n, pages)
+        low = high = None
+        if c.get("limits", True):  # streams that begin or end inside the splice
+            low = (first - torch.randint(0, 10, (n,), generator=g, device="cuda")).to(torch.int32).clamp(min=0)
+            high = (first + lengths - 1 + torch.randint(0, 4, (n,), generator=g, device="cuda")).to(torch.int32)
+        cap = n * -(-c["frames"] // step)
+        s.update(lengths=lengths, first=first, table=table, page=page, offsets=_offsets(c), step=step, low=low, high=high,
+                 clamp=c.get("clamp", True), rows=torch.full((cap, c["taps"]), -7, dtype=torch.int32, device="cuda"),
+                 starts=torch.zeros(n + 1, dtype=torch.int32, device="cuda"))
+        if c["kind"] == "map":
+            return s
+        starts, s["map"] = _plain_map(lengths, first, table, page, s["offsets"], step, low, high, s["clamp"], s["rows"])
+        s["count"] = starts[-1:]
+        x = torch.randn(n * page * pages, c["k"], generator=g, device="cuda")
+        s["codes"], s["scales"] = _plain_codes(x.clamp(min=-0.5))  # activations after a ReLU and BatchNorm
+        _epilogue_state(c, g, cap, s)
+        _weights(c["n"], c["k"], c["taps"], g, s)
+        s["into"] = torch.full((cap, c["n"]), 0.5, dtype=s["out_type"], device="cuda")
+        return s
+    m, k, t = c["rows"], c["k"], DTYPES[c["type"]]
+    # rows of very different sizes, as activations of loud and quiet frames are; some rows are all zeros
+    x = torch.randn(m, k, generator=g, device="cuda") * torch.exp(torch.randn(m, 1, generator=g, device="cuda"))
+    x[torch.rand(m, generator=g, device="cuda") < 0.01] = 0
+    if c["kind"] == "rows" and m > 2:  # halves between codes: rounded to even
+        x[1] = torch.randint(-254, 255, (k,), generator=g, device="cuda") * 0.5
+        x[1, 0] = 127
+    s["x"] = x.to(t)
+    if c["kind"] == "rows":
+        s["slots"] = None
+        if c["scatter"]:  # a cache of four times the rows; some rows belong to no stream
+            s["slots"] = torch.randperm(4 * m, generator=g, device="cuda")[:m].to(torch.int32)
+            s["slots"][torch.rand(m, generator=g, device="cuda") < 0.05] = -1
+            # (one row more than the cache has, where the plain form puts those)
+            s["codes_and_one"] = torch.full((4 * m + 1, _padded(k)), 5, dtype=torch.int8, device="cuda")
+            s["scales_and_one"] = torch.full((4 * m + 1,), -1.0, device="cuda")
+            s["codes"], s["scales"] = s["codes_and_one"][:-1], s["scales_and_one"][:-1]
+        return s
+    _epilogue_state(c, g, m, s)
+    _weights(c["n"], k, 1, g, s)
+    return s
+
+
+def run(s):
+    if own:
+        from vosk import ops
+        if s["kind"] == "map":
+            return ops.frame_map(s["lengths"], s["first"], s["table"], s["page"], s["rows"], starts=s["starts"],
+                                 offsets=s["offsets"], step=s["step"], low=s["low"], high=s["high"], clamp=s["clamp"])
+        if s["kind"] == "rows":
+            if s["slots"] is None:
+                return ops.quantize_rows(s["x"])
+            return ops.quantize_rows(s["x"], s["codes"], s["scales"], rows=s["slots"])
+        more = {"bias": s["bias"], "relu": s["relu"], "gain": s["gain"], "shift": s["shift"], "residual": s["residual"],
+                "residual_scale": s["residual_scale"]}
+        if s["kind"] == "linear":
+            return ops.linear_int8(s["x"], s["weight"], s["weight_scale"], dtype=s["out_type"], **more)
+        return ops.linear_int8(s["codes"], s["weight"], s["weight_scale"], scale=s["scales"], rows=s["map"], count=s["count"],
+                               out=s["into"], **more)
+    if s["kind"] == "map":
+        return _plain_map(s["lengths"], s["first"], s["table"], s["page"], s["offsets"], s["step"], s["low"], s["high"],
+                          s["clamp"], s["rows"])
+    if s["kind"] == "rows":
+        codes, scales = _plain_codes(s["x"])
+        if s["slots"] is None:
+            return codes, scales
+        at = torch.where(s["slots"] < 0, len(s["scales"]), s["slots"]).long()
+        s["codes_and_one"][at], s["scales_and_one"][at] = codes, scales
+        return s["codes"], s["scales"]
+    if s["kind"] == "linear":
+        return _plain_linear(*_plain_codes(s["x"]), s)
+    return _plain_splice(s)
+
+
+# ---- the work that no form can do without
+
+
+def work(c):
+    size = lambda t: torch.finfo(DTYPES[t]).bits // 8  # noqa: E731
+    if c["kind"] == "rows":
+        b = c["rows"] * (c["k"] * size(c["type"]) + _padded(c["k"]) + 4 + (4 if c["scatter"] else 0))
+        return {"bytes": b, "flops": 3 * c["rows"] * c["k"]}
+    if c["kind"] == "linear":
+        m, k, n, taps = c["rows"], c["k"], c["n"], 1
+        b = m * k * size(c["type"])
+    else:
+        share = 0.5 if c["ragged"] else 1.0
+        m = int(c["streams"] * share * -(-c["frames"] // c.get("step", 1)))
+        taps = c["taps"]
+        b = 8 * c["streams"] + 4 * m * taps
+        if c["kind"] == "map":
+            return {"bytes": b + 4 * c["streams"] * (1 + c["pages"] + (2 if c["limits"] else 0)), "flops": 10 * m * taps}
+        k, n = c["k"], c["n"]
+        b += m * (k + 4)
+    b += n * (taps * k + 4) + m * n * size(c["out"]) * (2 if c["residual"] else 1) + (12 * n if c["affine"] else 0)
+    return {"bytes": b, "flops": 2 * m * n * taps * k}
+
+
+# ---- the definition in 64 bits
+
+
+def exact(case, seed):
+    """What run() returns, from the formulas: floats in 64 bits; None for whole numbers, which have no error."""
+    s = prepare(case, seed)
+    if case["kind"] == "map":
+        return None
+    if case["kind"] == "rows":
+        scale = s["x"].to(torch.float64).abs().max(dim=1).values / 127.0
+        if s["slots"] is None:
+            return None, scale
+        full = torch.full((len(s["scales"]),), -1.0, dtype=torch.float64, device="cuda")
+        keep = s["slots"] >= 0
+        full[s["slots"][keep].long()] = scale[keep]
+        return None, full
+    w = s["weight"].to(torch.float64) * s["weight_scale"].to(torch.float64)[:, None]
+    taps = case.get("taps", 1)
+    w = w.view(case["n"], taps, -1)[:, :, :case["k"]]
+    if case["kind"] == "linear":
+        x = s["x"].to(torch.float64)
+        step = (x.abs().max(dim=1, keepdim=True).values / 127.0).to(torch.float32).to(torch.float64)
+        a = torch.where(step > 0, torch.round(x / step), torch.zeros_like(x)).clamp(-127, 127) * step
+        y = a @ w[:, 0].t()
+    else:
+        y = torch.zeros(len(s["map"]), case["n"], dtype=torch.float64, device="cuda")
+        a = s["codes"].to(torch.float64)[:, :case["k"]] * s["scales"].to(torch.float64)[:, None]
+        a = torch.cat([a, torch.zeros_like(a[:1])])
+        for j in range(taps):  # row -1 is the row of zeros behind the cache
+            y += a[s["map"][:, j].long().clamp(min=-1)] @ w[:, j].t()
+    if case["affine"]:
+        y += s["bias"].to(torch.float64)
+    if case["relu"]:
+        y = torch.maximum(y, torch.zeros_like(y))
+    if case["affine"]:
+        y = y * s["gain"].to(torch.float64) + s["shift"].to(torch.float64)
+    if case["residual"]:
+        y = y + s["residual_scale"] * s["residual"].to(torch.float64)
+    if case["kind"] == "splice":
+        y[int(s["count"]):] = s["into"].to(torch.float64)[int(s["count"]):]
+    return y
