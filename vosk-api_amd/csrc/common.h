@@ -14,6 +14,8 @@ namespace vamd {
 int LogLevel();
 void SetLogLevel(int level);
 void LogMessage(const char* kind, const std::string& msg);
+// what vamd_last_error() returns on this thread (vosk_api.cc)
+void SetLastError(const std::string& msg);
 
 struct Fatal : std::runtime_error {
   explicit Fatal(const std::string& m) : std::runtime_error(m) {}

@@ -1,0 +1,100 @@
+// The 8-bit operators (int8_ops.hip): per-row quantisation, row maps of frame
+// caches, and the matrix product over 8-bit codes.  Behind the C entry points
+// of include/vosk_amd_ops.h and the engine's 8-bit acoustic model.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace vamd {
+
+enum FloatType { kFloat32 = 0, kFloat16 = 1, kBFloat16 = 2 };
+
+constexpr int kMaxTaps = 16;
+constexpr int kInt8Pad = 64;         // code rows are a multiple of 64 bytes per tap
+constexpr int kInt8MaxK = 1 << 17;   // a tap's sum of 127 * 127 * K stays in 32 bits
+inline int Int8Padded(int k) { return (k + kInt8Pad - 1) / kInt8Pad * kInt8Pad; }
+
+// Codes and scales of M rows of k floats:
+//   s = fl32(max |x| / 127),  c = x / s rounded half to even (exact quotient)
+// A row of zeros gives s = 0, c = 0; a row holding an Inf or a NaN gives
+// s = NaN, c = 0, so whatever is computed from it is NaN.  Columns [k,
+// padded k) of a code row are zeroed.  rows (optional): row m goes to row
+// rows[m] of a cache of `cache_rows` rows; an entry outside it is skipped.
+struct QuantizeRows {
+  const void* x;
+  int type;            // FloatType
+  long long m;
+  int k;
+  long long ldx;       // elements
+  const int* rows;
+  const int* count;    // device: rows from *count on are skipped (or nullptr)
+  long long cache_rows;
+  int8_t* codes;
+  long long ldc;       // bytes, a multiple of 16
+  float* scales;
+};
+void LaunchQuantizeRows(const QuantizeRows& a, hipStream_t s);
+
+// Which cache rows the output rows of a step read.  Stream r has lengths[r]
+// new frames from time first[r] on and gives n_r = ceil(lengths[r] / step)
+// output rows, at times first[r] + step * i; output rows are packed stream
+// after stream (starts = exclusive sums of n_r, the total last).  Frame t of
+// stream r lies in cache row table[r][(t mod ring) / page] * page + t mod page,
+// ring = pages * page.  Entry (row, j) names the row of frame t + offset[j],
+// t limited to [low[r], high[r]] (clamp: the nearest inside, else -1), -1
+// where the page is not assigned or the ring cannot hold the frame beside
+// the newest that the stream's rows name.
+struct FrameMap {
+  const int* lengths;
+  const int* first;
+  int streams;
+  const int* table;    // [streams][pages], rows ldt apart
+  long long ldt;
+  int pages, page;
+  int taps, step, clamp;
+  const int* low;      // [streams] or nullptr
+  const int* high;
+  int* starts;         // [streams + 1]
+  int* rows;           // [cap][taps]; rows from the total on are left as they were
+  long long cap;
+  int max_offset;
+  int offset[kMaxTaps];
+};
+void LaunchFrameMap(const FrameMap& a, hipStream_t s);
+
+// out[m][n] = epi(sw[n] * sum_j sa[r(m,j)] * sum_k a[r(m,j)][k] * w[n][j * K + k])
+// with r(m, j) = rows[m][j] (rows == nullptr: m, taps 1); an entry outside
+// [0, arows) adds nothing.  The inner sums are exact in 32-bit integers, the
+// rest is 32-bit floats in this order:
+//   v = sum over j ascending of fma(float(sum_j), sa_j, v)
+//   v = v * sw[n];  v = v + bias[n];  v = max(v, 0) (NaN stays);
+//   v = v * gain[n] + shift[n];  v = res_scale * residual[m][n] + v
+struct LinearInt8 {
+  const int8_t* a;
+  long long lda;       // bytes, a multiple of 16
+  const float* sa;
+  long long arows;
+  const int* rows;
+  int taps;
+  const int* count;    // device: output rows from *count on are left as they were (or nullptr)
+  const int8_t* w;
+  long long ldw;       // bytes, a multiple of 16
+  const float* sw;
+  int m, n, k;         // k: columns of one tap, a multiple of kInt8Pad
+  const float* bias;
+  const float* gain;
+  const float* shift;
+  const void* residual;
+  long long ldr;       // elements
+  int res_type;
+  float res_scale;
+  int relu;
+  void* out;
+  long long ldo;       // elements
+  int out_type;
+};
+void LaunchLinearInt8(const LinearInt8& a, hipStream_t s);
+
+}  // namespace vamd

@@ -26,6 +26,8 @@ namespace {
 thread_local std::string g_last_error;
 }
 
+void vamd::SetLastError(const std::string& msg) { g_last_error = msg; }
+
 #define API_TRY try {
 #define API_CATCH(ret)                                   \
   }                                                      \
