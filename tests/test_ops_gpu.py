@@ -194,6 +194,22 @@ def test_frame_map(ops, streams, most, taps, step, page, pages, limits, clamp):
     _map_case(ops, streams, most, taps, step, page, pages, limits, clamp, streams + most)
 
 
+@pytest.mark.parametrize("clamp", [False, True])
+@pytest.mark.parametrize("only", ["low", "high"])
+def test_frame_map_one_limit(ops, only, clamp):
+    rng = np.random.default_rng(7)
+    lengths, first = rng.integers(0, 20, 30).astype(np.int32), rng.integers(-20, 20, 30).astype(np.int32)
+    limit = (first + rng.integers(0, 10, 30)).astype(np.int32)
+    table = rng.permutation(60).astype(np.int32).reshape(30, 2)
+    before = np.full((int(lengths.sum()), 3), -9, np.int32)
+    dev = lambda v: torch.from_numpy(v).cuda()  # noqa: E731
+    rows = dev(before)
+    ops.frame_map(dev(lengths), dev(first), dev(table), 16, rows, offsets=(-5, 0, 6), clamp=clamp, **{only: dev(limit)})
+    kw = dict(low=None, high=None)
+    kw[only] = limit
+    np.testing.assert_array_equal(rows.cpu().numpy(), ref.frame_map(lengths, first, table, 16, (-5, 0, 6), 1, kw["low"], kw["high"], clamp, before)[1])
+
+
 def test_frame_map_with_less_room_than_rows(ops):
     _map_case(ops, 20, 30, 3, 1, 64, 1, True, True, 2, extra=-40)
     _map_case(ops, 20, 30, 3, 1, 64, 1, True, True, 3, extra=-100000)

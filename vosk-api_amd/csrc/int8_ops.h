@@ -14,6 +14,7 @@ enum FloatType { kFloat32 = 0, kFloat16 = 1, kBFloat16 = 2 };
 constexpr int kMaxTaps = 16;
 constexpr int kInt8Pad = 64;         // code rows are a multiple of 64 bytes per tap
 constexpr int kInt8MaxK = 1 << 17;   // a tap's sum of 127 * 127 * K stays in 32 bits
+constexpr int kInt8MaxRows = 1 << 30;  // rows and columns of one product
 inline int Int8Padded(int k) { return (k + kInt8Pad - 1) / kInt8Pad * kInt8Pad; }
 
 // Codes and scales of M rows of k floats:

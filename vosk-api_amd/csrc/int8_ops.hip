@@ -40,158 +40,474 @@ __device__ __forceinline__ void store_float(void* p, int type, long long i, floa
 // s / 2 decides.
 __device__ __forceinline__ int code_of(float x, float s, float inv) {
   float r = rintf(x * inv);
-  const float d = fmaf(-r, s, x), h = 0.5f * s;
-  const float ad = fabsf(d);
-  if (ad > h || (ad == h && ((int)r & 1))) r += d > 0.0f ? 1.0f : -1.0f;
-  r = fminf(fmaxf(r, -127.0f), 127.0f);
-  return (int)r;
+  const float d = fmaf(-r, s, x), ad = fabsf(d), h = 0.5f * s;
+  if (ad >= h) {  // hardly ever
+    if (ad > h || ((int)r & 1)) r += d > 0.0f ? 1.0f : -1.0f;
+  }
+  return (int)__builtin_amdgcn_fmed3f(r, -127.0f, 127.0f);
 }
 
-// ---- rows to codes: one wave per row, two passes
-template <int TYPE>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeRows a) {
-  const int lane = threadIdx.x & 63;
-  const long long m = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (m >= a.m || (a.count && m >= *a.count)) return;
-  const long long to = a.rows ? a.rows[m] : m;
-  if (to < 0 || to >= a.cache_rows) return;
-  uint32_t top = 0;
-  for (int i = lane; i < a.k; i += 64) {
-    const uint32_t u = __float_as_uint(load_float(a.x, TYPE, m * a.ldx + i)) & 0x7fffffffu;
-    top = u > top ? u : top;
-  }
+// A row's scale, and what code_of divides by: scales near the end of the
+// range are brought up so that 1 / s is finite, x with them.
+struct RowScale {
+  float scale, s, inv, up;
+  bool zero;  // codes 0: a row of zeros, or one that holds an Inf or a NaN
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t top) {  // top: the largest |x| as bits
+  RowScale r;
+  r.scale = top < 0x7f800000u ? __uint_as_float(top) / 127.0f : __uint_as_float(0x7fc00000u);
+  r.zero = !(r.scale > 0.0f);
+  r.up = r.scale < 0x1p-100f ? 0x1p100f : 1.0f;
+  r.s = r.zero ? 1.0f : r.scale * r.up;
+  r.inv = 1.0f / r.s;
+  return r;
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
-    const uint32_t u = __shfl_xor(top, o);
-    top = u > top ? u : top;
+    const uint32_t u = __shfl_xor(v, o);
+    v = u > v ? u : v;
   }
-  const bool fine = top < 0x7f800000u;
-  float s = fine ? __uint_as_float(top) / 127.0f : __uint_as_float(0x7fc00000u);
-  if (lane == 0) a.scales[to] = s;
-  const bool zero = !(s > 0.0f);
-  // scales near the end of the range are brought up so that 1 / s is finite
-  const float up = s < 0x1p-100f ? 0x1p100f : 1.0f;
-  s = zero ? 1.0f : s * up;
-  const float inv = 1.0f / s;
-  int8_t* c = a.codes + to * a.ldc;
+  return v;
+}
+
+// 16 bytes of a row, which may lie at any element; past the row: zeros
+template <int TYPE>
+struct Chunk {
+  static constexpr int N = TYPE == kFloat32 ? 4 : 8;  // elements
+  float v[N];
+  __device__ __forceinline__ void load(const void* x, long long row0, int e, int k) {
+    const char* p = (const char*)x + (row0 + e) * (16 / N);
+    if (e + N <= k) {
+      uint32_t w[4];
+      __builtin_memcpy(w, p, 16);
+      if constexpr (TYPE == kFloat32) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = __uint_as_float(w[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if constexpr (TYPE == kBFloat16) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+          } else {
+            v[2 * i] = __half2float(__ushort_as_half((unsigned short)w[i]));
+            v[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16)));
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = e + i < k ? load_float(x, TYPE, row0 + e + i) : 0.0f;
+    }
+  }
+  __device__ __forceinline__ uint32_t top(uint32_t t) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const uint32_t u = __float_as_uint(v[i]) & 0x7fffffffu;
+      t = u > t ? u : t;
+    }
+    return t;
+  }
+  __device__ __forceinline__ void store(int8_t* to, const RowScale& r) const {
+    uint32_t w[N / 4];
+#pragma unroll
+    for (int q = 0; q < N / 4; q++) {
+      w[q] = 0;
+      if (!r.zero) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[q] |= (uint32_t)(code_of(v[4 * q + i] * r.up, r.s, r.inv) & 0xff) << (8 * i);
+      }
+    }
+    __builtin_memcpy(__builtin_assume_aligned(to, N), w, N);
+  }
+};
+
+// ---- rows to codes: TPR threads (64 or 256) a row, the row kept in
+// registers (NV chunks of 16 bytes a thread) between the maximum and the
+// codes, so it is read once; NV = 0: longer rows are read twice.
+template <int TYPE, int TPR, int NV>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeRows a) {
+  constexpr int N = Chunk<TYPE>::N;
+  __shared__ uint32_t part[4];
+  const int tid = threadIdx.x % TPR;
+  const long long m = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  long long to = -1;
+  if (m < a.m && !(a.count && m >= *a.count)) to = a.rows ? a.rows[m] : m;
+  if (to < 0 || to >= a.cache_rows) return;  // the same in all threads of the row
   const int kp = (a.k + kInt8Pad - 1) / kInt8Pad * kInt8Pad;
-  for (int i = lane; i < kp; i += 64)
-    c[i] = i < a.k && !zero ? (int8_t)code_of(load_float(a.x, TYPE, m * a.ldx + i) * up, s, inv) : (int8_t)0;
+  const long long row0 = m * a.ldx;
+  Chunk<TYPE> c[NV ? NV : 1];
+  uint32_t top = 0;
+  if (NV) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) c[i].load(a.x, row0, (i * TPR + tid) * N, a.k);
+#pragma unroll
+    for (int i = 0; i < NV; i++) top = c[i].top(top);
+  } else {
+    for (int e = tid * N; e < a.k; e += TPR * N) {
+      c[0].load(a.x, row0, e, a.k);
+      top = c[0].top(top);
+    }
+  }
+  top = wave_max(top);
+  if (TPR > 64) {  // one row a workgroup
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = max(max(part[0], part[1]), max(part[2], part[3]));
+  }
+  const RowScale r = row_scale(top);
+  if (tid == 0) a.scales[to] = r.scale;
+  int8_t* const q = a.codes + to * a.ldc;
+  if (NV) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int e = (i * TPR + tid) * N;
+      if (e < kp) c[i].store(q + e, r);
+    }
+  } else {
+    for (int e = tid * N; e < kp; e += TPR * N) {
+      c[0].load(a.x, row0, e, a.k);
+      c[0].store(q + e, r);
+    }
+  }
+}
+
+template <int TYPE>
+void LaunchQuantize(const QuantizeRows& a, unsigned rows4, hipStream_t s) {
+  constexpr int N = Chunk<TYPE>::N;
+  const int kp = Int8Padded(a.k);
+  if (kp <= 64 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 2>), dim3(rows4), dim3(256), 0, s, a);
+  else if (kp <= 64 * 8 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 8>), dim3(rows4), dim3(256), 0, s, a);
+  else if (kp <= 256 * 4 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 4>), dim3((unsigned)a.m), dim3(256), 0, s, a);
+  else if (kp <= 256 * 8 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 8>), dim3((unsigned)a.m), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 0>), dim3((unsigned)a.m), dim3(256), 0, s, a);
 }
 
 // ---- row maps
-constexpr int kMapThreads = 256;
+//
+// A workgroup makes `per` output rows of the packed order.  Up to
+// kMapStreams streams it sums the streams' row counts itself, in LDS (at most
+// 16 KB of lengths out of L2, against a launch of its own for the sums);
+// with more, a first launch has written `starts` and the search reads those.
+constexpr int kMapThreads = 256, kMapStreams = 4096;
+
+__device__ __forceinline__ unsigned frame_rows(const FrameMap& a, int r) {  // output rows of stream r
+  return ((unsigned)max(a.lengths[r], 0) + (unsigned)a.step - 1u) / (unsigned)a.step;
+}
+
+// exclusive sums over the workgroup; *total: the sum of all
+__device__ __forceinline__ long long block_scan(long long sum, long long* total) {
+  __shared__ long long part[kMapThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  long long v = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  long long before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kMapThreads / 64; w++) {
+    if (w < wave) before += part[w];
+    all += part[w];
+  }
+  *total = all;
+  return before + v - sum;
+}
+
+__device__ __forceinline__ int saturated(long long v) { return (int)min(v, (long long)INT_MAX); }
 
 // exclusive sums of the streams' row counts: one workgroup
 __global__ __launch_bounds__(kMapThreads) void frame_starts_kernel(FrameMap a) {
-  __shared__ long long part[kMapThreads];
-  const int tid = threadIdx.x;
-  const int per = (a.streams + kMapThreads - 1) / kMapThreads;
-  const int lo = min(tid * per, a.streams), hi = min(lo + per, a.streams);
-  long long sum = 0;
-  for (int r = lo; r < hi; r++) sum += (max(a.lengths[r], 0) + (long long)a.step - 1) / a.step;
-  part[tid] = sum;
-  __syncthreads();
-  for (int o = 1; o < kMapThreads; o <<= 1) {
-    const long long v = tid >= o ? part[tid - o] : 0;
-    __syncthreads();
-    part[tid] += v;
-    __syncthreads();
-  }
-  long long at = part[tid] - sum;
+  const int tid = threadIdx.x, per = (a.streams + kMapThreads - 1) / kMapThreads;
+  const int lo = min((long long)tid * per, (long long)a.streams), hi = min(lo + (long long)per, (long long)a.streams);
+  long long sum = 0, total;
+  for (int r = lo; r < hi; r++) sum += frame_rows(a, r);
+  long long at = block_scan(sum, &total);
   for (int r = lo; r < hi; r++) {
-    a.starts[r] = (int)min(at, (long long)INT_MAX);
-    at += (max(a.lengths[r], 0) + (long long)a.step - 1) / a.step;
+    a.starts[r] = saturated(at);
+    at += frame_rows(a, r);
   }
-  if (tid == kMapThreads - 1) a.starts[a.streams] = (int)min(part[tid], (long long)INT_MAX);
+  if (tid == 0) a.starts[a.streams] = saturated(total);
 }
 
-__global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a) {
-  const long long total = a.starts[a.streams];
-  const long long rows = min(total, a.cap);
-  const int ring = a.pages * a.page;
-  for (long long row = (long long)blockIdx.x * kMapThreads + threadIdx.x; row < rows;
-       row += (long long)gridDim.x * kMapThreads) {
-    int lo = 0, hi = a.streams - 1;  // the last stream whose first row is not after this one
+template <bool SUM>
+__global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a, int per) {
+  // counts, then starts; a gap every 16 so that a thread's 16 counts lie in other banks than its neighbours'
+  __shared__ int sums[SUM ? kMapStreams + kMapStreams / 16 + 1 : 1];
+  const int tid = threadIdx.x;
+  auto at = [](int r) { return r + (r >> 4); };
+  long long total;
+  if (SUM) {
+    for (int r = tid; r < a.streams; r += kMapThreads) sums[at(r)] = (int)frame_rows(a, r);
+    __syncthreads();
+    const int each = (a.streams + kMapThreads - 1) / kMapThreads;
+    const int lo = min(tid * each, a.streams), hi = min(lo + each, a.streams);
+    long long sum = 0;
+    for (int r = lo; r < hi; r++) sum += (unsigned)sums[at(r)];
+    long long v = block_scan(sum, &total);
+    for (int r = lo; r < hi; r++) {
+      const unsigned n = (unsigned)sums[at(r)];
+      sums[at(r)] = saturated(v);
+      v += n;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+      for (int r = tid; r < a.streams; r += kMapThreads) a.starts[r] = sums[at(r)];
+      if (tid == 0) a.starts[a.streams] = saturated(total);
+    }
+  } else {
+    total = a.starts[a.streams];
+  }
+  auto start = [&](int r) -> long long { return SUM ? sums[at(r)] : a.starts[r]; };
+
+  const long long rows = min(total, a.cap), row0 = (long long)blockIdx.x * per * kMapThreads;
+  const unsigned ring = (unsigned)a.pages * (unsigned)a.page;
+  int r = -1, pr = -1;  // the row's stream; the one that the values below are of
+  long long first = 0, newest = 0, begin = 0, low = INT_MIN, high = INT_MAX;
+  for (int i = 0; i < per; i++) {
+    const long long row = row0 + (long long)i * kMapThreads + tid;
+    if (row >= rows) return;
+    int lo = r < 0 ? 0 : r, hi = a.streams - 1;  // the last stream that begins at or before the row
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (a.starts[mid] <= row) lo = mid;
+      if (start(mid) <= row) lo = mid;
       else hi = mid - 1;
     }
-    const int r = lo;
-    const long long n = (max(a.lengths[r], 0) + (long long)a.step - 1) / a.step;
-    const long long t0 = a.first[r] + (long long)a.step * (row - a.starts[r]);
-    long long newest = a.first[r] + (long long)a.step * (n - 1) + a.max_offset;
-    if (a.high) newest = min(newest, (long long)a.high[r]);
+    r = lo;
+    if (r != pr) {
+      pr = r;
+      begin = start(r);
+      first = a.first[r];
+      if (a.low) low = a.low[r];
+      if (a.high) high = a.high[r];
+      newest = first + (long long)a.step * ((long long)frame_rows(a, r) - 1) + a.max_offset;
+      if (a.high) newest = min(newest, high);
+    }
+    const long long t0 = first + (long long)a.step * (row - begin);
+    const int* const table = a.table + r * a.ldt;
     for (int j = 0; j < a.taps; j++) {
       long long t = t0 + a.offset[j];
-      if (a.clamp) {
-        if (a.low) t = max(t, (long long)a.low[r]);
-        if (a.high) t = min(t, (long long)a.high[r]);
-      }
-      bool held = t > newest - ring && t >= INT_MIN && t <= INT_MAX;
-      if (a.low) held = held && t >= a.low[r];
-      if (a.high) held = held && t <= a.high[r];
+      if (a.clamp && a.low) t = max(t, low);
+      if (a.clamp && a.high) t = min(t, high);
+      // (no limits: INT_MIN and INT_MAX, past which no frame has a row either)
+      const bool held = t > newest - ring && t >= low && t <= high;
       int to = -1;
       if (held) {
-        int at = (int)t % ring;
-        if (at < 0) at += ring;
-        const int pg = a.table[r * a.ldt + at / a.page];
-        if (pg >= 0) to = pg * a.page + at % a.page;
+        const unsigned u = t >= 0 ? (unsigned)t % ring : ring - 1u - (unsigned)(-1 - t) % ring;
+        const unsigned q = u / (unsigned)a.page;
+        const int pg = table[q];
+        if (pg >= 0) to = pg * a.page + (int)(u - q * (unsigned)a.page);
       }
       a.rows[row * a.taps + j] = to;
     }
   }
 }
 
-// ---- the product: one wave per 32 x 32 block of the output, operands
-// streamed from global memory into v_mfma_i32_32x32x32_i8 (lane half h holds
-// 16 bytes of its row / column; the accumulator of lane l is column l & 31,
-// rows (i & 3) + 8 * (i >> 2) + 4 * (l >> 5))
-__device__ __forceinline__ float finish(const LinearInt8& a, float v, long long m, int n, float sw) {
-  v = v * sw;
-  if (a.bias) v = v + a.bias[n];
-  if (a.relu) v = v < 0.0f ? 0.0f : v;
-  if (a.gain) v = v * a.gain[n] + a.shift[n];
-  if (a.residual) v = a.res_scale * load_float(a.residual, a.res_type, m * a.ldr + n) + v;
-  return v;
+// ---- the product
+//
+// Tiles of TM rows x TN columns, WM x WN waves, each wave (TM / WM) x (TN / WN)
+// in 32 x 32 blocks of v_mfma_i32_32x32x32_i8 (lane half h holds 16 bytes of
+// its row / column; the accumulator of lane l is column l & 31, rows
+// (i & 3) + 8 * (i >> 2) + 4 * (l >> 5)).  64 bytes of K a step; the tile's
+// rows of A (gathered through the row map) and of W go straight from global
+// memory into an ST-deep ring of LDS buffers, so ST - 1 steps of loads are in
+// flight behind the matrix instructions and one barrier a step is enough.
+// Rows are 64 bytes in LDS, their four 16-byte chunks permuted by
+// (row >> 1) & 3 (on the global side of the load: LDS takes lane after lane),
+// which spreads the eight rows that a 128-byte read covers over all banks.
+constexpr int kStepBytes = 64;
+
+// lane l's 16 bytes at p go to LDS byte `to` + 16 * l (to: the same in all lanes).
+// The compiler does not count these loads: WaitStep does.
+__device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "memory", "m0");
 }
 
-__global__ __launch_bounds__(64) void linear_int8_kernel(LinearInt8 a) {
-  __shared__ float srow[32];
-  const int lane = threadIdx.x, r = lane & 31, h = lane >> 5;
-  const int m0 = blockIdx.x * 32, n0 = blockIdx.y * 32;
-  const int mrows = a.count ? min(a.m, *a.count) : a.m;
-  if (m0 >= mrows) return;
-  const int n = n0 + r, nn = n < a.n ? n : a.n - 1;
-  float v[16];
-#pragma unroll
-  for (int i = 0; i < 16; i++) v[i] = 0.0f;
-  for (int j = 0; j < a.taps; j++) {
-    long long row = -1;
-    if (m0 + r < mrows) row = a.rows ? a.rows[(long long)(m0 + r) * a.taps + j] : m0 + r;
-    const bool there = row >= 0 && row < a.arows;
-    if (!there) row = 0;
-    __syncthreads();
-    if (h == 0) srow[r] = there ? a.sa[row] : 0.0f;
-    __syncthreads();
-    const int8_t* ap = a.a + row * a.lda + 16 * h;
-    const int8_t* wp = a.w + nn * a.ldw + (long long)j * a.k + 16 * h;
-    intx16 acc;
-#pragma unroll
-    for (int i = 0; i < 16; i++) acc[i] = 0;
-    for (int k = 0; k < a.k; k += 32) {
-      const intx4 x = *reinterpret_cast<const intx4*>(ap + k), w = *reinterpret_cast<const intx4*>(wp + k);
-      acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(x, w, acc, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = fmaf((float)acc[i], srow[(i & 3) + 8 * (i >> 2) + 4 * h], v[i]);
-  }
+// waits until at most N of this wave's loads to LDS are still on their way and
+// its reads of LDS are done, then for all waves
+template <int N>
+__device__ __forceinline__ void wait_step() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// Epilogue of 16 accumulator values of one column: rows m0 + (i & 3) + 8 * (i >> 2)
+__device__ __forceinline__ void finish_16(const LinearInt8& a, float (&v)[16], int m0, int n, int mrows) {
   if (n >= a.n) return;
   const float sw = a.sw[n];
 #pragma unroll
+  for (int i = 0; i < 16; i++) v[i] = v[i] * sw;
+  if (a.bias) {
+    const float b = a.bias[n];
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = v[i] + b;
+  }
+  if (a.relu) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+  }
+  if (a.gain) {
+    const float g = a.gain[n], c = a.shift[n];
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = v[i] * g + c;
+  }
+  if (a.residual) {
+    float z[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int m = m0 + (i & 3) + 8 * (i >> 2);
+      z[i] = m < mrows ? load_float(a.residual, a.res_type, (long long)m * a.ldr + n) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = a.res_scale * z[i] + v[i];
+  }
+#pragma unroll
   for (int i = 0; i < 16; i++) {
-    const int m = m0 + (i & 3) + 8 * (i >> 2) + 4 * h;
-    if (m < mrows) store_float(a.out, a.out_type, m * a.ldo + n, finish(a, v[i], m, n, sw));
+    const int m = m0 + (i & 3) + 8 * (i >> 2);
+    if (m < mrows) store_float(a.out, a.out_type, (long long)m * a.ldo + n, v[i]);
+  }
+}
+
+template <int TM, int TN, int WM, int WN, int ST, bool MULTI>
+__global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a, int tiles_m, int tiles_n) {
+  constexpr int NW = WM * WN, NT = 64 * NW;
+  constexpr int BM = TM / WM / 32, BN = TN / WN / 32;  // 32 x 32 blocks of a wave
+  constexpr int LOADS = (TM + TN) / 16 / NW;           // load instructions of a wave a step
+  static_assert((TM + TN) % (16 * NW) == 0 && (TM / 16) % LOADS == 0, "a wave loads rows of one operand");
+  extern __shared__ char smem[];                       // ST x [TM + TN][64], scales [taps][TM], rows [taps][TM]
+  float* const sscale = (float*)(smem + ST * (TM + TN) * kStepBytes);
+  int* const srow = (int*)(sscale + a.taps * TM);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // blocks b, b + 8, ... run on one XCD: give each XCD neighbouring tiles of
+  // a row of tiles, whose rows of A its L2 then reads once
+  const int tiles = tiles_m * tiles_n;
+  int t = blockIdx.x;
+  if (tiles % 8 == 0) t = (t & 7) * (tiles >> 3) + (t >> 3);
+  const int m0 = t / tiles_n * TM, n0 = t % tiles_n * TN;
+  const int mrows = a.count ? min(a.m, *a.count) : a.m;
+  if (m0 >= mrows) return;
+
+  for (int i = tid; i < TM * a.taps; i += NT) {
+    const int j = i / TM, m = m0 + i - j * TM;
+    long long row = -1;
+    if (m < mrows) row = a.rows ? a.rows[(long long)m * a.taps + j] : m;
+    const bool there = row >= 0 && row < a.arows;
+    srow[i] = there ? (int)row : 0;  // absent rows read row 0 with scale 0
+    sscale[i] = there ? a.sa[row] : 0.0f;
+  }
+  __syncthreads();
+
+  const int kt = a.k / kStepBytes, steps = kt * a.taps;
+  // this wave's loads: LOADS groups of 16 rows, lane l row l >> 2, chunk slot l & 3
+  const bool is_a = wave * LOADS < TM / 16;
+  const int group0 = is_a ? wave * LOADS : wave * LOADS - TM / 16;
+  const int lrow = lane >> 2, chunk = (lane & 3) ^ ((lrow >> 1) & 3);
+  const int8_t* p[LOADS];
+  auto aim = [&](int tap) {
+#pragma unroll
+    for (int g = 0; g < LOADS; g++) {
+      const int r = (group0 + g) * 16 + lrow;
+      if (is_a) p[g] = a.a + (long long)srow[tap * TM + r] * a.lda + 16 * chunk;
+      else if (tap == 0) p[g] = a.w + (long long)min(n0 + r, a.n - 1) * a.ldw + 16 * chunk;
+    }
+  };
+  aim(0);
+  const uint32_t to = lds_address(smem) + wave * LOADS * 1024;
+  int issued = 0, ik = 0, itap = 0, ibuf = 0;
+  auto issue = [&] {
+#pragma unroll
+    for (int g = 0; g < LOADS; g++) {
+      load_to_lds(p[g], to + ibuf * ((TM + TN) * kStepBytes) + g * 1024);
+      p[g] += kStepBytes;
+    }
+    issued++;
+    ibuf = ibuf + 1 == ST ? 0 : ibuf + 1;
+    if (MULTI && ++ik == kt) {
+      ik = 0;
+      if (++itap < a.taps) aim(itap);
+    }
+  };
+
+  const int r32 = lane & 31, h = lane >> 5;
+  const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
+  const int f0 = r32 * 64 + (((h) ^ ((r32 >> 1) & 3)) << 4), f1 = r32 * 64 + (((2 + h) ^ ((r32 >> 1) & 3)) << 4);
+  intx16 acc[BM][BN];
+  float v[MULTI ? BM : 1][MULTI ? BN : 1][16];
+#pragma unroll
+  for (int x = 0; x < BM; x++)
+#pragma unroll
+    for (int y = 0; y < BN; y++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        acc[x][y][i] = 0;
+        if (MULTI) v[x][y][i] = 0.0f;
+      }
+
+  for (int s = 0; s < ST - 1 && s < steps; s++) issue();
+  int buf = 0, k = 0, tap = 0;
+  for (int s = 0; s < steps; s++) {
+    const int behind = issued - s - 1;  // steps in flight after this one
+    if (behind >= ST - 2) wait_step<(ST - 2) * LOADS>();
+    else if (ST > 3 && behind == 1) wait_step<LOADS>();
+    else wait_step<0>();
+    if (issued < steps) issue();  // into the buffer that every wave left before the barrier
+    const char* const sa = smem + buf * ((TM + TN) * kStepBytes) + wm * 64;
+    const char* const sb = smem + buf * ((TM + TN) * kStepBytes) + (TM + wn) * 64;
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      const int f = q ? f1 : f0;
+      intx4 fa[BM], fb[BN];
+#pragma unroll
+      for (int x = 0; x < BM; x++) fa[x] = *reinterpret_cast<const intx4*>(sa + x * 2048 + f);
+#pragma unroll
+      for (int y = 0; y < BN; y++) fb[y] = *reinterpret_cast<const intx4*>(sb + y * 2048 + f);
+#pragma unroll
+      for (int x = 0; x < BM; x++)
+#pragma unroll
+        for (int y = 0; y < BN; y++) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[x], fb[y], acc[x][y], 0, 0, 0);
+    }
+    buf = buf + 1 == ST ? 0 : buf + 1;
+    if (MULTI && ++k == kt) {
+      k = 0;
+#pragma unroll
+      for (int x = 0; x < BM; x++) {
+        float sc[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) sc[i] = sscale[tap * TM + wm + x * 32 + 4 * h + (i & 3) + 8 * (i >> 2)];
+#pragma unroll
+        for (int y = 0; y < BN; y++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            v[x][y][i] = fmaf((float)acc[x][y][i], sc[i], v[x][y][i]);
+            acc[x][y][i] = 0;
+          }
+      }
+      tap++;
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < BM; x++) {
+    float sc[16];
+    if (!MULTI) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) sc[i] = sscale[wm + x * 32 + 4 * h + (i & 3) + 8 * (i >> 2)];
+    }
+#pragma unroll
+    for (int y = 0; y < BN; y++) {
+      float w[16];
+#pragma unroll
+      for (int i = 0; i < 16; i++) w[i] = MULTI ? v[x][y][i] : fmaf((float)acc[x][y][i], sc[i], 0.0f);
+      finish_16(a, w, m0 + wm + x * 32 + 4 * h, n0 + wn + y * 32 + r32, mrows);
+    }
   }
 }
 
@@ -205,24 +521,54 @@ unsigned Blocks(long long n, long long per) {
 
 void LaunchQuantizeRows(const QuantizeRows& a, hipStream_t s) {
   if (a.m <= 0) return;
-  const dim3 grid(Blocks(a.m, 4));
-  if (a.type == kFloat32) hipLaunchKernelGGL(quantize_rows_kernel<kFloat32>, grid, dim3(256), 0, s, a);
-  else if (a.type == kFloat16) hipLaunchKernelGGL(quantize_rows_kernel<kFloat16>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(quantize_rows_kernel<kBFloat16>, grid, dim3(256), 0, s, a);
+  const unsigned rows4 = Blocks(a.m, 4);
+  if (a.type == kFloat32) LaunchQuantize<kFloat32>(a, rows4, s);
+  else if (a.type == kFloat16) LaunchQuantize<kFloat16>(a, rows4, s);
+  else LaunchQuantize<kBFloat16>(a, rows4, s);
 }
 
 void LaunchFrameMap(const FrameMap& a, hipStream_t s) {
+  // about four workgroups a CU at most: each sums the streams once
+  const long long blocks256 = (a.cap + kMapThreads - 1) / kMapThreads;
+  const int per = (int)((blocks256 + 1023) / 1024 > 0 ? (blocks256 + 1023) / 1024 : 1);
+  const unsigned grid = (unsigned)((blocks256 + per - 1) / per);
+  if (a.streams <= kMapStreams) {
+    hipLaunchKernelGGL(frame_map_kernel<true>, dim3(grid ? grid : 1), dim3(kMapThreads), 0, s, a, per);
+    return;
+  }
   hipLaunchKernelGGL(frame_starts_kernel, dim3(1), dim3(kMapThreads), 0, s, a);
-  if (a.cap <= 0) return;
-  const long long b = (a.cap + kMapThreads - 1) / kMapThreads;
-  hipLaunchKernelGGL(frame_map_kernel, dim3((unsigned)(b < 65536 ? b : 65536)), dim3(kMapThreads), 0, s, a);
+  if (grid) hipLaunchKernelGGL(frame_map_kernel<false>, dim3(grid), dim3(kMapThreads), 0, s, a, per);
 }
+
+namespace {
+
+template <int TM, int TN, int WM, int WN, int ST, bool MULTI>
+void LaunchTile(const LinearInt8& a, hipStream_t s) {
+  const long long tm = ((long long)a.m + TM - 1) / TM, tn = ((long long)a.n + TN - 1) / TN;
+  if (tm * tn > INT_MAX) VAMD_ERR("too many tiles for one launch: " << a.m << " x " << a.n);
+  const size_t lds = ST * (TM + TN) * kStepBytes + (size_t)a.taps * TM * 8;
+  auto kernel = linear_tile_kernel<TM, TN, WM, WN, ST, MULTI>;
+  static const bool big = [&] {  // more than the default 64 KB of LDS has to be asked for
+    return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
+  }();
+  if (!big && lds > 65536) VAMD_ERR("the device does not give a workgroup " << lds << " bytes of LDS");
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, s, a, (int)tm, (int)tn);
+}
+
+}  // namespace
 
 void LaunchLinearInt8(const LinearInt8& a, hipStream_t s) {
   if (a.m <= 0 || a.n <= 0) return;
-  const unsigned gy = Blocks(a.n, 32);
-  if (gy > 65535) VAMD_ERR("too many columns for one launch: " << a.n);
-  hipLaunchKernelGGL(linear_int8_kernel, dim3(Blocks(a.m, 32), gy), dim3(64), 0, s, a);
+  auto tiles = [&](int tm, int tn) { return (((long long)a.m + tm - 1) / tm) * (((long long)a.n + tn - 1) / tn); };
+  const int pick = a.taps == 1 && tiles(256, 256) >= 256 ? 0 : tiles(128, 128) >= 384 ? 1 : 2;
+  if (a.taps > 1) {
+    if (pick <= 1) LaunchTile<128, 128, 2, 2, 4, true>(a, s);
+    else LaunchTile<64, 64, 2, 2, 4, true>(a, s);
+  } else {
+    if (pick == 0) LaunchTile<256, 256, 2, 4, 4, false>(a, s);
+    else if (pick == 1) LaunchTile<128, 128, 2, 2, 4, false>(a, s);
+    else LaunchTile<64, 64, 2, 2, 4, false>(a, s);
+  }
 }
 
 }  // namespace vamd

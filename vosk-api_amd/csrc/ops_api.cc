@@ -70,7 +70,7 @@ void CheckRows(const QuantizeRows& a) {
 }
 
 void CheckLinear(const LinearInt8& a) {
-  Want(a.m >= 0 && a.n >= 0, "linear_int8: bad sizes");
+  Want(a.m >= 0 && a.n >= 0 && a.m <= kInt8MaxRows && a.n <= kInt8MaxRows, "linear_int8: bad sizes");
   Want(a.k >= 1 && a.k <= kInt8MaxK, "linear_int8: k has to be in [1, 131072]");
   Want(a.taps >= 1 && a.taps <= kMaxTaps, "linear_int8: 1 to 16 taps");
   Want(FloatTypeOk(a.out_type), "linear_int8: unknown output type");
