@@ -24,11 +24,57 @@ def _err(lib):
     return lib.vamd_last_error().decode()
 
 
-def test_header_is_plain_c_and_every_function_is_exported(lib):
+_p, _q, _i, _f = C.c_void_p, C.c_longlong, C.c_int, C.c_float
+
+
+class Rows(C.Structure):
+    _fields_ = [(n, _p) for n in "x rows count codes scales".split()] + [(n, _q) for n in "m ldx cache_rows ldc".split()] + \
+        [(n, _i) for n in "type k".split()]
+
+
+class Map(C.Structure):
+    _fields_ = [(n, _p) for n in "lengths first table low high starts rows".split()] + [("ldt", _q), ("cap", _q)] + \
+        [(n, _i) for n in "streams pages page taps step clamp".split()] + [("offsets", _i * 16)]
+
+
+class Linear(C.Structure):
+    _fields_ = [(n, _p) for n in "codes scale rows count x workspace w wscale bias gain shift residual out".split()] + \
+        [(n, _q) for n in "cache_rows lda ldx ldw ldr ldo".split()] + \
+        [(n, _i) for n in "m n k taps relu x_type residual_type out_type".split()] + [("residual_scale", _f)]
+
+
+def _call(lib, name, kind, **fields):
+    return getattr(lib, name)(0, None, C.cast(C.pointer(kind(**fields)), C.c_char_p))
+
+
+def test_header_is_plain_c_and_every_function_is_exported(lib, tmp_path):
     subprocess.run(["gcc", "-fsyntax-only", "-Wall", "-Werror", "-x", "c", HDR], check=True)
     names = set(re.findall(r"\b(vamd_op_\w+)\s*\(", open(HDR).read()))
-    assert len(names) == 6
+    assert len(names) == 5
     assert not [n for n in names if not hasattr(lib, n)]
+
+
+def test_structures_are_laid_out_as_the_bindings_have_them(tmp_path):
+    """sizeof and offsetof of every field, from a C compiler, against the structures here and the packing in vosk.ops."""
+    from vosk import ops
+    kinds = {"VamdQuantizeRows": Rows, "VamdFrameMap": Map, "VamdLinearInt8": Linear}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "%s"' % HDR, "int main(void) {"]
+    for name, kind in kinds.items():
+        lines.append('printf("%%zu ", sizeof(%s));' % name)
+        lines += ['printf("%%zu ", offsetof(%s, %s));' % (name, f) for f, _ in kind._fields_]
+    (tmp_path / "a.c").write_text("\n".join(lines) + "return 0; }\n")
+    subprocess.run(["gcc", str(tmp_path / "a.c"), "-o", str(tmp_path / "a")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "a")], capture_output=True, text=True, check=True).stdout.split()]
+    want = []
+    for kind in kinds.values():
+        want += [C.sizeof(kind)] + [getattr(kind, f).offset for f, _ in kind._fields_]
+    assert got == want
+    assert len(ops._ROWS(*range(11))) == C.sizeof(Rows)
+    assert len(ops._MAP(*range(31))) == C.sizeof(Map)
+    packed = ops._LINEAR(*range(1, 28), 0.5)
+    assert C.sizeof(Linear) - 8 < len(packed) <= C.sizeof(Linear)
+    back = Linear.from_buffer_copy(packed.ljust(C.sizeof(Linear), b"\0"))
+    assert [getattr(back, f) for f, _ in Linear._fields_] == [*range(1, 28), 0.5]
 
 
 @pytest.mark.parametrize("k,want", [(1, 64), (64, 64), (65, 128), (1 << 17, 1 << 17), (0, -1), (-3, -1), ((1 << 17) + 1, -1)])
@@ -37,13 +83,21 @@ def test_code_bytes(lib, k, want):
 
 
 def test_workspace(lib):
-    assert lib.vamd_op_linear_workspace(3, 65) == 3 * (128 + 4)
-    assert lib.vamd_op_linear_workspace(0, 65) == 0
-    assert lib.vamd_op_linear_workspace(-1, 65) < 0
-    assert lib.vamd_op_linear_workspace(1, 0) < 0
+    assert lib.vamd_op_linear_workspace(1000, 500, 65) == 1000 * (128 + 4)
+    assert lib.vamd_op_linear_workspace(0, 5, 65) == 0
+    assert lib.vamd_op_linear_workspace(-1, 5, 65) < 0
+    assert lib.vamd_op_linear_workspace(1, -5, 65) < 0
+    assert lib.vamd_op_linear_workspace(1, 5, 0) < 0
+    assert lib.vamd_op_linear_workspace((1 << 30) + 1, 5, 64) < 0
 
 
-ROWS = dict(device=0, stream=None, x=P, type=0, m=4, k=100, ldx=100, rows=None, count=None, cache_rows=4, codes=P, ldc=128, scales=P)
+def test_no_arguments(lib):
+    for name in ("vamd_op_quantize_rows", "vamd_op_frame_map", "vamd_op_linear_int8"):
+        assert getattr(lib, name)(0, None, None) < 0
+        assert "null" in _err(lib)
+
+
+ROWS = dict(x=P, m=4, k=100, ldx=100, cache_rows=4, codes=P, ldc=128, scales=P)
 
 
 @pytest.mark.parametrize("change,what", [
@@ -53,65 +107,62 @@ ROWS = dict(device=0, stream=None, x=P, type=0, m=4, k=100, ldx=100, rows=None, 
     (dict(cache_rows=3), "fewer"), (dict(rows=P, cache_rows=-1), "fewer"),
 ])
 def test_quantize_rows_refuses(lib, change, what):
-    assert lib.vamd_op_quantize_rows(*{**ROWS, **change}.values()) < 0
+    assert _call(lib, "vamd_op_quantize_rows", Rows, **{**ROWS, **change}) < 0
     assert what in _err(lib)
 
 
 def test_nothing_to_do_is_no_error(lib):
-    assert lib.vamd_op_quantize_rows(*{**ROWS, "m": 0}.values()) == 0
-    assert lib.vamd_op_linear_int8(*{**LINEAR, "m": 0}.values()) == 0
-    assert lib.vamd_op_linear_int8(*{**LINEAR, "n": 0}.values()) == 0
+    assert _call(lib, "vamd_op_quantize_rows", Rows, **{**ROWS, "m": 0}) == 0
+    assert _call(lib, "vamd_op_linear_int8", Linear, **{**LINEAR, "m": 0}) == 0
+    assert _call(lib, "vamd_op_linear_int8", Linear, **{**FLOAT, "n": 0}) == 0
 
 
-MAP = dict(device=0, stream=None, lengths=P, first=P, streams=2, table=P, ldt=3, pages=3, page=8, offsets=None, taps=2, step=1,
-           low=None, high=None, clamp=1, starts=P, rows=P, cap=10)
+MAP = dict(lengths=P, first=P, streams=2, table=P, ldt=3, pages=3, page=8, taps=2, step=1, clamp=1, starts=P, rows=P, cap=10)
 
 
 @pytest.mark.parametrize("change,what", [
     (dict(streams=-1), "sizes"), (dict(cap=-1), "sizes"), (dict(cap=1 << 31), "sizes"), (dict(pages=0), "pages"),
     (dict(page=0), "pages"), (dict(pages=1 << 16, page=1 << 15), "pages"), (dict(taps=0), "offsets"), (dict(taps=17), "offsets"),
-    (dict(offsets=0), "offsets"), (dict(step=0), "step"), (dict(starts=None), "null"), (dict(lengths=None), "null"),
+    (dict(step=0), "step"), (dict(starts=None), "null"), (dict(lengths=None), "null"),
     (dict(first=None), "null"), (dict(table=None), "null"), (dict(rows=None), "null"), (dict(ldt=2), "overlap"),
 ])
 def test_frame_map_refuses(lib, change, what):
-    offsets = (C.c_int * 17)(*range(17))
-    a = {**MAP, "offsets": C.cast(offsets, C.c_void_p), **change}
-    a["offsets"] = a["offsets"] or None
-    assert lib.vamd_op_frame_map(*a.values()) < 0
+    assert _call(lib, "vamd_op_frame_map", Map, **{**MAP, **change}) < 0
     assert what in _err(lib)
 
 
-LINEAR = dict(device=0, stream=None, codes=P, lda=128, scale=P, cache_rows=5, rows=P, taps=2, count=None, w=P, ldw=256,
-              wscale=P, m=7, n=9, k=100, bias=None, relu=0, gain=None, shift=None, residual=None, ldr=0, residual_type=0,
-              residual_scale=1.0, out=P, ldo=9, out_type=0)
+LINEAR = dict(codes=P, lda=128, scale=P, cache_rows=5, rows=P, taps=2, w=P, ldw=256, wscale=P, m=7, n=9, k=100, residual_scale=1.0,
+              out=P, ldo=9)
 
 
 @pytest.mark.parametrize("change,what", [
-    (dict(m=-1), "sizes"), (dict(n=-1), "sizes"), (dict(k=0), "k has"), (dict(k=(1 << 17) + 1), "k has"), (dict(taps=0), "taps"),
-    (dict(taps=17), "taps"), (dict(out_type=-1), "output type"), (dict(codes=None), "null"), (dict(scale=None), "null"),
-    (dict(w=None), "null"), (dict(wscale=None), "null"), (dict(out=None), "null"), (dict(codes=P + 1), "16-byte"),
-    (dict(lda=136), "16-byte"), (dict(w=P + 4), "16-byte"), (dict(ldw=264), "16-byte"), (dict(cache_rows=0), "shorter"),
-    (dict(lda=64), "shorter"), (dict(ldw=128), "shorter"), (dict(rows=None), "row map"),
-    (dict(rows=None, taps=1, cache_rows=6), "fewer"), (dict(gain=P), "together"), (dict(shift=P), "together"),
-    (dict(ldo=8), "overlap"), (dict(out=P + 2), "aligned"), (dict(residual=P, residual_type=5), "residual type"),
-    (dict(residual=P + 2), "residual is not aligned"),
+    (dict(m=-1), "sizes"), (dict(n=-1), "sizes"), (dict(m=(1 << 30) + 1), "sizes"), (dict(n=(1 << 23) + 1), "sizes"),
+    (dict(ldo=(1 << 23) + 1), "2^23"), (dict(residual=P, ldr=(1 << 23) + 1), "2^23"), (dict(residual=P, ldr=8), "overlap"),
+    (dict(k=0), "k has"),
+    (dict(k=(1 << 17) + 1), "k has"), (dict(taps=0), "taps"), (dict(taps=17), "taps"), (dict(out_type=-1), "output type"),
+    (dict(codes=None), "null"), (dict(scale=None), "null"), (dict(w=None), "null"), (dict(wscale=None), "null"),
+    (dict(out=None), "null"), (dict(codes=P + 1), "16-byte"), (dict(lda=136), "16-byte"), (dict(w=P + 4), "16-byte"),
+    (dict(ldw=264), "16-byte"), (dict(cache_rows=0), "shorter"), (dict(lda=64), "shorter"), (dict(ldw=128), "shorter"),
+    (dict(rows=None), "row map"), (dict(rows=None, taps=1, cache_rows=6), "fewer"), (dict(gain=P), "together"),
+    (dict(shift=P), "together"), (dict(ldo=8), "overlap"), (dict(out=P + 2), "aligned"),
+    (dict(residual=P, residual_type=5), "residual type"), (dict(residual=P + 2, ldr=9), "residual is not aligned"),
+    (dict(x=P), "without codes"),
 ])
 def test_linear_int8_refuses(lib, change, what):
-    assert lib.vamd_op_linear_int8(*{**LINEAR, **change}.values()) < 0
+    assert _call(lib, "vamd_op_linear_int8", Linear, **{**LINEAR, **change}) < 0
     assert what in _err(lib)
 
 
-FLOAT = dict(device=0, stream=None, x=P, type=0, ldx=100, workspace=P, count=None, w=P, ldw=128, wscale=P, m=7, n=9, k=100,
-             bias=None, relu=0, gain=None, shift=None, residual=None, ldr=0, residual_type=0, residual_scale=1.0, out=P, ldo=9,
-             out_type=0)
+FLOAT = dict(x=P, ldx=100, workspace=P, w=P, ldw=128, wscale=P, m=700, n=9, k=100, taps=1, residual_scale=1.0, out=P, ldo=9)
 
 
 @pytest.mark.parametrize("change,what", [
-    (dict(k=0), "k has"), (dict(type=7), "element type"), (dict(x=None), "null"), (dict(ldx=50), "overlap"),
-    (dict(workspace=None), "null"), (dict(workspace=P + 4), "16-byte"), (dict(ldw=64), "shorter"), (dict(m=-2), "rows"),
+    (dict(k=0), "k has"), (dict(x_type=7), "element type"), (dict(ldx=50), "overlap"), (dict(x=P + 1), "aligned"),
+    (dict(workspace=None), "null"), (dict(workspace=P + 4), "16-byte"), (dict(ldw=64), "shorter"), (dict(m=-2), "sizes"),
+    (dict(rows=P), "without codes"), (dict(taps=2), "without codes"),
 ])
-def test_linear_float_refuses(lib, change, what):
-    assert lib.vamd_op_linear_float(*{**FLOAT, **change}.values()) < 0
+def test_linear_of_floats_refuses(lib, change, what):
+    assert _call(lib, "vamd_op_linear_int8", Linear, **{**FLOAT, **change}) < 0
     assert what in _err(lib)
 
 

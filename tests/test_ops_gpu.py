@@ -400,25 +400,31 @@ def test_refusals(ops):
     rows = torch.zeros(4, 1, dtype=torch.int32, device="cuda")
     cases = [
         (lambda: ops.quantize_rows(x.double()), "float32"),
-        (lambda: ops.quantize_rows(x.requires_grad_()), "gradient"),
-        (lambda: ops.quantize_rows(x.detach(), c), "together"),
-        (lambda: ops.quantize_rows(x.detach(), rows=rows[:, 0]), "codes and scales"),
-        (lambda: ops.quantize_rows(x.detach(), c[:, :64], s), "columns"),
-        (lambda: ops.quantize_rows(x.detach(), c[:3], s[:3]), "fewer"),
-        (lambda: ops.quantize_rows(x.detach(), c, s, rows=rows[:3, 0]), "4 elements"),
-        (lambda: ops.quantize_rows(x.detach()[:, :0]), "columns"),
+        (lambda: ops.quantize_rows(x.clone().requires_grad_()), "gradient"),
+        (lambda: ops.quantize_rows(x, c), "together"),
+        (lambda: ops.quantize_rows(x, rows=rows[:, 0]), "codes and scales"),
+        (lambda: ops.quantize_rows(x, c[:, :64], s), "columns"),
+        (lambda: ops.quantize_rows(x, c[:3], s[:3]), "fewer"),
+        (lambda: ops.quantize_rows(x, c, s, rows=rows[:3, 0]), "4 elements"),
+        (lambda: ops.quantize_rows(x[:, :0]), "columns"),
         (lambda: ops.linear_int8(c, w, ws), "scales"),
         (lambda: ops.linear_int8(c[:, :100], w, ws, scale=s), "multiple"),
         (lambda: ops.linear_int8(c, w[:, :64], ws, scale=s), "columns"),
         (lambda: ops.linear_int8(c, w, ws[:3], scale=s), "elements"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, rows=rows.long()), "int32"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, rows=rows.expand(4, 2)), "contiguous"),
-        (lambda: ops.linear_int8(x.detach(), w, ws, rows=rows), "belong to codes"),
+        (lambda: ops.linear_int8(x, w, ws, rows=rows), "belong to codes"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, gain=ws), "together"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, bias=ws.cpu()), "another device"),
-        (lambda: ops.linear_int8(c, w, ws, scale=s, residual=x.detach()), "residual"),
-        (lambda: ops.linear_int8(c, w, ws, scale=s, out=x.detach()), "out has"),
+        (lambda: ops.linear_int8(c, w, ws, scale=s, residual=x), "residual"),
+        (lambda: ops.linear_int8(c, w, ws, scale=s, out=x), "out has"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, dtype=torch.float64), "dtype"),
+        (lambda: ops.linear_int8(c, w, None, scale=s), "null"),
+        (lambda: ops.linear_int8(c, w, ws, scale=s, bias=3.0), "tensor"),
+        (lambda: ops.linear_int8(c, None, ws, scale=s), "tensor"),
+        (lambda: ops.linear_int8(x, w, ws, bias=ws.clone().requires_grad_()), "gradient"),
+        (lambda: ops.frame_map(rows[:, 0], None, rows, 8, rows), "first"),
+        (lambda: ops.frame_map(rows[:, 0], rows[:, 0], rows, 8, rows, offsets=(2**31,)), "32-bit"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, count=rows[:2, 0]), "elements"),
         (lambda: ops.frame_map(rows[:, 0], rows[:3, 0], rows, 8, rows), "elements"),
         (lambda: ops.frame_map(rows[:, 0], rows[:, 0], rows[:2], 8, rows), "row for each"),

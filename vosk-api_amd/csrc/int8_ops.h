@@ -14,7 +14,8 @@ enum FloatType { kFloat32 = 0, kFloat16 = 1, kBFloat16 = 2 };
 constexpr int kMaxTaps = 16;
 constexpr int kInt8Pad = 64;         // code rows are a multiple of 64 bytes per tap
 constexpr int kInt8MaxK = 1 << 17;   // a tap's sum of 127 * 127 * K stays in 32 bits
-constexpr int kInt8MaxRows = 1 << 30;  // rows and columns of one product
+constexpr long long kInt8MaxStride = 1 << 23;  // 32 rows of floats in a buffer of 2^30 bytes
+constexpr int kInt8MaxRows = 1 << 30, kInt8MaxCols = 1 << 23;  // of one product
 inline int Int8Padded(int k) { return (k + kInt8Pad - 1) / kInt8Pad * kInt8Pad; }
 
 // Codes and scales of M rows of k floats:
@@ -97,5 +98,9 @@ struct LinearInt8 {
   int out_type;
 };
 void LaunchLinearInt8(const LinearInt8& a, hipStream_t s);
+// The product of float rows: x's codes and scales are a's (a workspace, not
+// used where LinearFloatFused(a.m, a.k): one launch then quantises in LDS).
+bool LinearFloatFused(int m, int k);
+void LaunchLinearFloat(const LinearInt8& a, const QuantizeRows& x, hipStream_t s);
 
 }  // namespace vamd

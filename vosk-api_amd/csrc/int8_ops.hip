@@ -21,17 +21,10 @@ __device__ __forceinline__ float load_float(const void* p, int type, long long i
   return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
 }
 
-// round to nearest even; a NaN stays a (quiet) NaN
-__device__ __forceinline__ uint16_t to_bf16(float v) {
-  const uint32_t u = __float_as_uint(v);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
-
 __device__ __forceinline__ void store_float(void* p, int type, long long i, float v) {
   if (type == kFloat32) ((float*)p)[i] = v;
   else if (type == kFloat16) ((__half*)p)[i] = __float2half(v);
-  else ((uint16_t*)p)[i] = to_bf16(v);
+  else ((__bf16*)p)[i] = (__bf16)v;
 }
 
 // x / s rounded half to even, exactly: r = rint(x * (1 / s)) is off by one at
@@ -178,8 +171,11 @@ template <int TYPE>
 void LaunchQuantize(const QuantizeRows& a, unsigned rows4, hipStream_t s) {
   constexpr int N = Chunk<TYPE>::N;
   const int kp = Int8Padded(a.k);
+  // a wave a row as long as it fits its registers; with too few rows to fill
+  // the chip so, four waves share the longer ones
   if (kp <= 64 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 2>), dim3(rows4), dim3(256), 0, s, a);
-  else if (kp <= 64 * 8 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 8>), dim3(rows4), dim3(256), 0, s, a);
+  else if (kp <= 64 * 8 * N && a.m > 2048) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 8>), dim3(rows4), dim3(256), 0, s, a);
+  else if (kp <= 256 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 2>), dim3((unsigned)a.m), dim3(256), 0, s, a);
   else if (kp <= 256 * 4 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 4>), dim3((unsigned)a.m), dim3(256), 0, s, a);
   else if (kp <= 256 * 8 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 8>), dim3((unsigned)a.m), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 0>), dim3((unsigned)a.m), dim3(256), 0, s, a);
@@ -325,7 +321,7 @@ constexpr int kStepBytes = 64;
 // lane l's 16 bytes at p go to LDS byte `to` + 16 * l (to: the same in all lanes).
 // The compiler does not count these loads: WaitStep does.
 __device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "memory");
 }
 
 // waits until at most N of this wave's loads to LDS are still on their way and
@@ -335,44 +331,91 @@ __device__ __forceinline__ void wait_step() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// the same where only `behind` <= B steps of LOADS loads are left
+template <int B, int LOADS>
+__device__ __forceinline__ void wait_last(int behind) {
+  if constexpr (B > 0) {
+    if (behind == B) wait_step<B * LOADS>();
+    else wait_last<B - 1, LOADS>(behind);
+  } else {
+    wait_step<0>();
+  }
+}
+
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
-// Epilogue of 16 accumulator values of one column: rows m0 + (i & 3) + 8 * (i >> 2)
-__device__ __forceinline__ void finish_16(const LinearInt8& a, float (&v)[16], int m0, int n, int mrows) {
-  if (n >= a.n) return;
-  const float sw = a.sw[n];
+// The 16 values that a lane holds of a 32 x 32 block, rows (i & 3) + 8 * (i >>
+// 2) after its first: through a buffer that begins at the block's first row
+// and ends behind the last row of the matrix, so an access costs one 32-bit
+// add and the hardware's range check leaves out the rows past the end (and
+// the columns past it, whose offset is kOutside).
+constexpr uint32_t kOutside = 0x80000000u;
+struct BlockRows {
+  __amdgpu_buffer_rsrc_t rows;
+  uint32_t ld;  // bytes
+  __device__ __forceinline__ BlockRows(const void* p, int size, long long ldx, int first, int end)
+      : rows(__builtin_amdgcn_make_buffer_rsrc((char*)const_cast<void*>(p) + first * ldx * size, 0,
+                                               (int)min(max((long long)end - first, 0ll) * ldx * size, 32 * ldx * size),
+                                               0x00020000)),
+        ld((uint32_t)ldx * size) {}
+};
+template <class F>
+__device__ __forceinline__ void each_16(uint32_t off, uint32_t ld, F f) {
 #pragma unroll
-  for (int i = 0; i < 16; i++) v[i] = v[i] * sw;
+  for (int i = 0; i < 16; i++) f(i, off + ((i & 3) + 8 * (i >> 2)) * ld);
+}
+__device__ __forceinline__ void load_16(const BlockRows& b, int type, uint32_t off, float (&z)[16]) {
+  if (type == kFloat32)
+    each_16(off, b.ld, [&](int i, uint32_t o) { z[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b.rows, o, 0, 0)); });
+  else if (type == kFloat16)
+    each_16(off, b.ld, [&](int i, uint32_t o) { z[i] = __half2float(__ushort_as_half(__builtin_amdgcn_raw_buffer_load_b16(b.rows, o, 0, 0))); });
+  else
+    each_16(off, b.ld, [&](int i, uint32_t o) { z[i] = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(b.rows, o, 0, 0) << 16); });
+}
+__device__ __forceinline__ void store_16(const BlockRows& b, int type, uint32_t off, const float (&v)[16]) {
+  if (type == kFloat32)
+    each_16(off, b.ld, [&](int i, uint32_t o) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[i]), b.rows, o, 0, 0); });
+  else if (type == kFloat16)
+    each_16(off, b.ld, [&](int i, uint32_t o) { __builtin_amdgcn_raw_buffer_store_b16(__half_as_ushort(__float2half(v[i])), b.rows, o, 0, 0); });
+  else
+    each_16(off, b.ld, [&](int i, uint32_t o) { __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (__bf16)v[i]), b.rows, o, 0, 0); });
+}
+
+struct Column {  // a column's constants
+  float sw, bias, gain, shift;
+};
+__device__ __forceinline__ Column column(const LinearInt8& a, int n) {
+  Column c{a.sw[n], 0.0f, 1.0f, 0.0f};
+  if (a.bias) c.bias = a.bias[n];
+  if (a.gain) {
+    c.gain = a.gain[n];
+    c.shift = a.shift[n];
+  }
+  return c;
+}
+
+// Epilogue of a lane's 16 values of the block at row m0, column n of the lane
+// (z: the residual's)
+__device__ __forceinline__ void finish_16(const LinearInt8& a, float (&v)[16], const Column& c, const float (&z)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i++) v[i] = v[i] * c.sw;
   if (a.bias) {
-    const float b = a.bias[n];
 #pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = v[i] + b;
+    for (int i = 0; i < 16; i++) v[i] = v[i] + c.bias;
   }
   if (a.relu) {
 #pragma unroll
     for (int i = 0; i < 16; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];
   }
   if (a.gain) {
-    const float g = a.gain[n], c = a.shift[n];
 #pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = v[i] * g + c;
+    for (int i = 0; i < 16; i++) v[i] = v[i] * c.gain + c.shift;
   }
   if (a.residual) {
-    float z[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const int m = m0 + (i & 3) + 8 * (i >> 2);
-      z[i] = m < mrows ? load_float(a.residual, a.res_type, (long long)m * a.ldr + n) : 0.0f;
-    }
 #pragma unroll
     for (int i = 0; i < 16; i++) v[i] = a.res_scale * z[i] + v[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 16; i++) {
-    const int m = m0 + (i & 3) + 8 * (i >> 2);
-    if (m < mrows) store_float(a.out, a.out_type, (long long)m * a.ldo + n, v[i]);
   }
 }
 
@@ -381,18 +424,19 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
   constexpr int NW = WM * WN, NT = 64 * NW;
   constexpr int BM = TM / WM / 32, BN = TN / WN / 32;  // 32 x 32 blocks of a wave
   constexpr int LOADS = (TM + TN) / 16 / NW;           // load instructions of a wave a step
-  static_assert((TM + TN) % (16 * NW) == 0 && (TM / 16) % LOADS == 0, "a wave loads rows of one operand");
+  static_assert((TM + TN) % (16 * NW) == 0, "every wave has the same number of loads");
   extern __shared__ char smem[];                       // ST x [TM + TN][64], scales [taps][TM], rows [taps][TM]
   float* const sscale = (float*)(smem + ST * (TM + TN) * kStepBytes);
   int* const srow = (int*)(sscale + a.taps * TM);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // blocks b, b + 8, ... run on one XCD: give each XCD neighbouring tiles of
-  // a row of tiles, whose rows of A its L2 then reads once
-  const int tiles = tiles_m * tiles_n;
-  int t = blockIdx.x;
-  if (tiles % 8 == 0) t = (t & 7) * (tiles >> 3) + (t >> 3);
-  const int m0 = t / tiles_n * TM, n0 = t % tiles_n * TN;
+  // workgroups b, b + 8, ... run on one XCD: each XCD gets neighbouring tiles
+  // (GROUP rows of tiles, column after column), whose rows its L2 reads once
+  constexpr int GROUP = 4;
+  const int tiles = tiles_m * tiles_n, xcd = blockIdx.x & 7;
+  const int t = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (blockIdx.x >> 3);
+  const int g0 = t / (GROUP * tiles_n) * GROUP, gm = min(GROUP, tiles_m - g0), gt = t - g0 * tiles_n;
+  const int m0 = (g0 + gt % gm) * TM, n0 = gt / gm * TN;
   const int mrows = a.count ? min(a.m, *a.count) : a.m;
   if (m0 >= mrows) return;
 
@@ -408,16 +452,14 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
 
   const int kt = a.k / kStepBytes, steps = kt * a.taps;
   // this wave's loads: LOADS groups of 16 rows, lane l row l >> 2, chunk slot l & 3
-  const bool is_a = wave * LOADS < TM / 16;
-  const int group0 = is_a ? wave * LOADS : wave * LOADS - TM / 16;
   const int lrow = lane >> 2, chunk = (lane & 3) ^ ((lrow >> 1) & 3);
   const int8_t* p[LOADS];
   auto aim = [&](int tap) {
 #pragma unroll
     for (int g = 0; g < LOADS; g++) {
-      const int r = (group0 + g) * 16 + lrow;
-      if (is_a) p[g] = a.a + (long long)srow[tap * TM + r] * a.lda + 16 * chunk;
-      else if (tap == 0) p[g] = a.w + (long long)min(n0 + r, a.n - 1) * a.ldw + 16 * chunk;
+      const int r = (wave * LOADS + g) * 16 + lrow;  // of the tile's rows of A, then of W
+      if (r < TM) p[g] = a.a + (long long)srow[tap * TM + r] * a.lda + 16 * chunk;
+      else if (tap == 0) p[g] = a.w + (long long)min(n0 + r - TM, a.n - 1) * a.ldw + 16 * chunk;
     }
   };
   aim(0);
@@ -439,6 +481,22 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
 
   const int r32 = lane & 31, h = lane >> 5;
   const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
+  // the columns' constants, and the residual of a wave's only block, are on their way during the product
+  Column col[BN];
+#pragma unroll
+  for (int y = 0; y < BN; y++) col[y] = column(a, min(n0 + wn + y * 32 + r32, a.n - 1));
+  const int rsize = a.res_type == kFloat32 ? 4 : 2, osize = a.out_type == kFloat32 ? 4 : 2;
+  // a lane's offset in a block's rows
+  auto place = [&](int y, uint32_t ld, int size) {
+    const int n = n0 + wn + y * 32 + r32;
+    return n < a.n ? 4 * h * ld + (uint32_t)(n * size) : kOutside;
+  };
+  auto residual = [&](int x, int y, float (&z)[16]) {
+    const BlockRows b(a.residual, rsize, a.ldr, m0 + wm + x * 32, mrows);
+    load_16(b, a.res_type, place(y, b.ld, rsize), z);
+  };
+  float z[16];
+  if (BM * BN == 1 && a.residual) residual(0, 0, z);
   const int f0 = r32 * 64 + (((h) ^ ((r32 >> 1) & 3)) << 4), f1 = r32 * 64 + (((2 + h) ^ ((r32 >> 1) & 3)) << 4);
   intx16 acc[BM][BN];
   float v[MULTI ? BM : 1][MULTI ? BN : 1][16];
@@ -452,13 +510,22 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
         if (MULTI) v[x][y][i] = 0.0f;
       }
 
+  auto row_scales = [&](int tap, int x, float (&sc)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const float4 f = *reinterpret_cast<const float4*>(&sscale[tap * TM + wm + x * 32 + 4 * h + 8 * q]);
+      sc[4 * q] = f.x;
+      sc[4 * q + 1] = f.y;
+      sc[4 * q + 2] = f.z;
+      sc[4 * q + 3] = f.w;
+    }
+  };
   for (int s = 0; s < ST - 1 && s < steps; s++) issue();
   int buf = 0, k = 0, tap = 0;
   for (int s = 0; s < steps; s++) {
     const int behind = issued - s - 1;  // steps in flight after this one
     if (behind >= ST - 2) wait_step<(ST - 2) * LOADS>();
-    else if (ST > 3 && behind == 1) wait_step<LOADS>();
-    else wait_step<0>();
+    else wait_last<ST - 3, LOADS>(behind);
     if (issued < steps) issue();  // into the buffer that every wave left before the barrier
     const char* const sa = smem + buf * ((TM + TN) * kStepBytes) + wm * 64;
     const char* const sb = smem + buf * ((TM + TN) * kStepBytes) + (TM + wn) * 64;
@@ -481,8 +548,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
 #pragma unroll
       for (int x = 0; x < BM; x++) {
         float sc[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) sc[i] = sscale[tap * TM + wm + x * 32 + 4 * h + (i & 3) + 8 * (i >> 2)];
+        row_scales(tap, x, sc);
 #pragma unroll
         for (int y = 0; y < BN; y++)
 #pragma unroll
@@ -497,18 +563,179 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
 #pragma unroll
   for (int x = 0; x < BM; x++) {
     float sc[16];
-    if (!MULTI) {
-#pragma unroll
-      for (int i = 0; i < 16; i++) sc[i] = sscale[wm + x * 32 + 4 * h + (i & 3) + 8 * (i >> 2)];
-    }
+    if (!MULTI) row_scales(0, x, sc);
 #pragma unroll
     for (int y = 0; y < BN; y++) {
       float w[16];
 #pragma unroll
       for (int i = 0; i < 16; i++) w[i] = MULTI ? v[x][y][i] : fmaf((float)acc[x][y][i], sc[i], 0.0f);
-      finish_16(a, w, m0 + wm + x * 32 + 4 * h, n0 + wn + y * 32 + r32, mrows);
+      if (BM * BN > 1 && a.residual) residual(x, y, z);
+      finish_16(a, w, col[y], z);
+      const BlockRows b(a.out, osize, a.ldo, m0 + wm + x * 32, mrows);
+      store_16(b, a.out_type, place(y, b.ld, osize), w);
     }
   }
+}
+
+// ---- few rows
+//
+// The weights are what there is to read: a workgroup takes 16 columns, its
+// eight waves share the K steps (64 bytes of 16 weight rows each, straight
+// into v_mfma_i32_16x16x64_i8: lane l holds row / column l & 15, bytes
+// 16 * (l >> 4) of the step) and their integer sums are joined in LDS.  The
+// rows of codes lie in LDS whole; float rows are quantised there by the
+// workgroup itself, each workgroup for itself, which costs less than a launch
+// before this one.  A first batch of weight loads is on its way meanwhile.
+constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
+constexpr int kFusedValues = 16384;  // float values (rows x padded columns) that a workgroup quantises itself
+
+template <int TYPE, int RT>  // TYPE < 0: codes; RT blocks of 16 rows
+__global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, QuantizeRows x) {
+  constexpr int R = 16 * RT, AHEAD = 4;
+  extern __shared__ char smem[];  // codes [R][ldl], partial sums [8][RT][256], scales [taps][R], maxima [R]
+  const int kk = a.k * a.taps, ldl = kk + 16;  // 16 bytes on: rows in other banks
+  int* const part = (int*)(smem + R * ldl);
+  float* const sscale = (float*)(part + kFewWaves * RT * 256);
+  uint32_t* const smax = (uint32_t*)(sscale + a.taps * R);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int mrows = a.count ? min(a.m, *a.count) : a.m;
+  const int n0 = blockIdx.x * 16;
+  if (mrows <= 0) return;
+
+  const int steps = kk / 64;
+  const int8_t* const wp = a.w + (long long)min(n0 + (lane & 15), a.n - 1) * a.ldw + 16 * (lane >> 4);
+  intx4 w[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    const int s = wave + kFewWaves * i;
+    w[i] = *reinterpret_cast<const intx4*>(wp + 64 * (s < steps ? s : 0));
+  }
+
+  if constexpr (TYPE >= 0) {
+    constexpr int N = Chunk<TYPE < 0 ? 0 : TYPE>::N;
+    // all chunks of all rows (LinearFloatFused: HELD a thread) stay in registers
+    const int chunks = a.k / N, all = mrows * chunks;  // past a row's end: zeros
+    constexpr int HELD = kFusedValues / (kFewThreads * N);
+    Chunk<TYPE < 0 ? 0 : TYPE> c[HELD];
+    int mm[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+      const int q = tid + i * kFewThreads;
+      mm[i] = q / chunks;
+      if (q < all) c[i].load(x.x, mm[i] * x.ldx, (q - mm[i] * chunks) * N, x.k);
+    }
+    if (tid < R) smax[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+      if (tid + i * kFewThreads >= all) break;
+      uint32_t top = c[i].top(0);
+      if (__all(mm[i] == __builtin_amdgcn_readfirstlane(mm[i]))) {  // one atomic a wave where it holds one row
+        top = wave_max(top);
+        if (lane == 0) atomicMax(&smax[mm[i]], top);
+      } else {
+        atomicMax(&smax[mm[i]], top);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+      const int q = tid + i * kFewThreads;
+      if (q >= all) break;
+      const int e = (q - mm[i] * chunks) * N;
+      const RowScale r = row_scale(smax[mm[i]]);
+      c[i].store((int8_t*)smem + mm[i] * ldl + e, r);
+      if (e == 0) sscale[mm[i]] = r.scale;
+    }
+  } else {
+    const int chunks = a.k / 16, all = mrows * a.taps * chunks;
+    for (int i = tid; i < all; i += kFewThreads) {
+      const int q = i / chunks, e = (i - q * chunks) * 16, m = q / a.taps, j = q - m * a.taps;
+      long long row = a.rows ? a.rows[q] : m;
+      const bool there = row >= 0 && row < a.arows;
+      if (!there) row = 0;
+      *reinterpret_cast<intx4*>(smem + m * ldl + j * a.k + e) = *reinterpret_cast<const intx4*>(a.a + row * a.lda + e);
+      if (e == 0) sscale[j * R + m] = there ? a.sa[row] : 0.0f;
+    }
+  }
+  __syncthreads();
+
+  // element t of the 16 x 16 blocks: row t >> 4, column t & 15
+  constexpr int EACH = (RT * 256 + kFewThreads - 1) / kFewThreads;
+  float v[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; i++) v[i] = 0.0f;
+  intx4 acc[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) acc[t] = intx4{0, 0, 0, 0};
+  const int kt = a.k / 64;
+  const char* const ap = smem + (lane & 15) * ldl + 16 * (lane >> 4);
+  int tap = 0, end = kt;  // the tap's steps end there
+  auto join = [&] {       // the tap's integer sums, then the row's scale
+    if (tap) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        part[(wave * RT + t) * 256 + ((lane >> 4) * 4 + i) * 16 + (lane & 15)] = acc[t][i];
+        acc[t][i] = 0;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      const int t = tid + i * kFewThreads;
+      if (t < RT * 256) {
+        int sum = 0;
+#pragma unroll
+        for (int u = 0; u < kFewWaves; u++) sum += part[u * RT * 256 + t];
+        v[i] = fmaf((float)sum, sscale[tap * R + (t >> 4)], v[i]);
+      }
+    }
+    tap++;
+    end += kt;
+  };
+  for (int s0 = wave; s0 < steps; s0 += kFewWaves * AHEAD) {
+    // (a wave joins a tap when it is past it: every wave joins every tap once, in order)
+    intx4 u[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) {
+      u[i] = w[i];
+      const int s = s0 + kFewWaves * (AHEAD + i);
+      if (s < steps) w[i] = *reinterpret_cast<const intx4*>(wp + 64 * s);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) {
+      const int s = s0 + kFewWaves * i;
+      while (tap < a.taps && s >= end) join();
+      if (s < steps) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+          const intx4 f = *reinterpret_cast<const intx4*>(ap + t * 16 * ldl + 64 * s);
+          acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, u[i], acc[t], 0, 0, 0);
+        }
+      }
+    }
+  }
+  while (tap < a.taps) join();
+
+#pragma unroll
+  for (int i = 0; i < EACH; i++) {
+    const int t = tid + i * kFewThreads, m = t >> 4, n = n0 + (t & 15);
+    if (t >= RT * 256 || m >= mrows || n >= a.n) continue;
+    float y = v[i] * a.sw[n];
+    if (a.bias) y = y + a.bias[n];
+    if (a.relu) y = y < 0.0f ? 0.0f : y;
+    if (a.gain) y = y * a.gain[n] + a.shift[n];
+    if (a.residual) y = a.res_scale * load_float(a.residual, a.res_type, m * a.ldr + n) + y;
+    store_float(a.out, a.out_type, m * a.ldo + n, y);
+  }
+}
+
+// more than 64 KB of LDS has to be asked for
+void AskLds(const void* kernel, size_t bytes) {
+  if (bytes > 64 * 1024 &&
+      hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess)
+    VAMD_ERR("the device does not give a workgroup " << bytes << " bytes of LDS");
 }
 
 unsigned Blocks(long long n, long long per) {
@@ -548,26 +775,88 @@ void LaunchTile(const LinearInt8& a, hipStream_t s) {
   if (tm * tn > INT_MAX) VAMD_ERR("too many tiles for one launch: " << a.m << " x " << a.n);
   const size_t lds = ST * (TM + TN) * kStepBytes + (size_t)a.taps * TM * 8;
   auto kernel = linear_tile_kernel<TM, TN, WM, WN, ST, MULTI>;
-  static const bool big = [&] {  // more than the default 64 KB of LDS has to be asked for
-    return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess;
-  }();
-  if (!big && lds > 65536) VAMD_ERR("the device does not give a workgroup " << lds << " bytes of LDS");
+  AskLds((const void*)kernel, lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, s, a, (int)tm, (int)tn);
 }
 
 }  // namespace
 
+namespace {
+
+size_t FewLds(int m, int k, int taps) {
+  const size_t rt = m <= 16 ? 1 : 2;
+  return rt * 16 * ((size_t)k * taps + 16) + kFewWaves * rt * 1024 + rt * 16 * 4 * (taps + 1);
+}
+
+template <int TYPE, int RT>
+void LaunchFew(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
+  auto kernel = linear_few_kernel<TYPE, RT>;
+  const size_t lds = FewLds(a.m, a.k, a.taps);
+  AskLds((const void*)kernel, lds);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((a.n + 15) / 16)), dim3(kFewThreads), lds, s, a, x);
+}
+
+template <int TYPE>
+void LaunchFewRows(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
+  if (a.m <= 16) LaunchFew<TYPE, 1>(a, x, s);
+  else LaunchFew<TYPE, 2>(a, x, s);
+}
+
+}  // namespace
+
+// Up to 32 rows: with 64 the tiles take as long (us, few / tiles, k x n: 192 x
+// 2000 4.1 / 4.5, 1024 x 96 7.0 / 6.5, 4096 x 4096 15.3 / 15.3), with 32 they
+// take longer (3.3 / 4.4, 4.9 / 6.7, 14.1 / 15.4).
+bool LinearFewRows(int m, int k, int taps) { return m <= 32 && FewLds(m, k, taps) <= 160 * 1024; }
+
+// Each workgroup quantises all rows: worth it up to 16384 values (us, fused /
+// two launches: 4 rows of 4096 10.7 / 12.4, 17 of 512 6.5 / 7.0, 32 of 192
+// 5.0 / 6.3; but 16 of 1024 8.4 / 7.2, 32 of 512 8.6 / 7.1).
+bool LinearFloatFused(int m, int k) { return LinearFewRows(m, k, 1) && (long long)m * k <= kFusedValues; }
+
+void LaunchLinearFloat(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
+  if (a.m <= 0 || a.n <= 0) return;
+  if (LinearFloatFused(a.m, a.k)) {
+    if (x.type == kFloat32) LaunchFewRows<kFloat32>(a, x, s);
+    else if (x.type == kFloat16) LaunchFewRows<kFloat16>(a, x, s);
+    else LaunchFewRows<kBFloat16>(a, x, s);
+    return;
+  }
+  LaunchQuantizeRows(x, s);
+  LaunchLinearInt8(a, s);
+}
+
 void LaunchLinearInt8(const LinearInt8& a, hipStream_t s) {
   if (a.m <= 0 || a.n <= 0) return;
+  if (LinearFewRows(a.m, a.k, a.taps)) {
+    LaunchFewRows<-1>(a, QuantizeRows{}, s);
+    return;
+  }
+  // Tiles as large as leaves every CU one (us, 64 x 64 / 128 x 128 / 128 x 256 /
+  // 256 x 256 tiles, m x n x k):
+  //   1999 x 777 x 1001   6.8 /   8.9 /  11.7 /  16.6
+  //   4352 x 512 x 512    6.9 /   7.7 /   9.4 /  12.0
+  //   2048 x 2000 x 1024 13.3 /  12.2 /  14.4 /  19.1
+  //   4352 x 4096 x 1024 51.4 /  36.8 /  35.1 /  40.7
+  //   8192 x 4096 x 4096  278 /   187 /   157 /   130
+  //   4096 x 4096 x 4096  146 /    97 /    81 /    71
+  // but short products, which the stores bound, in the smallest:
+  //   13056 x 2000 x 96  21.0 /  22.5 /  23.2 /  22.8
+  // Several taps hold a second set of accumulators, which the larger tiles
+  // have no registers for; theirs gain from 128 x 128 at short K too
+  //   13056 x 512 x 2 * 96  12.4 / 10.5
   auto tiles = [&](int tm, int tn) { return (((long long)a.m + tm - 1) / tm) * (((long long)a.n + tn - 1) / tn); };
-  const int pick = a.taps == 1 && tiles(256, 256) >= 256 ? 0 : tiles(128, 128) >= 384 ? 1 : 2;
   if (a.taps > 1) {
-    if (pick <= 1) LaunchTile<128, 128, 2, 2, 4, true>(a, s);
-    else LaunchTile<64, 64, 2, 2, 4, true>(a, s);
+    if (tiles(128, 128) >= 256) LaunchTile<128, 128, 4, 2, 3, true>(a, s);
+    else LaunchTile<64, 64, 2, 2, 3, true>(a, s);
+  } else if (a.k < 256 || tiles(128, 128) < 256) {
+    LaunchTile<64, 64, 2, 2, 3, false>(a, s);
+  } else if (a.k >= 2048 && tiles(256, 256) >= 128) {
+    LaunchTile<256, 256, 4, 4, 4, false>(a, s);
+  } else if (tiles(128, 256) >= 256) {
+    LaunchTile<128, 256, 2, 4, 3, false>(a, s);
   } else {
-    if (pick == 0) LaunchTile<256, 256, 2, 4, 4, false>(a, s);
-    else if (pick == 1) LaunchTile<128, 128, 2, 2, 4, false>(a, s);
-    else LaunchTile<64, 64, 2, 2, 4, false>(a, s);
+    LaunchTile<128, 128, 4, 2, 3, false>(a, s);
   }
 }
 

@@ -70,8 +70,6 @@ void CheckRows(const QuantizeRows& a) {
 }
 
 void CheckLinear(const LinearInt8& a) {
-  Want(a.m >= 0 && a.n >= 0 && a.m <= kInt8MaxRows && a.n <= kInt8MaxRows, "linear_int8: bad sizes");
-  Want(a.k >= 1 && a.k <= kInt8MaxK, "linear_int8: k has to be in [1, 131072]");
   Want(a.taps >= 1 && a.taps <= kMaxTaps, "linear_int8: 1 to 16 taps");
   Want(FloatTypeOk(a.out_type), "linear_int8: unknown output type");
   if (a.m == 0 || a.n == 0) return;
@@ -85,9 +83,12 @@ void CheckLinear(const LinearInt8& a) {
   Want(a.rows || a.arows >= a.m, "linear_int8: fewer code rows than output rows");
   Want(!a.gain == !a.shift, "linear_int8: gain and shift go together");
   Want(a.ldo >= a.n || a.m == 1, "linear_int8: output rows overlap");
+  Want(a.ldo <= kInt8MaxStride || a.m == 1, "linear_int8: rows of out may be 2^23 elements apart at most");
   Want(Aligned(a.out, Bytes(a.out_type)), "linear_int8: out is not aligned to its elements");
   if (a.residual) {
     Want(FloatTypeOk(a.res_type), "linear_int8: unknown residual type");
+    Want(a.ldr >= a.n || a.m == 1, "linear_int8: residual rows overlap");
+    Want(a.ldr <= kInt8MaxStride || a.m == 1, "linear_int8: rows of residual may be 2^23 elements apart at most");
     Want(Aligned(a.residual, Bytes(a.res_type)), "linear_int8: residual is not aligned to its elements");
   }
 }
@@ -104,36 +105,35 @@ int vamd_op_code_bytes(int k) {
   return Int8Padded(k);
 }
 
-int vamd_op_quantize_rows(int device, void* stream, const void* x, int type, long long m, int k, long long ldx,
-                          const int* rows, const int* count, long long cache_rows, signed char* codes, long long ldc,
-                          float* scales) {
+int vamd_op_quantize_rows(int device, void* stream, const VamdQuantizeRows* p) {
   return Guarded([&] {
-    const QuantizeRows a{x, type, m, k, ldx, rows, count, cache_rows, (int8_t*)codes, ldc, scales};
+    Want(p != nullptr, "quantize_rows: null pointer");
+    const QuantizeRows a{p->x, p->type, p->m, p->k, p->ldx, p->rows, p->count, p->cache_rows,
+                         (int8_t*)p->codes, p->ldc, p->scales};
     CheckRows(a);
-    if (m == 0) return;
+    if (a.m == 0) return;
     OnDevice guard(device);
     LaunchQuantizeRows(a, (hipStream_t)stream);
     OnDevice::Check(hipGetLastError());
   });
 }
 
-int vamd_op_frame_map(int device, void* stream, const int* lengths, const int* first, int streams, const int* table,
-                      long long ldt, int pages, int page, const int* offsets, int taps, int step, const int* low,
-                      const int* high, int clamp, int* starts, int* rows, long long cap) {
+int vamd_op_frame_map(int device, void* stream, const VamdFrameMap* p) {
   return Guarded([&] {
-    Want(streams >= 0 && cap >= 0 && cap <= INT_MAX, "frame_map: bad sizes");
-    Want(pages >= 1 && page >= 1 && (long long)pages * page <= INT_MAX, "frame_map: bad pages");
-    Want(taps >= 1 && taps <= kMaxTaps && offsets, "frame_map: 1 to 16 offsets");
-    Want(step >= 1, "frame_map: step has to be at least 1");
-    Want(starts != nullptr, "frame_map: null pointer");
-    Want(streams == 0 || (lengths && first && table), "frame_map: null pointer");
-    Want(streams <= 1 || ldt >= pages, "frame_map: table rows overlap");
-    Want(cap == 0 || rows, "frame_map: null pointer");
-    FrameMap a{lengths, first, streams, table, ldt, pages, page, taps, step, clamp ? 1 : 0,
-               low, high, starts, rows, cap, INT_MIN, {}};
-    for (int j = 0; j < taps; j++) {
-      a.offset[j] = offsets[j];
-      if (offsets[j] > a.max_offset) a.max_offset = offsets[j];
+    Want(p != nullptr, "frame_map: null pointer");
+    Want(p->streams >= 0 && p->cap >= 0 && p->cap <= INT_MAX, "frame_map: bad sizes");
+    Want(p->pages >= 1 && p->page >= 1 && (long long)p->pages * p->page <= INT_MAX, "frame_map: bad pages");
+    Want(p->taps >= 1 && p->taps <= kMaxTaps, "frame_map: 1 to 16 offsets");
+    Want(p->step >= 1, "frame_map: step has to be at least 1");
+    Want(p->starts != nullptr, "frame_map: null pointer");
+    Want(p->streams == 0 || (p->lengths && p->first && p->table), "frame_map: null pointer");
+    Want(p->streams <= 1 || p->ldt >= p->pages, "frame_map: table rows overlap");
+    Want(p->cap == 0 || p->rows, "frame_map: null pointer");
+    FrameMap a{p->lengths, p->first, p->streams, p->table, p->ldt, p->pages, p->page, p->taps, p->step,
+               p->clamp ? 1 : 0, p->low, p->high, p->starts, p->rows, p->cap, INT_MIN, {}};
+    for (int j = 0; j < a.taps; j++) {
+      a.offset[j] = p->offsets[j];
+      if (a.offset[j] > a.max_offset) a.max_offset = a.offset[j];
     }
     OnDevice guard(device);
     LaunchFrameMap(a, (hipStream_t)stream);
@@ -141,54 +141,52 @@ int vamd_op_frame_map(int device, void* stream, const int* lengths, const int* f
   });
 }
 
-int vamd_op_linear_int8(int device, void* stream, const signed char* codes, long long lda, const float* scale,
-                        long long cache_rows, const int* rows, int taps, const int* count, const signed char* w,
-                        long long ldw, const float* wscale, int m, int n, int k, const float* bias, int relu,
-                        const float* gain, const float* shift, const void* residual, long long ldr, int residual_type,
-                        float residual_scale, void* out, long long ldo, int out_type) {
+int vamd_op_linear_int8(int device, void* stream, const VamdLinearInt8* p) {
   return Guarded([&] {
-    LinearInt8 a{(const int8_t*)codes, lda, scale, cache_rows, rows, taps, count, (const int8_t*)w, ldw, wscale,
-                 m, n, k, bias, gain, shift, residual, ldr, residual_type, residual_scale, relu ? 1 : 0,
-                 out, ldo, out_type};
+    Want(p != nullptr, "linear_int8: null pointer");
+    Want(p->m >= 0 && p->n >= 0 && p->m <= kInt8MaxRows && p->n <= kInt8MaxCols, "linear_int8: bad sizes");
+    Want(p->k >= 1 && p->k <= kInt8MaxK, "linear_int8: k has to be in [1, 131072]");
+    LinearInt8 a{(const int8_t*)p->codes, p->lda, p->scale, p->cache_rows, p->rows, p->taps, p->count,
+                 (const int8_t*)p->w, p->ldw, p->wscale, p->m, p->n, p->k, p->bias, p->gain, p->shift,
+                 p->residual, p->ldr, p->residual_type, p->residual_scale, p->relu ? 1 : 0, p->out, p->ldo, p->out_type};
+    QuantizeRows q{};
+    if (p->x) {
+      Want(!p->codes && !p->scale && !p->rows && p->taps == 1, "linear_int8: x comes without codes, scale and rows");
+      const int kb = Int8Padded(p->k);
+      a.a = (const int8_t*)p->workspace;
+      a.lda = kb;
+      a.sa = (const float*)(a.a + (long long)p->m * kb);
+      a.arows = p->m;
+      q = QuantizeRows{p->x, p->x_type, p->m, p->k, p->ldx, nullptr, p->count, p->m, (int8_t*)p->workspace, kb, (float*)a.sa};
+      if (p->m && p->n) {
+        if (LinearFloatFused(p->m, kb)) {  // no workspace: the checks below want addresses
+          static char none[16] __attribute__((aligned(16)));
+          q.codes = (int8_t*)none;
+          q.scales = (float*)none;
+          a.a = q.codes;
+          a.sa = q.scales;
+        }
+        CheckRows(q);
+      }
+    }
     CheckLinear(a);
-    if (m == 0 || n == 0) return;
-    a.k = Int8Padded(k);
+    if (a.m == 0 || a.n == 0) return;
+    a.k = Int8Padded(a.k);
+    if (a.m == 1) a.ldo = a.ldr = a.n;  // one row: any stride was right
     OnDevice guard(device);
-    LaunchLinearInt8(a, (hipStream_t)stream);
+    if (p->x) LaunchLinearFloat(a, q, (hipStream_t)stream);
+    else LaunchLinearInt8(a, (hipStream_t)stream);
     OnDevice::Check(hipGetLastError());
   });
 }
 
-long long vamd_op_linear_workspace(int m, int k) {
-  if (m < 0 || k < 1 || k > kInt8MaxK) {
-    SetLastError("bad sizes");
+long long vamd_op_linear_workspace(int m, int n, int k) {
+  if (m < 0 || m > kInt8MaxRows || n < 0 || n > kInt8MaxCols || k < 1 || k > kInt8MaxK) {
+    SetLastError("linear_int8: bad sizes");
     return -1;
   }
+  if (n == 0 || LinearFloatFused(m, Int8Padded(k))) return 0;
   return (long long)m * Int8Padded(k) + 4ll * m;
-}
-
-int vamd_op_linear_float(int device, void* stream, const void* x, int type, long long ldx, void* workspace,
-                         const int* count, const signed char* w, long long ldw, const float* wscale, int m, int n, int k,
-                         const float* bias, int relu, const float* gain, const float* shift, const void* residual,
-                         long long ldr, int residual_type, float residual_scale, void* out, long long ldo,
-                         int out_type) {
-  return Guarded([&] {
-    Want(k >= 1 && k <= kInt8MaxK, "linear_float: k has to be in [1, 131072]");
-    const int kb = Int8Padded(k);
-    int8_t* codes = (int8_t*)workspace;
-    float* scales = (float*)(codes + (long long)m * kb);
-    const QuantizeRows q{x, type, m, k, ldx, nullptr, count, m, codes, kb, scales};
-    LinearInt8 a{codes, kb, scales, m, nullptr, 1, count, (const int8_t*)w, ldw, wscale, m, n, k, bias, gain, shift,
-                 residual, ldr, residual_type, residual_scale, relu ? 1 : 0, out, ldo, out_type};
-    if (m != 0 && n != 0) CheckRows(q);
-    CheckLinear(a);
-    if (m == 0 || n == 0) return;
-    a.k = kb;
-    OnDevice guard(device);
-    LaunchQuantizeRows(q, (hipStream_t)stream);
-    LaunchLinearInt8(a, (hipStream_t)stream);
-    OnDevice::Check(hipGetLastError());
-  });
 }
 
 }  // extern "C"

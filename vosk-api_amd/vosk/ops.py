@@ -20,6 +20,7 @@ is imported first; importing this module after vosk alone raises ImportError.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -39,16 +40,12 @@ def _one_runtime():
 
 _one_runtime()
 
-_vp, _i, _ll, _f = C.c_void_p, C.c_int, C.c_longlong, C.c_float
 _SIGS = {
-    "vamd_op_code_bytes": (_i, [_i]),
-    "vamd_op_quantize_rows": (_i, [_i, _vp, _vp, _i, _ll, _i, _ll, _vp, _vp, _ll, _vp, _ll, _vp]),
-    "vamd_op_frame_map": (_i, [_i, _vp, _vp, _vp, _i, _vp, _ll, _i, _i, _vp, _i, _i, _vp, _vp, _i, _vp, _vp, _ll]),
-    "vamd_op_linear_int8": (_i, [_i, _vp, _vp, _ll, _vp, _ll, _vp, _i, _vp, _vp, _ll, _vp, _i, _i, _i, _vp, _i, _vp, _vp,
-                                 _vp, _ll, _i, _f, _vp, _ll, _i]),
-    "vamd_op_linear_workspace": (_ll, [_i, _i]),
-    "vamd_op_linear_float": (_i, [_i, _vp, _vp, _i, _ll, _vp, _vp, _vp, _ll, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _ll,
-                                  _i, _f, _vp, _ll, _i]),
+    "vamd_op_code_bytes": (C.c_int, [C.c_int]),
+    "vamd_op_quantize_rows": (C.c_int, [C.c_int, C.c_void_p, C.c_char_p]),
+    "vamd_op_frame_map": (C.c_int, [C.c_int, C.c_void_p, C.c_char_p]),
+    "vamd_op_linear_int8": (C.c_int, [C.c_int, C.c_void_p, C.c_char_p]),
+    "vamd_op_linear_workspace": (C.c_longlong, [C.c_int, C.c_int, C.c_int]),
     "vamd_last_error": (C.c_char_p, []),
 }
 for _name, (_res, _args) in _SIGS.items():
@@ -56,10 +53,24 @@ for _name, (_res, _args) in _SIGS.items():
     _fn.restype = _res
     _fn.argtypes = _args
 
+# the structures of vosk_amd_ops.h, packed in one call (a ctypes argument
+# costs 0.1 us, and the smallest operators take three)
+_ROWS = struct.Struct("@5P4q2i").pack
+_MAP = struct.Struct("@7P2q6i16i").pack
+_LINEAR = struct.Struct("@13P6q8if").pack
+
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 PAD = 64          # code rows are a multiple of this many bytes
 MAX_K = 1 << 17   # columns of one tap
 MAX_TAPS = 16
+_ZEROS = (0,) * MAX_TAPS
+_i8, _i32, _f32 = torch.int8, torch.int32, torch.float32
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+def _refuse(what):
+    raise ValueError(what)
 
 
 def _chk(r):
@@ -68,52 +79,63 @@ def _chk(r):
     return r
 
 
-def _want(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _on(t, name):
+    """The GPU that a tensor is on."""
+    if not isinstance(t, torch.Tensor):
+        _refuse(name + " has to be a tensor")
+    d = t.get_device() if t.is_cuda else -1
+    if d < 0:
+        _refuse(name + " has to be on the GPU")
+    return d
+
+
+def _vector(t, name, dtype, n, dev):
+    """The address of a vector of n elements (None: 0)."""
+    if t is None:
+        return 0
+    try:
+        if t.dtype is dtype and t.numel() == n and t.dim() == 1 and t.get_device() == dev and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
+        _refuse("%s has to be a tensor of %s" % (name, dtype))
+    if t.get_device() != dev:
+        _refuse(name + " is on another device")
+    if t.dim() != 1 or t.numel() != n:
+        _refuse("%s has to have %d elements" % (name, n))
+    _refuse(name + " has to be contiguous")
+
+
+def _matrix(t, name, dev):
+    """Address, rows, columns and row stride of a matrix whose rows are contiguous and do not overlap."""
+    if not isinstance(t, torch.Tensor):
+        _refuse(name + " has to be a tensor")
+    if t.get_device() != dev:
+        _refuse(name + " is on another device")
+    if t.dim() != 2:
+        _refuse(name + " has to be a matrix")
+    m, n = t.shape
+    ld, sc = t.stride()
+    if sc != 1 and n > 1 and m:
+        _refuse("rows of %s have to be contiguous" % name)
+    if m <= 1:  # any stride will do
+        ld = -(-n // 16) * 16
+    elif ld < n:
+        _refuse("rows of %s overlap" % name)
+    return t.data_ptr(), m, n, ld
+
+
+def _no_grad(*ts):
+    if torch.is_grad_enabled():
+        for t in ts:
+            if getattr(t, "requires_grad", False):
+                _refuse("a tensor requires a gradient: the 8-bit operators have no backward")
 
 
 def code_bytes(k):
     """Bytes of a code row of k values: k rounded up to a multiple of 64."""
     return _chk(_c.vamd_op_code_bytes(k))
-
-
-def _device(t, name):
-    _want(isinstance(t, torch.Tensor), name + " has to be a tensor")
-    d = t.device
-    _want(d.type == "cuda", name + " has to be on the GPU")
-    return d
-
-
-def _vector(t, name, dtype, n, device):
-    """The pointer of an optional vector of n elements."""
-    if t is None:
-        return None
-    _want(isinstance(t, torch.Tensor) and t.dtype is dtype, "%s has to be a tensor of %s" % (name, dtype))
-    _want(t.device == device, name + " is on another device")
-    _want(t.dim() == 1 and t.shape[0] == n, "%s has to have %d elements" % (name, n))
-    _want(n <= 1 or t.stride(0) == 1, name + " has to be contiguous")
-    _no_grad(t, name)
-    return t.data_ptr()
-
-
-def _no_grad(t, name):
-    _want(not (t.requires_grad and torch.is_grad_enabled()), name + " requires a gradient: the 8-bit operators have none")
-
-
-def _matrix(t, name, device):
-    """(pointer, row stride) of a matrix whose rows are contiguous and do not overlap."""
-    _want(t.device == device, name + " is on another device")
-    _want(t.dim() == 2, name + " has to be a matrix")
-    m, n = t.shape
-    ld, sc = t.stride()
-    _want(n <= 1 or sc == 1, "rows of %s have to be contiguous" % name)
-    _want(m <= 1 or ld >= n, "rows of %s overlap" % name)
-    return t.data_ptr(), (ld if m > 1 else max(ld, n))
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 def quantize_rows(x, codes=None, scales=None, rows=None, count=None):
@@ -134,26 +156,34 @@ def quantize_rows(x, codes=None, scales=None, rows=None, count=None):
     on are skipped; what frame_map leaves behind its last row names old frames,
     so a map's total belongs here.
     """
-    dev = _device(x, "x")
-    _want(x.dtype in _TYPES, "x has to be float32, float16 or bfloat16")
-    _no_grad(x, "x")
-    xp, ldx = _matrix(x, "x", dev)
-    m, k = x.shape
-    _want(1 <= k <= MAX_K, "x has to have 1 to %d columns" % MAX_K)
+    dev = _on(x, "x")
+    t = _TYPES.get(x.dtype)
+    if t is None:
+        _refuse("x has to be float32, float16 or bfloat16")
+    _no_grad(x)
+    xp, m, k, ldx = _matrix(x, "x", dev)
+    if not 1 <= k <= MAX_K:
+        _refuse("x has to have 1 to %d columns" % MAX_K)
     kb = -(-k // PAD) * PAD
-    _want((codes is None) == (scales is None), "codes and scales go together")
-    if codes is None:
-        _want(rows is None, "rows needs codes and scales to write into")
-        codes = torch.empty(m, kb, dtype=torch.int8, device=dev)
-        scales = torch.empty(m, dtype=torch.float32, device=dev)
-    _want(codes.dtype is torch.int8, "codes has to be int8")
-    cp, ldc = _matrix(codes, "codes", dev)
-    c = codes.shape[0]
-    _want(codes.shape[1] >= kb, "codes has to have %d columns" % kb)
-    sp = _vector(scales, "scales", torch.float32, c, dev)
-    rp = _vector(rows, "rows", torch.int32, m, dev)
-    np_ = _vector(count, "count", torch.int32, 1, dev)
-    _chk(_c.vamd_op_quantize_rows(dev.index, _stream(dev), xp, _TYPES[x.dtype], m, k, ldx, rp, np_, c, cp, ldc, sp))
+    if codes is None or scales is None:
+        if codes is not scales:
+            _refuse("codes and scales go together")
+        if rows is not None:
+            _refuse("rows needs codes and scales to write into")
+        codes = torch.empty(m, kb, dtype=_i8, device=x.device)
+        scales = torch.empty(m, dtype=_f32, device=x.device)
+        cp, sp, c, ldc, rp = codes.data_ptr(), scales.data_ptr(), m, kb, 0
+    else:
+        cp, c, cols, ldc = _matrix(codes, "codes", dev)
+        if codes.dtype is not _i8:
+            _refuse("codes has to be int8")
+        if cols < kb:
+            _refuse("codes has to have %d columns" % kb)
+        sp = _vector(scales, "scales", _f32, c, dev)
+        rp = _vector(rows, "rows", _i32, m, dev)
+    if _c.vamd_op_quantize_rows(dev, _raw_stream(dev), _ROWS(xp, rp, _vector(count, "count", _i32, 1, dev), cp, sp,
+                                                             m, ldx, c, ldc, t, k)) < 0:
+        _chk(-1)
     return codes, scales
 
 
@@ -162,12 +192,13 @@ def quantize_weight(w, taps=1):
     frame) as linear_int8 takes it: (codes int8 [N, taps * code_bytes(K)],
     scales float32 [N]), one scale for each output column n, the rounding of
     quantize_rows."""
-    dev = _device(w, "w")
-    _want(w.dim() == 2 and taps >= 1 and w.shape[1] % taps == 0, "w has to be [N, taps * K]")
+    _on(w, "w")
+    if w.dim() != 2 or taps < 1 or w.shape[1] % taps:
+        _refuse("w has to be [N, taps * K]")
     n, k = w.shape[0], w.shape[1] // taps
     codes, scales = quantize_rows(w)
     kb = code_bytes(k)
-    out = torch.zeros(n, taps, kb, dtype=torch.int8, device=dev)
+    out = torch.zeros(n, taps, kb, dtype=_i8, device=w.device)
     out[:, :, :k] = codes[:, :taps * k].view(n, taps, k)
     return out.view(n, taps * kb), scales
 
@@ -191,27 +222,30 @@ def frame_map(lengths, first, table, page, rows, starts=None, offsets=(0,), step
     on are left as they were; rows past cap are not written.
     Returns (starts, rows).
     """
-    dev = _device(lengths, "lengths")
-    _want(lengths.dim() == 1, "lengths has to be a vector")
-    r = lengths.shape[0]
-    lp = _vector(lengths, "lengths", torch.int32, r, dev)
-    fp = _vector(first, "first", torch.int32, r, dev)
-    _want(fp is not None, "first is missing")
-    _want(isinstance(table, torch.Tensor) and table.dtype is torch.int32, "table has to be a tensor of int32")
-    tp, ldt = _matrix(table, "table", dev)
-    _want(table.shape[0] == r, "table has to have a row for each stream")
-    _want(isinstance(rows, torch.Tensor) and rows.dtype is torch.int32, "rows has to be a tensor of int32")
-    taps = len(offsets)
-    _want(1 <= taps <= MAX_TAPS, "1 to %d offsets" % MAX_TAPS)
-    _want(rows.device == dev and rows.dim() == 2 and rows.shape[1] == taps and rows.is_contiguous(),
-          "rows has to be contiguous, [cap, %d], on the device of lengths" % taps)
+    dev = _on(lengths, "lengths")
+    r = lengths.numel()
+    lp = _vector(lengths, "lengths", _i32, r, dev)
+    fp = _vector(first, "first", _i32, r, dev) or (r and _refuse("first is missing"))
+    tp, tr, pages, ldt = _matrix(table, "table", dev)
+    rp, cap, taps, ldr = _matrix(rows, "rows", dev)
+    if table.dtype is not _i32 or rows.dtype is not _i32:
+        _refuse("table and rows have to be int32")
+    if tr != r:
+        _refuse("table has to have a row for each stream")
+    if not 1 <= len(offsets) <= MAX_TAPS:
+        _refuse("1 to %d offsets" % MAX_TAPS)
+    if taps != len(offsets) or (cap > 1 and ldr != taps):
+        _refuse("rows has to be contiguous, [cap, %d]" % len(offsets))
     if starts is None:
-        starts = torch.empty(r + 1, dtype=torch.int32, device=dev)
-    sp = _vector(starts, "starts", torch.int32, r + 1, dev)
-    _chk(_c.vamd_op_frame_map(dev.index, _stream(dev), lp, fp, r, tp, ldt, table.shape[1], page,
-                              (_i * taps)(*offsets), taps, step, _vector(low, "low", torch.int32, r, dev),
-                              _vector(high, "high", torch.int32, r, dev), 1 if clamp else 0, sp, rows.data_ptr(),
-                              rows.shape[0]))
+        starts = torch.empty(r + 1, dtype=_i32, device=lengths.device)
+    try:
+        args = _MAP(lp, fp, tp, _vector(low, "low", _i32, r, dev), _vector(high, "high", _i32, r, dev),
+                    _vector(starts, "starts", _i32, r + 1, dev), rp, ldt, cap, r, pages, page, taps, step, 1 if clamp else 0,
+                    *offsets, *_ZEROS[taps:])
+    except struct.error:
+        _refuse("offsets, page and step have to be 32-bit whole numbers")
+    if _c.vamd_op_frame_map(dev, _raw_stream(dev), args) < 0:
+        _chk(-1)
     return starts, rows
 
 
@@ -236,61 +270,65 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     out [M, N] may be given, else it is made, of `dtype` (float32).  It may be
     residual itself; it must not overlap another input.
     """
-    dev = _device(x, "x")
-    _want(isinstance(weight, torch.Tensor) and weight.dtype is torch.int8, "weight has to be a tensor of int8")
-    wp, ldw = _matrix(weight, "weight", dev)
-    n = weight.shape[0]
-    wsp = _vector(weight_scale, "weight_scale", torch.float32, n, dev)
-    _want(wsp is not None, "weight_scale is missing")
-    xp, ldx = _matrix(x, "x", dev)
-    m, k = x.shape
-    taps, rp = 1, None
-    if x.dtype is torch.int8:
-        _want(scale is not None, "codes need their scales")
-        _want(k % PAD == 0, "codes have to have a multiple of %d columns" % PAD)
-        c = m
-        scp = _vector(scale, "scale", torch.float32, c, dev)
-        if rows is not None:
-            _want(isinstance(rows, torch.Tensor) and rows.dtype is torch.int32 and rows.device == dev and rows.dim() == 2
-                  and rows.is_contiguous(), "rows has to be contiguous int32 [M, J] on the device of x")
-            m, taps = rows.shape
-            _want(1 <= taps <= MAX_TAPS, "rows has to have 1 to %d columns" % MAX_TAPS)
-            rp = rows.data_ptr()
-    else:
-        _want(x.dtype in _TYPES, "x has to be int8 codes, float32, float16 or bfloat16")
-        _want(scale is None and rows is None, "scale and rows belong to codes")
-        _no_grad(x, "x")
-    _want(1 <= k <= MAX_K, "x has to have 1 to %d columns" % MAX_K)
+    dev = _on(x, "x")
+    xp, m, k, ldx = _matrix(x, "x", dev)
+    wp, n, wk, ldw = _matrix(weight, "weight", dev)
+    if weight.dtype is not _i8:
+        _refuse("weight has to be a tensor of int8")
+    if not 1 <= k <= MAX_K:
+        _refuse("x has to have 1 to %d columns" % MAX_K)
     kb = -(-k // PAD) * PAD
-    _want(weight.shape[1] == taps * kb, "weight has to have %d columns" % (taps * kb))
-    bp = _vector(bias, "bias", torch.float32, n, dev)
-    gp, hp = _vector(gain, "gain", torch.float32, n, dev), _vector(shift, "shift", torch.float32, n, dev)
-    _want((gp is None) == (hp is None), "gain and shift go together")
-    qp, ldr, rt = None, 0, 0
+    taps, rp, wsp, c = 1, 0, 0, m
+    if x.dtype is _i8:
+        if scale is None:
+            _refuse("codes need their scales")
+        if k != kb:
+            _refuse("codes have to have a multiple of %d columns" % PAD)
+        xt, sp, cp, lda, xp, ldx = 0, _vector(scale, "scale", _f32, m, dev), xp, ldx, 0, 0
+        if rows is not None:
+            rp, m, taps, ldr = _matrix(rows, "rows", dev)
+            if rows.dtype is not _i32 or (m > 1 and ldr != taps):
+                _refuse("rows has to be contiguous int32 [M, J]")
+            if not 1 <= taps <= MAX_TAPS:
+                _refuse("rows has to have 1 to %d columns" % MAX_TAPS)
+    else:
+        xt = _TYPES.get(x.dtype)
+        if xt is None:
+            _refuse("x has to be int8 codes, float32, float16 or bfloat16")
+        if scale is not None or rows is not None:
+            _refuse("scale and rows belong to codes")
+        sp = cp = lda = 0
+    if wk != taps * kb:
+        _refuse("weight has to have %d columns" % (taps * kb))
+    _no_grad(x, residual, out, bias, gain, shift)
+    qp = ldr = rt = 0
     if residual is not None:
-        _want(isinstance(residual, torch.Tensor) and residual.dtype in _TYPES, "residual has to be a tensor of floats")
-        _want(residual.shape == (m, n), "residual has to be [%d, %d]" % (m, n))
-        _no_grad(residual, "residual")
-        qp, ldr = _matrix(residual, "residual", dev)
-        rt = _TYPES[residual.dtype]
-    cp = _vector(count, "count", torch.int32, 1, dev)
+        qp, rm, rn, ldr = _matrix(residual, "residual", dev)
+        rt = _TYPES.get(residual.dtype)
+        if rt is None or rm != m or rn != n:
+            _refuse("residual has to be [%d, %d] floats" % (m, n))
     if out is None:
-        dtype = dtype or torch.float32
-        _want(dtype in _TYPES, "dtype has to be float32, float16 or bfloat16")
-        out = torch.empty(m, n, dtype=dtype, device=dev)
+        if dtype is None:
+            dtype = _f32
+        if dtype not in _TYPES:
+            _refuse("dtype has to be float32, float16 or bfloat16")
+        out = torch.empty(m, n, dtype=dtype, device=x.device)
         op, ldo = out.data_ptr(), n
     else:
-        _want(isinstance(out, torch.Tensor) and out.dtype in _TYPES and (dtype is None or dtype is out.dtype),
-              "out has to be a tensor of float32, float16 or bfloat16")
-        _want(out.shape == (m, n), "out has to be [%d, %d]" % (m, n))
-        _no_grad(out, "out")
-        op, ldo = _matrix(out, "out", dev)
-    tail = (wp, ldw, wsp, m, n, k, bp, 1 if relu else 0, gp, hp, qp, ldr, rt, residual_scale, op, ldo, _TYPES[out.dtype])
-    if x.dtype is torch.int8:
-        if m == 0 or n == 0:
-            return out
-        _chk(_c.vamd_op_linear_int8(dev.index, _stream(dev), xp, ldx, scp, c, rp, taps, cp, *tail))
-    elif m and n:
-        ws = torch.empty(m * (kb + 4), dtype=torch.int8, device=dev)
-        _chk(_c.vamd_op_linear_float(dev.index, _stream(dev), xp, _TYPES[x.dtype], ldx, ws.data_ptr(), cp, *tail))
+        op, om, on, ldo = _matrix(out, "out", dev)
+        if om != m or on != n or out.dtype not in _TYPES or (dtype is not None and dtype is not out.dtype):
+            _refuse("out has to be [%d, %d] float32, float16 or bfloat16" % (m, n))
+    if m == 0 or n == 0:
+        return out
+    if xp:
+        size = _chk(_c.vamd_op_linear_workspace(m, n, k))
+        if size:
+            ws = torch.empty(size, dtype=_i8, device=x.device)
+            wsp = ws.data_ptr()
+    if _c.vamd_op_linear_int8(dev, _raw_stream(dev), _LINEAR(
+            cp, sp, rp, _vector(count, "count", _i32, 1, dev), xp, wsp, wp,
+            _vector(weight_scale, "weight_scale", _f32, n, dev), _vector(bias, "bias", _f32, n, dev),
+            _vector(gain, "gain", _f32, n, dev), _vector(shift, "shift", _f32, n, dev), qp, op,
+            c, lda, ldx, ldw, ldr, ldo, m, n, k, taps, 1 if relu else 0, xt, rt, _TYPES[out.dtype], residual_scale)) < 0:
+        _chk(-1)
     return out
