@@ -48,6 +48,27 @@ void LaunchQuantizeRows(const QuantizeRows& a, hipStream_t s);
 // t limited to [low[r], high[r]] (clamp: the nearest inside, else -1), -1
 // where the page is not assigned or the ring cannot hold the frame beside
 // the newest that the stream's rows name.
+// Division by a number that is fixed for the launch: the high word of a
+// product with a rounded reciprocal (Granlund and Montgomery, "Division by
+// invariant integers using multiplication", 1994; exact for all 32-bit n).
+struct Divider {
+  uint32_t d = 1, magic = 1;
+  int s1 = 0, s2 = 0;
+  Divider() = default;
+  explicit Divider(uint32_t by) : d(by) {
+    int l = 0;
+    while ((1ull << l) < by) l++;
+    magic = (uint32_t)(((1ull << 32) * ((1ull << l) - by)) / by + 1);
+    s1 = l < 1 ? l : 1;
+    s2 = l > 0 ? l - 1 : 0;
+  }
+  __host__ __device__ uint32_t div(uint32_t n) const {
+    const uint32_t t = (uint32_t)(((uint64_t)magic * n) >> 32);
+    return (t + ((n - t) >> s1)) >> s2;
+  }
+  __host__ __device__ uint32_t mod(uint32_t n) const { return n - div(n) * d; }
+};
+
 struct FrameMap {
   const int* lengths;
   const int* first;
@@ -63,6 +84,7 @@ struct FrameMap {
   long long cap;
   int max_offset;
   int offset[kMaxTaps];
+  Divider by_ring, by_page;
 };
 void LaunchFrameMap(const FrameMap& a, hipStream_t s);
 

@@ -66,54 +66,74 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 }
 
 // 16 bytes of a row, which may lie at any element; past the row: zeros
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 template <int TYPE>
 struct Chunk {
   static constexpr int N = TYPE == kFloat32 ? 4 : 8;  // elements
-  float v[N];
+  uint32_t w[4];
   __device__ __forceinline__ void load(const void* x, long long row0, int e, int k) {
     const char* p = (const char*)x + (row0 + e) * (16 / N);
     if (e + N <= k) {
-      uint32_t w[4];
       __builtin_memcpy(w, p, 16);
-      if constexpr (TYPE == kFloat32) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = __uint_as_float(w[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          if constexpr (TYPE == kBFloat16) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-          } else {
-            v[2 * i] = __half2float(__ushort_as_half((unsigned short)w[i]));
-            v[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16)));
-          }
-        }
-      }
     } else {
 #pragma unroll
-      for (int i = 0; i < N; i++) v[i] = e + i < k ? load_float(x, TYPE, row0 + e + i) : 0.0f;
+      for (int i = 0; i < 4; i++) {
+        w[i] = 0;
+        if constexpr (N == 4) {
+          if (e + i < k) __builtin_memcpy(&w[i], p + 4 * i, 4);
+        } else {
+          if (e + 2 * i < k) w[i] = *(const uint16_t*)(p + 4 * i);
+          if (e + 2 * i + 1 < k) w[i] |= (uint32_t)*(const uint16_t*)(p + 4 * i + 2) << 16;
+        }
+      }
     }
   }
+  // the largest |x| so far: 32-bit patterns, or two 16-bit ones at once
   __device__ __forceinline__ uint32_t top(uint32_t t) const {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const uint32_t u = __float_as_uint(v[i]) & 0x7fffffffu;
-      t = u > t ? u : t;
+    for (int i = 0; i < 4; i++) {
+      if constexpr (N == 4) {
+        t = max(t, w[i] & 0x7fffffffu);
+      } else {
+        t = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, t),
+                                                                   __builtin_bit_cast(ushort2v, w[i] & 0x7fff7fffu)));
+      }
     }
     return t;
   }
+  static __device__ __forceinline__ uint32_t top_bits(uint32_t t) {  // ... as the bits of a 32-bit float
+    if constexpr (N == 4) return t;
+    t = max(t & 0xffffu, t >> 16);
+    if constexpr (TYPE == kBFloat16) return t << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)t)));
+  }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (TYPE == kFloat32) return __uint_as_float(w[i]);
+    if constexpr (TYPE == kBFloat16) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (i & 1 ? 16 : 0))));
+  }
+  // The sum x * (1 / s) + 1.5 * 2^23 is rounded to a whole number, whose low
+  // byte is the code; x - code * s, as in code_of, says whether any of the
+  // chunk's has to be looked at again.
   __device__ __forceinline__ void store(int8_t* to, const RowScale& r) const {
-    uint32_t w[N / 4];
+    uint32_t z[N], out[N / 4];
+    constexpr float kWhole = 12582912.0f;
+    float off = 0.0f;
 #pragma unroll
-    for (int q = 0; q < N / 4; q++) {
-      w[q] = 0;
-      if (!r.zero) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) w[q] |= (uint32_t)(code_of(v[4 * q + i] * r.up, r.s, r.inv) & 0xff) << (8 * i);
-      }
+    for (int i = 0; i < N; i++) {
+      const float v = value(i), y = fmaf(v, r.inv, kWhole);
+      z[i] = __float_as_uint(y);
+      off = fmaxf(off, fabsf(fmaf(-(y - kWhole), r.s, v)));
     }
-    __builtin_memcpy(__builtin_assume_aligned(to, N), w, N);
+    if (off >= 0.5f * r.s || r.up != 1.0f || r.zero) {
+#pragma unroll
+      for (int i = 0; i < N; i++) z[i] = r.zero ? 0u : (uint32_t)code_of(value(i) * r.up, r.s, r.inv);
+    }
+#pragma unroll
+    for (int q = 0; q < N / 4; q++)
+      out[q] = __builtin_amdgcn_perm(z[4 * q + 1], z[4 * q], 0x0c0c0400u) |
+               __builtin_amdgcn_perm(z[4 * q + 3], z[4 * q + 2], 0x04000c0cu);
+    __builtin_memcpy(__builtin_assume_aligned(to, N), out, N);
   }
 };
 
@@ -144,7 +164,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeRows a) {
       top = c[0].top(top);
     }
   }
-  top = wave_max(top);
+  top = wave_max(Chunk<TYPE>::top_bits(top));
   if (TPR > 64) {  // one row a workgroup
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
@@ -190,7 +210,8 @@ void LaunchQuantize(const QuantizeRows& a, unsigned rows4, hipStream_t s) {
 constexpr int kMapThreads = 256, kMapStreams = 4096;
 
 __device__ __forceinline__ unsigned frame_rows(const FrameMap& a, int r) {  // output rows of stream r
-  return ((unsigned)max(a.lengths[r], 0) + (unsigned)a.step - 1u) / (unsigned)a.step;
+  const unsigned n = (unsigned)max(a.lengths[r], 0);
+  return a.step == 1 ? n : (n + (unsigned)a.step - 1u) / (unsigned)a.step;
 }
 
 // exclusive sums over the workgroup; *total: the sum of all
@@ -239,6 +260,7 @@ __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a, int 
   auto at = [](int r) { return r + (r >> 4); };
   long long total;
   if (SUM) {
+#pragma unroll 4
     for (int r = tid; r < a.streams; r += kMapThreads) sums[at(r)] = (int)frame_rows(a, r);
     __syncthreads();
     const int each = (a.streams + kMapThreads - 1) / kMapThreads;
@@ -260,46 +282,86 @@ __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a, int 
     total = a.starts[a.streams];
   }
   auto start = [&](int r) -> long long { return SUM ? sums[at(r)] : a.starts[r]; };
-
-  const long long rows = min(total, a.cap), row0 = (long long)blockIdx.x * per * kMapThreads;
-  const unsigned ring = (unsigned)a.pages * (unsigned)a.page;
-  int r = -1, pr = -1;  // the row's stream; the one that the values below are of
-  long long first = 0, newest = 0, begin = 0, low = INT_MIN, high = INT_MAX;
-  for (int i = 0; i < per; i++) {
-    const long long row = row0 + (long long)i * kMapThreads + tid;
-    if (row >= rows) return;
-    int lo = r < 0 ? 0 : r, hi = a.streams - 1;  // the last stream that begins at or before the row
+  // the last stream from lo on that begins at or before the row, looked for
+  // in steps that double: it is near
+  auto stream_of = [&](int lo, long long row) {
+    int hi = lo, by = 1;
+    while (hi + by < a.streams && start(hi + by) <= row) {
+      hi += by;
+      by *= 2;
+    }
+    lo = hi;
+    hi = min(hi + by, a.streams) - 1;  // (the one after is past the row, or there is none)
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (start(mid) <= row) lo = mid;
       else hi = mid - 1;
     }
-    r = lo;
-    if (r != pr) {
-      pr = r;
-      begin = start(r);
-      first = a.first[r];
-      if (a.low) low = a.low[r];
-      if (a.high) high = a.high[r];
-      newest = first + (long long)a.step * ((long long)frame_rows(a, r) - 1) + a.max_offset;
-      if (a.high) newest = min(newest, high);
+    return lo;
+  };
+
+  const long long rows = min(total, a.cap);
+  const unsigned ring = (unsigned)a.pages * (unsigned)a.page;
+  const int lane = tid & 63;
+  // a wave's rows are neighbours: those of its first and last row bound the lanes' search
+  long long row0 = ((long long)blockIdx.x * per * kMapThreads) + (tid - lane) * per;
+  int r0 = 0;
+  if (row0 < rows) {
+    int hi = a.streams - 1;
+    while (r0 < hi) {
+      const int mid = (r0 + hi + 1) >> 1;
+      if (start(mid) <= row0) r0 = mid;
+      else hi = mid - 1;
     }
-    const long long t0 = first + (long long)a.step * (row - begin);
+  }
+  for (int i = 0; i < per && row0 < rows; i++, row0 += 64) {
+    const long long row = row0 + lane;
+    const int r1 = stream_of(r0, min(row0 + 63, rows - 1));
+    int r = r0, hi = r1;
+    while (r < hi) {
+      const int mid = (r + hi + 1) >> 1;
+      if (start(mid) <= row) r = mid;
+      else hi = mid - 1;
+    }
+    r0 = r1;
+    if (row >= rows) return;
+    const int low = a.low ? a.low[r] : INT_MIN, high = a.high ? a.high[r] : INT_MAX;
+    const long long t0 = a.first[r] + (long long)a.step * (row - start(r));
+    long long newest = a.first[r] + (long long)a.step * ((long long)frame_rows(a, r) - 1) + a.max_offset;
+    if (a.high) newest = min(newest, (long long)high);
+    // the first frame that has a row (no limits: INT_MIN and INT_MAX, past which no frame has one either)
+    const int oldest = (int)min(max(max(newest - ring + 1, (long long)low), (long long)INT_MIN), (long long)INT_MAX);
     const int* const table = a.table + r * a.ldt;
-    for (int j = 0; j < a.taps; j++) {
-      long long t = t0 + a.offset[j];
-      if (a.clamp && a.low) t = max(t, low);
-      if (a.clamp && a.high) t = min(t, high);
-      // (no limits: INT_MIN and INT_MAX, past which no frame has a row either)
-      const bool held = t > newest - ring && t >= low && t <= high;
-      int to = -1;
-      if (held) {
-        const unsigned u = t >= 0 ? (unsigned)t % ring : ring - 1u - (unsigned)(-1 - t) % ring;
-        const unsigned q = u / (unsigned)a.page;
-        const int pg = table[q];
-        if (pg >= 0) to = pg * a.page + (int)(u - q * (unsigned)a.page);
+    for (int j0 = 0; j0 < a.taps; j0 += 4) {
+      int pg[4];
+      unsigned in[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (j0 + j >= a.taps) break;
+        // (times outside 32 bits: clamped just outside, or to the limits)
+        const long long far = t0 + a.offset[j0 + j];
+        int t = (int)min(max(far, (long long)INT_MIN), (long long)INT_MAX);
+        bool held = t == far;
+        if (a.clamp && a.low) {
+          held = held || far < low;
+          t = max(t, low);
+        }
+        if (a.clamp && a.high) {
+          held = held || far > high;
+          t = min(t, high);
+        }
+        held = held && t >= oldest && t <= high;
+        const unsigned sign = (unsigned)(t >> 31);  // t mod ring: of -1 - t, from the other end
+        const unsigned rest = a.by_ring.mod((unsigned)t ^ sign), u = (rest ^ sign) + (sign & ring);
+        const unsigned q = a.pages == 1 ? 0u : a.by_page.div(u);
+        in[j] = u - q * (unsigned)a.page;
+        pg[j] = held ? table[q] : -1;
       }
-      a.rows[row * a.taps + j] = to;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (j0 + j >= a.taps) break;
+        a.rows[row * a.taps + j0 + j] = pg[j] >= 0 ? pg[j] * a.page + (int)in[j] : -1;
+      }
     }
   }
 }
@@ -309,14 +371,14 @@ __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a, int 
 // Tiles of TM rows x TN columns, WM x WN waves, each wave (TM / WM) x (TN / WN)
 // in 32 x 32 blocks of v_mfma_i32_32x32x32_i8 (lane half h holds 16 bytes of
 // its row / column; the accumulator of lane l is column l & 31, rows
-// (i & 3) + 8 * (i >> 2) + 4 * (l >> 5)).  64 bytes of K a step; the tile's
-// rows of A (gathered through the row map) and of W go straight from global
-// memory into an ST-deep ring of LDS buffers, so ST - 1 steps of loads are in
-// flight behind the matrix instructions and one barrier a step is enough.
-// Rows are 64 bytes in LDS, their four 16-byte chunks permuted by
-// (row >> 1) & 3 (on the global side of the load: LDS takes lane after lane),
-// which spreads the eight rows that a 128-byte read covers over all banks.
-constexpr int kStepBytes = 64;
+// (i & 3) + 8 * (i >> 2) + 4 * (l >> 5)).  K goes in parts of 64 bytes, KB
+// parts a step: the tile's rows of A (gathered through the row map) and of W go
+// straight from global memory into a ring of ST LDS buffers, so ST - 1 steps
+// of loads are in flight behind the matrix instructions and one barrier a step
+// is enough.  A part's rows are 64 bytes in LDS, their four 16-byte chunks
+// permuted by (row >> 1) & 3 (on the global side of the load: LDS takes lane
+// after lane), which spreads the rows that a read covers over the banks.
+constexpr int kPartBytes = 64;
 
 // lane l's 16 bytes at p go to LDS byte `to` + 16 * l (to: the same in all lanes).
 // The compiler does not count these loads: WaitStep does.
@@ -419,14 +481,17 @@ __device__ __forceinline__ void finish_16(const LinearInt8& a, float (&v)[16], c
   }
 }
 
-template <int TM, int TN, int WM, int WN, int ST, bool MULTI>
-__global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a, int tiles_m, int tiles_n) {
+// (two waves a SIMD leave 256 registers a wave: the accumulators then stay
+// where the products and the epilogue both use them, without a copy a step)
+template <int TM, int TN, int WM, int WN, int ST, int KB, bool MULTI>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2))) void linear_tile_kernel(LinearInt8 a, int tiles_m, int tiles_n) {
   constexpr int NW = WM * WN, NT = 64 * NW;
   constexpr int BM = TM / WM / 32, BN = TN / WN / 32;  // 32 x 32 blocks of a wave
-  constexpr int LOADS = (TM + TN) / 16 / NW;           // load instructions of a wave a step
+  constexpr int LOADS = (TM + TN) / 16 / NW;           // load instructions of a wave for a part of K
+  constexpr int PART = (TM + TN) * kPartBytes;         // LDS bytes of those
   static_assert((TM + TN) % (16 * NW) == 0, "every wave has the same number of loads");
-  extern __shared__ char smem[];                       // ST x [TM + TN][64], scales [taps][TM], rows [taps][TM]
-  float* const sscale = (float*)(smem + ST * (TM + TN) * kStepBytes);
+  extern __shared__ char smem[];                       // ST x KB x [TM + TN][64], scales [taps][TM], rows [taps][TM]
+  float* const sscale = (float*)(smem + ST * KB * PART);
   int* const srow = (int*)(sscale + a.taps * TM);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -437,47 +502,53 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
   const int t = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (blockIdx.x >> 3);
   const int g0 = t / (GROUP * tiles_n) * GROUP, gm = min(GROUP, tiles_m - g0), gt = t - g0 * tiles_n;
   const int m0 = (g0 + gt % gm) * TM, n0 = gt / gm * TN;
-  const int mrows = a.count ? min(a.m, *a.count) : a.m;
-  if (m0 >= mrows) return;
-
-  for (int i = tid; i < TM * a.taps; i += NT) {
-    const int j = i / TM, m = m0 + i - j * TM;
-    long long row = -1;
-    if (m < mrows) row = a.rows ? a.rows[(long long)m * a.taps + j] : m;
-    const bool there = row >= 0 && row < a.arows;
-    srow[i] = there ? (int)row : 0;  // absent rows read row 0 with scale 0
-    sscale[i] = there ? a.sa[row] : 0.0f;
-  }
-  __syncthreads();
-
-  const int kt = a.k / kStepBytes, steps = kt * a.taps;
-  // this wave's loads: LOADS groups of 16 rows, lane l row l >> 2, chunk slot l & 3
+  // which row each output row reads; those past the count, which is not known yet, as well
+  auto row_of = [&](int m, int tap) {  // -1: adds nothing
+    const int row = m < a.m ? a.rows ? a.rows[(long long)m * a.taps + tap] : m : -1;
+    return row < a.arows ? row : -1;
+  };
+  const int kt = a.k / kPartBytes, parts = kt * a.taps, steps = (parts + KB - 1) / KB;
+  // this wave's loads: LOADS groups of 16 rows (the tile's rows of A, then of
+  // W), lane l row l >> 2, chunk slot l & 3; absent rows read row 0
   const int lrow = lane >> 2, chunk = (lane & 3) ^ ((lrow >> 1) & 3);
   const int8_t* p[LOADS];
-  auto aim = [&](int tap) {
 #pragma unroll
-    for (int g = 0; g < LOADS; g++) {
-      const int r = (wave * LOADS + g) * 16 + lrow;  // of the tile's rows of A, then of W
-      if (r < TM) p[g] = a.a + (long long)srow[tap * TM + r] * a.lda + 16 * chunk;
-      else if (tap == 0) p[g] = a.w + (long long)min(n0 + r - TM, a.n - 1) * a.ldw + 16 * chunk;
-    }
-  };
-  aim(0);
+  for (int g = 0; g < LOADS; g++) {
+    const int r = (wave * LOADS + g) * 16 + lrow;
+    p[g] = (r < TM ? a.a + max(row_of(m0 + r, 0), 0) * a.lda : a.w + (long long)min(n0 + r - TM, a.n - 1) * a.ldw) + 16 * chunk;
+  }
+  if (MULTI) {  // the loads of later taps ask this table
+    for (int i = tid; i < TM * a.taps; i += NT) srow[i] = row_of(m0 + i % TM, i / TM);
+  }
+  const int mrows = a.count ? min(a.m, *a.count) : a.m;
+  if (m0 >= mrows) return;
+  if (MULTI) __syncthreads();
   const uint32_t to = lds_address(smem) + wave * LOADS * 1024;
-  int issued = 0, ik = 0, itap = 0, ibuf = 0;
+  int issued = 0, ipart = 0, ik = 0, itap = 0, ibuf = 0;
   auto issue = [&] {
 #pragma unroll
-    for (int g = 0; g < LOADS; g++) {
-      load_to_lds(p[g], to + ibuf * ((TM + TN) * kStepBytes) + g * 1024);
-      p[g] += kStepBytes;
+    for (int u = 0; u < KB; u++) {
+      const bool last = ik + 1 == kt;  // of the tap
+#pragma unroll
+      for (int g = 0; g < LOADS; g++) load_to_lds(p[g], to + (ibuf * KB + u) * PART + g * 1024);
+      if (++ipart >= parts) continue;  // (a step's parts behind the last one are loads of the last one again)
+      ik = last ? 0 : ik + 1;
+      itap += last;
+#pragma unroll
+      for (int g = 0; g < LOADS; g++) {
+        const int r = (wave * LOADS + g) * 16 + lrow;
+        if (MULTI && last && r < TM) p[g] = a.a + (long long)max(srow[itap * TM + r], 0) * a.lda + 16 * chunk;
+        else p[g] += kPartBytes;
+      }
     }
     issued++;
     ibuf = ibuf + 1 == ST ? 0 : ibuf + 1;
-    if (MULTI && ++ik == kt) {
-      ik = 0;
-      if (++itap < a.taps) aim(itap);
-    }
   };
+  for (int s = 0; s < ST - 1 && s < steps; s++) issue();
+  for (int i = tid; i < TM * a.taps; i += NT) {  // read behind the first of the loop's barriers
+    const int row = MULTI ? srow[i] : row_of(m0 + i, 0);
+    sscale[i] = row >= 0 ? a.sa[row] : 0.0f;
+  }
 
   const int r32 = lane & 31, h = lane >> 5;
   const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
@@ -497,7 +568,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
   };
   float z[16];
   if (BM * BN == 1 && a.residual) residual(0, 0, z);
-  const int f0 = r32 * 64 + (((h) ^ ((r32 >> 1) & 3)) << 4), f1 = r32 * 64 + (((2 + h) ^ ((r32 >> 1) & 3)) << 4);
+  const int f0 = (h ^ ((r32 >> 1) & 3)) << 4, f1 = ((2 + h) ^ ((r32 >> 1) & 3)) << 4;
   intx16 acc[BM][BN];
   float v[MULTI ? BM : 1][MULTI ? BN : 1][16];
 #pragma unroll
@@ -509,7 +580,6 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
         acc[x][y][i] = 0;
         if (MULTI) v[x][y][i] = 0.0f;
       }
-
   auto row_scales = [&](int tap, int x, float (&sc)[16]) {
 #pragma unroll
     for (int q = 0; q < 4; q++) {
@@ -520,45 +590,49 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearInt8 a,
       sc[4 * q + 3] = f.w;
     }
   };
-  for (int s = 0; s < ST - 1 && s < steps; s++) issue();
+
   int buf = 0, k = 0, tap = 0;
   for (int s = 0; s < steps; s++) {
     const int behind = issued - s - 1;  // steps in flight after this one
-    if (behind >= ST - 2) wait_step<(ST - 2) * LOADS>();
-    else wait_last<ST - 3, LOADS>(behind);
+    if (behind >= ST - 2) wait_step<(ST - 2) * KB * LOADS>();
+    else wait_last<ST - 3, KB * LOADS>(behind);
     if (issued < steps) issue();  // into the buffer that every wave left before the barrier
-    const char* const sa = smem + buf * ((TM + TN) * kStepBytes) + wm * 64;
-    const char* const sb = smem + buf * ((TM + TN) * kStepBytes) + (TM + wn) * 64;
 #pragma unroll
-    for (int q = 0; q < 2; q++) {
-      const int f = q ? f1 : f0;
-      intx4 fa[BM], fb[BN];
+    for (int u = 0; u < KB; u++) {
+      if (KB > 1 && s * KB + u >= parts) break;
+      const char* const sa = smem + (buf * KB + u) * PART + (wm + r32) * kPartBytes;
+      const char* const sb = smem + (buf * KB + u) * PART + (TM + wn + r32) * kPartBytes;
 #pragma unroll
-      for (int x = 0; x < BM; x++) fa[x] = *reinterpret_cast<const intx4*>(sa + x * 2048 + f);
+      for (int q = 0; q < 2; q++) {
+        const int f = q ? f1 : f0;
+        intx4 fa[BM], fb[BN];
 #pragma unroll
-      for (int y = 0; y < BN; y++) fb[y] = *reinterpret_cast<const intx4*>(sb + y * 2048 + f);
+        for (int x = 0; x < BM; x++) fa[x] = *reinterpret_cast<const intx4*>(sa + x * 32 * kPartBytes + f);
 #pragma unroll
-      for (int x = 0; x < BM; x++)
+        for (int y = 0; y < BN; y++) fb[y] = *reinterpret_cast<const intx4*>(sb + y * 32 * kPartBytes + f);
 #pragma unroll
-        for (int y = 0; y < BN; y++) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[x], fb[y], acc[x][y], 0, 0, 0);
+        for (int x = 0; x < BM; x++)
+#pragma unroll
+          for (int y = 0; y < BN; y++) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[x], fb[y], acc[x][y], 0, 0, 0);
+      }
+      if (MULTI && ++k == kt) {
+        k = 0;
+#pragma unroll
+        for (int x = 0; x < BM; x++) {
+          float sc[16];
+          row_scales(tap, x, sc);
+#pragma unroll
+          for (int y = 0; y < BN; y++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              v[x][y][i] = fmaf((float)acc[x][y][i], sc[i], v[x][y][i]);
+              acc[x][y][i] = 0;
+            }
+        }
+        tap++;
+      }
     }
     buf = buf + 1 == ST ? 0 : buf + 1;
-    if (MULTI && ++k == kt) {
-      k = 0;
-#pragma unroll
-      for (int x = 0; x < BM; x++) {
-        float sc[16];
-        row_scales(tap, x, sc);
-#pragma unroll
-        for (int y = 0; y < BN; y++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            v[x][y][i] = fmaf((float)acc[x][y][i], sc[i], v[x][y][i]);
-            acc[x][y][i] = 0;
-          }
-      }
-      tap++;
-    }
   }
 #pragma unroll
   for (int x = 0; x < BM; x++) {
@@ -591,7 +665,7 @@ constexpr int kFusedValues = 16384;  // float values (rows x padded columns) tha
 
 template <int TYPE, int RT>  // TYPE < 0: codes; RT blocks of 16 rows
 __global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, QuantizeRows x) {
-  constexpr int R = 16 * RT, AHEAD = 4;
+  constexpr int R = 16 * RT, AHEAD = 8;
   extern __shared__ char smem[];  // codes [R][ldl], partial sums [8][RT][256], scales [taps][R], maxima [R]
   const int kk = a.k * a.taps, ldl = kk + 16;  // 16 bytes on: rows in other banks
   int* const part = (int*)(smem + R * ldl);
@@ -611,6 +685,7 @@ __global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, Q
     w[i] = *reinterpret_cast<const intx4*>(wp + 64 * (s < steps ? s : 0));
   }
 
+  const Column col = column(a, min(n0 + (tid & 15), a.n - 1));  // of the values below
   if constexpr (TYPE >= 0) {
     constexpr int N = Chunk<TYPE < 0 ? 0 : TYPE>::N;
     // all chunks of all rows (LinearFloatFused: HELD a thread) stay in registers
@@ -629,7 +704,7 @@ __global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, Q
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
       if (tid + i * kFewThreads >= all) break;
-      uint32_t top = c[i].top(0);
+      uint32_t top = c[i].top_bits(c[i].top(0));
       if (__all(mm[i] == __builtin_amdgcn_readfirstlane(mm[i]))) {  // one atomic a wave where it holds one row
         top = wave_max(top);
         if (lane == 0) atomicMax(&smax[mm[i]], top);
@@ -722,10 +797,10 @@ __global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, Q
   for (int i = 0; i < EACH; i++) {
     const int t = tid + i * kFewThreads, m = t >> 4, n = n0 + (t & 15);
     if (t >= RT * 256 || m >= mrows || n >= a.n) continue;
-    float y = v[i] * a.sw[n];
-    if (a.bias) y = y + a.bias[n];
+    float y = v[i] * col.sw;
+    if (a.bias) y = y + col.bias;
     if (a.relu) y = y < 0.0f ? 0.0f : y;
-    if (a.gain) y = y * a.gain[n] + a.shift[n];
+    if (a.gain) y = y * col.gain + col.shift;
     if (a.residual) y = a.res_scale * load_float(a.residual, a.res_type, m * a.ldr + n) + y;
     store_float(a.out, a.out_type, m * a.ldo + n, y);
   }
@@ -769,12 +844,12 @@ void LaunchFrameMap(const FrameMap& a, hipStream_t s) {
 
 namespace {
 
-template <int TM, int TN, int WM, int WN, int ST, bool MULTI>
+template <int TM, int TN, int WM, int WN, int ST, int KB, bool MULTI>
 void LaunchTile(const LinearInt8& a, hipStream_t s) {
   const long long tm = ((long long)a.m + TM - 1) / TM, tn = ((long long)a.n + TN - 1) / TN;
   if (tm * tn > INT_MAX) VAMD_ERR("too many tiles for one launch: " << a.m << " x " << a.n);
-  const size_t lds = ST * (TM + TN) * kStepBytes + (size_t)a.taps * TM * 8;
-  auto kernel = linear_tile_kernel<TM, TN, WM, WN, ST, MULTI>;
+  const size_t lds = ST * KB * (TM + TN) * kPartBytes + (size_t)a.taps * TM * 8;
+  auto kernel = linear_tile_kernel<TM, TN, WM, WN, ST, KB, MULTI>;
   AskLds((const void*)kernel, lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, s, a, (int)tm, (int)tn);
 }
@@ -782,6 +857,17 @@ void LaunchTile(const LinearInt8& a, hipStream_t s) {
 }  // namespace
 
 namespace {
+
+// 64 x 64 tiles: the longer K is, the more of it a step (us, 1 / 2 / 4 parts):
+// 4352 x 512 x 96 5.6 / 5.5 / 6.8, 128 x 96 x 1024 6.2 / 5.6 / 5.2; four parts
+// take 64 KB of LDS, which more than two tiles a CU miss: 4352 x 512 x 1024
+// (544 tiles) 9.1 / 8.6 / 10.4.
+template <bool MULTI>
+void LaunchSmallTiles(const LinearInt8& a, long long tiles, hipStream_t s) {
+  if (a.k * a.taps < 512) LaunchTile<64, 64, 2, 2, 3, 1, MULTI>(a, s);
+  else if (tiles <= 512) LaunchTile<64, 64, 2, 2, 2, 4, MULTI>(a, s);
+  else LaunchTile<64, 64, 2, 2, 3, 2, MULTI>(a, s);
+}
 
 size_t FewLds(int m, int k, int taps) {
   const size_t rt = m <= 16 ? 1 : 2;
@@ -845,18 +931,32 @@ void LaunchLinearInt8(const LinearInt8& a, hipStream_t s) {
   // Several taps hold a second set of accumulators, which the larger tiles
   // have no registers for; theirs gain from 128 x 128 at short K too
   //   13056 x 512 x 2 * 96  12.4 / 10.5
+  // Tiles as large as leaves every CU one or more (us in a graph, 64 x 64 / 128 x
+  // 128 / 128 x 256 / 256 x 256 tiles, m x n x k):
+  //   1999 x 777 x 1001    7.3 /  9.6 / 13.0 / 18.6
+  //   4352 x 512 x 1024    8.6 /  9.6 / 12.9 / 18.0
+  //   2048 x 2000 x 512    9.4 /  9.0 / 10.8 / 13.3
+  //   13056 x 4096 x 1024  120 / 84.6 / 80.7 / 87.3
+  //   4352 x 2000 x 4096  67.4 / 58.9 / 63.5 / 54.8
+  //   8192 x 4096 x 4096   232 /  162 /  148 /  132
+  // but short products, which the stores bound, in the smallest:
+  //   4352 x 2000 x 192   10.5 / 13.5 / 12.3 / 12.2
+  // Several taps hold a second set of accumulators, for which the larger
+  // tiles have no registers; theirs gain from 128 x 128 at short K too:
+  //   13056 x 512 x 2 * 96  14.5 / 13.5
   auto tiles = [&](int tm, int tn) { return (((long long)a.m + tm - 1) / tm) * (((long long)a.n + tn - 1) / tn); };
+  const bool wide = tiles(128, 128) >= 256;
   if (a.taps > 1) {
-    if (tiles(128, 128) >= 256) LaunchTile<128, 128, 4, 2, 3, true>(a, s);
-    else LaunchTile<64, 64, 2, 2, 3, true>(a, s);
-  } else if (a.k < 256 || tiles(128, 128) < 256) {
-    LaunchTile<64, 64, 2, 2, 3, false>(a, s);
+    if (wide) LaunchTile<128, 128, 4, 2, 2, 2, true>(a, s);
+    else LaunchSmallTiles<true>(a, tiles(64, 64), s);
+  } else if (!wide || a.k < 256) {
+    LaunchSmallTiles<false>(a, tiles(64, 64), s);
   } else if (a.k >= 2048 && tiles(256, 256) >= 128) {
-    LaunchTile<256, 256, 4, 4, 4, false>(a, s);
+    LaunchTile<256, 256, 4, 4, 2, 2, false>(a, s);
   } else if (tiles(128, 256) >= 256) {
-    LaunchTile<128, 256, 2, 4, 3, false>(a, s);
+    LaunchTile<128, 256, 2, 4, 3, 1, false>(a, s);
   } else {
-    LaunchTile<128, 128, 4, 2, 3, false>(a, s);
+    LaunchTile<128, 128, 4, 2, 2, 2, false>(a, s);
   }
 }
 

@@ -130,7 +130,8 @@ int vamd_op_frame_map(int device, void* stream, const VamdFrameMap* p) {
     Want(p->streams <= 1 || p->ldt >= p->pages, "frame_map: table rows overlap");
     Want(p->cap == 0 || p->rows, "frame_map: null pointer");
     FrameMap a{p->lengths, p->first, p->streams, p->table, p->ldt, p->pages, p->page, p->taps, p->step,
-               p->clamp ? 1 : 0, p->low, p->high, p->starts, p->rows, p->cap, INT_MIN, {}};
+               p->clamp ? 1 : 0, p->low, p->high, p->starts, p->rows, p->cap, INT_MIN, {},
+               Divider((uint32_t)p->pages * (uint32_t)p->page), Divider((uint32_t)p->page)};
     for (int j = 0; j < a.taps; j++) {
       a.offset[j] = p->offsets[j];
       if (a.offset[j] > a.max_offset) a.max_offset = a.offset[j];
