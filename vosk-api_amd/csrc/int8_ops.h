@@ -85,6 +85,8 @@ struct FrameMap {
   int max_offset;
   int offset[kMaxTaps];
   Divider by_ring, by_page;
+  bool far_offsets;               // an offset past +-2^30
+  unsigned offset_at[kMaxTaps];   // offset mod ring, 0 .. ring - 1
 };
 void LaunchFrameMap(const FrameMap& a, hipStream_t s);
 

@@ -77,14 +77,19 @@ struct Chunk {
       __builtin_memcpy(w, p, 16);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        w[i] = 0;
-        if constexpr (N == 4) {
-          if (e + i < k) __builtin_memcpy(&w[i], p + 4 * i, 4);
-        } else {
-          if (e + 2 * i < k) w[i] = *(const uint16_t*)(p + 4 * i);
-          if (e + 2 * i + 1 < k) w[i] |= (uint32_t)*(const uint16_t*)(p + 4 * i + 2) << 16;
+      for (int i = 0; i < 4; i++) w[i] = 0;
+      if (e < k) {  // the row's end: all loads at once, those past it of its last element
+        uint32_t v[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          const char* const q = p + min(i, k - 1 - e) * (16 / N);
+          if constexpr (N == 4) __builtin_memcpy(&v[i], q, 4);
+          else v[i] = *(const uint16_t*)q;
         }
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = e + i < k ? v[i] : 0u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = N == 4 ? v[i] : v[2 * i % N] | v[(2 * i + 1) % N] << 16;
       }
     }
   }
@@ -193,7 +198,9 @@ void LaunchQuantize(const QuantizeRows& a, unsigned rows4, hipStream_t s) {
   const int kp = Int8Padded(a.k);
   // a wave a row as long as it fits its registers; with too few rows to fill
   // the chip so, four waves share the longer ones
-  if (kp <= 64 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 2>), dim3(rows4), dim3(256), 0, s, a);
+  if (kp <= 64 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 1>), dim3(rows4), dim3(256), 0, s, a);
+  else if (kp <= 64 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 2>), dim3(rows4), dim3(256), 0, s, a);
+  else if (kp <= 64 * 4 * N && a.m > 2048) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 4>), dim3(rows4), dim3(256), 0, s, a);
   else if (kp <= 64 * 8 * N && a.m > 2048) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 8>), dim3(rows4), dim3(256), 0, s, a);
   else if (kp <= 256 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 2>), dim3((unsigned)a.m), dim3(256), 0, s, a);
   else if (kp <= 256 * 4 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 4>), dim3((unsigned)a.m), dim3(256), 0, s, a);
@@ -214,64 +221,85 @@ __device__ __forceinline__ unsigned frame_rows(const FrameMap& a, int r) {  // o
   return a.step == 1 ? n : (n + (unsigned)a.step - 1u) / (unsigned)a.step;
 }
 
+// Sums end at 2^32 - 1 instead of wrapping (and at INT_MAX in `starts`).
+__device__ __forceinline__ unsigned add_sat(unsigned a, unsigned b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ int saturated(unsigned v) { return (int)min(v, (unsigned)INT_MAX); }
+
 // exclusive sums over the workgroup; *total: the sum of all
-__device__ __forceinline__ long long block_scan(long long sum, long long* total) {
-  __shared__ long long part[kMapThreads / 64];
+__device__ __forceinline__ unsigned block_scan(unsigned sum, unsigned* total) {
+  __shared__ unsigned part[kMapThreads / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  long long v = sum;
+  unsigned v = sum;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const long long u = __shfl_up(v, o);
-    if (lane >= o) v += u;
+    const unsigned u = __shfl_up(v, o);
+    if (lane >= o) v = add_sat(v, u);
   }
   if (lane == 63) part[wave] = v;
+  v = __shfl_up(v, 1);
+  if (lane == 0) v = 0;
   __syncthreads();
-  long long before = 0, all = 0;
+  unsigned before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kMapThreads / 64; w++) {
-    if (w < wave) before += part[w];
-    all += part[w];
+    if (w < wave) before = add_sat(before, part[w]);
+    all = add_sat(all, part[w]);
   }
   *total = all;
-  return before + v - sum;
+  return add_sat(before, v);
 }
-
-__device__ __forceinline__ int saturated(long long v) { return (int)min(v, (long long)INT_MAX); }
 
 // exclusive sums of the streams' row counts: one workgroup
 __global__ __launch_bounds__(kMapThreads) void frame_starts_kernel(FrameMap a) {
-  const int tid = threadIdx.x, per = (a.streams + kMapThreads - 1) / kMapThreads;
-  const int lo = min((long long)tid * per, (long long)a.streams), hi = min(lo + (long long)per, (long long)a.streams);
-  long long sum = 0, total;
-  for (int r = lo; r < hi; r++) sum += frame_rows(a, r);
-  long long at = block_scan(sum, &total);
+  const int tid = threadIdx.x;
+  const long long per = (a.streams + kMapThreads - 1ll) / kMapThreads;
+  const int lo = (int)min(tid * per, (long long)a.streams), hi = (int)min(lo + per, (long long)a.streams);
+  unsigned sum = 0, total;
+  for (int r = lo; r < hi; r++) sum = add_sat(sum, frame_rows(a, r));
+  unsigned at = block_scan(sum, &total);
   for (int r = lo; r < hi; r++) {
     a.starts[r] = saturated(at);
-    at += frame_rows(a, r);
+    at = add_sat(at, frame_rows(a, r));
   }
   if (tid == 0) a.starts[a.streams] = saturated(total);
 }
 
-template <bool SUM>
-__global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a, int per) {
-  // counts, then starts; a gap every 16 so that a thread's 16 counts lie in other banks than its neighbours'
-  __shared__ int sums[SUM ? kMapStreams + kMapStreams / 16 + 1 : 1];
+// SUM: the workgroup sums the streams itself.  A lane makes ROWS rows, 64
+// apart, of the ROWS * 64 of its wave, their loads in flight together.
+template <bool SUM, int ROWS>
+__global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a) {
+  constexpr int EACH = kMapStreams / kMapThreads;
+  // starts; a gap every EACH so that a thread's lie in other banks than its neighbours'
+  __shared__ int sums[SUM ? kMapStreams + kMapThreads : 1];
   const int tid = threadIdx.x;
-  auto at = [](int r) { return r + (r >> 4); };
-  long long total;
+  auto at = [](int r) { return r + r / EACH; };
+  unsigned total;
   if (SUM) {
-#pragma unroll 4
-    for (int r = tid; r < a.streams; r += kMapThreads) sums[at(r)] = (int)frame_rows(a, r);
+    unsigned n[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      const int r = tid + i * kMapThreads;
+      n[i] = r < a.streams ? frame_rows(a, r) : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; i++) sums[at(tid + i * kMapThreads)] = (int)n[i];
     __syncthreads();
-    const int each = (a.streams + kMapThreads - 1) / kMapThreads;
-    const int lo = min(tid * each, a.streams), hi = min(lo + each, a.streams);
-    long long sum = 0;
-    for (int r = lo; r < hi; r++) sum += (unsigned)sums[at(r)];
-    long long v = block_scan(sum, &total);
-    for (int r = lo; r < hi; r++) {
-      const unsigned n = (unsigned)sums[at(r)];
-      sums[at(r)] = saturated(v);
-      v += n;
+    unsigned sum = 0;
+    const bool any = tid * EACH < a.streams;
+    if (any) {
+#pragma unroll
+      for (int i = 0; i < EACH; i++) {
+        n[i] = (unsigned)sums[tid * (EACH + 1) + i];
+        sum = add_sat(sum, n[i]);
+      }
+    }
+    unsigned v = block_scan(sum, &total);
+    if (any) {
+#pragma unroll
+      for (int i = 0; i < EACH; i++) {
+        sums[tid * (EACH + 1) + i] = saturated(v);
+        v = add_sat(v, n[i]);
+      }
     }
     __syncthreads();
     if (blockIdx.x == 0) {
@@ -281,89 +309,117 @@ __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a, int 
   } else {
     total = a.starts[a.streams];
   }
-  auto start = [&](int r) -> long long { return SUM ? sums[at(r)] : a.starts[r]; };
-  // the last stream from lo on that begins at or before the row, looked for
-  // in steps that double: it is near
-  auto stream_of = [&](int lo, long long row) {
-    int hi = lo, by = 1;
-    while (hi + by < a.streams && start(hi + by) <= row) {
-      hi += by;
-      by *= 2;
+  auto start = [&](int r) { return SUM ? sums[at(r)] : a.starts[r]; };
+  // the last stream that begins at or before a row that is the same in all
+  // lanes: 64 candidates at a time
+  auto wave_stream_of = [&](long long row) {
+    long long span = 64;
+    while (span < a.streams) span *= 64;
+    int base = 0;
+    for (span /= 64; span >= 1; span /= 64) {
+      const long long r = base + (threadIdx.x & 63) * span;
+      base += (int)span * (__popcll(__ballot(r < a.streams && start((int)r) <= row)) - 1);
     }
-    lo = hi;
-    hi = min(hi + by, a.streams) - 1;  // (the one after is past the row, or there is none)
+    return base;
+  };
+  auto stream_of = [&](int lo, int hi, long long row) {  // the last of them that begins at or before the row
     while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
+      const int mid = (int)(((unsigned)lo + (unsigned)hi + 1u) >> 1);
       if (start(mid) <= row) lo = mid;
       else hi = mid - 1;
     }
     return lo;
   };
 
-  const long long rows = min(total, a.cap);
+  const long long rows = min((long long)saturated(total), a.cap);
   const unsigned ring = (unsigned)a.pages * (unsigned)a.page;
   const int lane = tid & 63;
-  // a wave's rows are neighbours: those of its first and last row bound the lanes' search
-  long long row0 = ((long long)blockIdx.x * per * kMapThreads) + (tid - lane) * per;
-  int r0 = 0;
-  if (row0 < rows) {
-    int hi = a.streams - 1;
-    while (r0 < hi) {
-      const int mid = (r0 + hi + 1) >> 1;
-      if (start(mid) <= row0) r0 = mid;
-      else hi = mid - 1;
-    }
+  const long long row0 = ((long long)blockIdx.x * kMapThreads + (tid - lane)) * ROWS;
+  if (row0 >= rows) return;
+  // the wave's rows are neighbours: those of its first and last row bound the lanes' search
+  const int r0 = wave_stream_of(row0), r1 = wave_stream_of(min(row0 + 64 * ROWS, rows) - 1);
+  int r[ROWS], low[ROWS], high[ROWS], first[ROWS];
+  unsigned n[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) r[i] = stream_of(r0, r1, row0 + i * 64 + lane);
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+    first[i] = a.first[r[i]];
+    n[i] = frame_rows(a, r[i]);
+    low[i] = a.low ? a.low[r[i]] : INT_MIN;
+    high[i] = a.high ? a.high[r[i]] : INT_MAX;
   }
-  for (int i = 0; i < per && row0 < rows; i++, row0 += 64) {
-    const long long row = row0 + lane;
-    const int r1 = stream_of(r0, min(row0 + 63, rows - 1));
-    int r = r0, hi = r1;
-    while (r < hi) {
-      const int mid = (r + hi + 1) >> 1;
-      if (start(mid) <= row) r = mid;
-      else hi = mid - 1;
-    }
-    r0 = r1;
-    if (row >= rows) return;
-    const int low = a.low ? a.low[r] : INT_MIN, high = a.high ? a.high[r] : INT_MAX;
-    const long long t0 = a.first[r] + (long long)a.step * (row - start(r));
-    long long newest = a.first[r] + (long long)a.step * ((long long)frame_rows(a, r) - 1) + a.max_offset;
-    if (a.high) newest = min(newest, (long long)high);
+  auto mod_ring = [&](int t) {  // 0 .. ring - 1; of a negative t: of -1 - t, from the other end
+    const unsigned sign = (unsigned)(t >> 31);
+    return (a.by_ring.mod((unsigned)t ^ sign) ^ sign) + (sign & ring);
+  };
+  long long t0[ROWS];
+  int oldest[ROWS];
+  bool far = a.far_offsets;  // some time may be outside 32 bits
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+    t0[i] = first[i] + (long long)a.step * (row0 + i * 64 + lane - start(r[i]));
+    long long newest = first[i] + (long long)a.step * ((long long)n[i] - 1) + a.max_offset;
+    if (a.high) newest = min(newest, (long long)high[i]);
     // the first frame that has a row (no limits: INT_MIN and INT_MAX, past which no frame has one either)
-    const int oldest = (int)min(max(max(newest - ring + 1, (long long)low), (long long)INT_MIN), (long long)INT_MAX);
-    const int* const table = a.table + r * a.ldt;
-    for (int j0 = 0; j0 < a.taps; j0 += 4) {
-      int pg[4];
-      unsigned in[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (j0 + j >= a.taps) break;
-        // (times outside 32 bits: clamped just outside, or to the limits)
-        const long long far = t0 + a.offset[j0 + j];
-        int t = (int)min(max(far, (long long)INT_MIN), (long long)INT_MAX);
-        bool held = t == far;
-        if (a.clamp && a.low) {
-          held = held || far < low;
-          t = max(t, low);
-        }
-        if (a.clamp && a.high) {
-          held = held || far > high;
-          t = min(t, high);
-        }
-        held = held && t >= oldest && t <= high;
-        const unsigned sign = (unsigned)(t >> 31);  // t mod ring: of -1 - t, from the other end
-        const unsigned rest = a.by_ring.mod((unsigned)t ^ sign), u = (rest ^ sign) + (sign & ring);
-        const unsigned q = a.pages == 1 ? 0u : a.by_page.div(u);
-        in[j] = u - q * (unsigned)a.page;
-        pg[j] = held ? table[q] : -1;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (j0 + j >= a.taps) break;
-        a.rows[row * a.taps + j0 + j] = pg[j] >= 0 ? pg[j] * a.page + (int)in[j] : -1;
-      }
-    }
+    oldest[i] = (int)min(max(newest - ring + 1, (long long)low[i]), (long long)INT_MAX);
+    far = far || t0[i] < -(1 << 30) || t0[i] >= (1 << 30);
   }
+  far = __any(far);
+  // places in the ring of the row's time and of the limits, from which those of the taps follow
+  unsigned at0[ROWS], at_low[ROWS], at_high[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+    at0[i] = far ? 0u : mod_ring((int)t0[i]);
+    at_low[i] = a.clamp && a.low ? mod_ring(low[i]) : 0u;
+    at_high[i] = a.clamp && a.high ? mod_ring(high[i]) : 0u;
+  }
+  // a wave's entries are turned in LDS, so that they go out as whole lines
+  extern __shared__ int entries[];  // [waves][ROWS][64][taps]
+  int* const turn = entries + (tid >> 6) * ROWS * 64 * a.taps;
+  for (int j0 = 0; j0 < a.taps; j0 += 4) {
+    int to[ROWS][4];
+#pragma unroll
+    for (int i = 0; i < ROWS; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        to[i][j] = -1;
+        if (j0 + j >= a.taps) break;
+        int t;
+        unsigned u;
+        bool held = true;
+        if (!far) {
+          t = (int)t0[i] + a.offset[j0 + j];
+          u = at0[i] + a.offset_at[j0 + j];
+          u = min(u, u - ring);  // (below the ring, the difference wraps and is larger)
+        } else {
+          const long long wide = t0[i] + a.offset[j0 + j];
+          t = (int)min(max(wide, (long long)INT_MIN), (long long)INT_MAX);
+          held = t == wide || (a.clamp && ((a.low && wide < low[i]) || (a.high && wide > high[i])));
+          u = mod_ring(t);
+        }
+        if (a.clamp && a.low && t < low[i]) {
+          t = low[i];
+          u = at_low[i];
+        }
+        if (a.clamp && a.high && t > high[i]) {
+          t = high[i];
+          u = at_high[i];
+        }
+        held = held && t >= oldest[i] && t <= high[i];
+        const unsigned q = a.pages == 1 ? 0u : a.by_page.div(u);
+        const int pg = held ? a.table[r[i] * a.ldt + q] : -1;
+        if (pg >= 0) to[i][j] = (pg - (int)q) * a.page + (int)u;
+      }
+#pragma unroll
+    for (int i = 0; i < ROWS; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (j0 + j < a.taps) turn[(i * 64 + lane) * a.taps + j0 + j] = to[i][j];
+  }
+  const long long left = (rows - row0) * a.taps;
+  int* const out = a.rows + row0 * a.taps;
+  for (int e = lane; e < ROWS * 64 * a.taps && e < left; e += 64) out[e] = turn[e];
 }
 
 // ---- the product
@@ -830,16 +886,16 @@ void LaunchQuantizeRows(const QuantizeRows& a, hipStream_t s) {
 }
 
 void LaunchFrameMap(const FrameMap& a, hipStream_t s) {
-  // about four workgroups a CU at most: each sums the streams once
-  const long long blocks256 = (a.cap + kMapThreads - 1) / kMapThreads;
-  const int per = (int)((blocks256 + 1023) / 1024 > 0 ? (blocks256 + 1023) / 1024 : 1);
-  const unsigned grid = (unsigned)((blocks256 + per - 1) / per);
-  if (a.streams <= kMapStreams) {
-    hipLaunchKernelGGL(frame_map_kernel<true>, dim3(grid ? grid : 1), dim3(kMapThreads), 0, s, a, per);
-    return;
-  }
-  hipLaunchKernelGGL(frame_starts_kernel, dim3(1), dim3(kMapThreads), 0, s, a);
-  if (grid) hipLaunchKernelGGL(frame_map_kernel<false>, dim3(grid), dim3(kMapThreads), 0, s, a, per);
+  const bool sum = a.streams <= kMapStreams;
+  if (!sum) hipLaunchKernelGGL(frame_starts_kernel, dim3(1), dim3(kMapThreads), 0, s, a);
+  // two rows a lane once there are enough rows for it: then fewer workgroups sum the streams
+  const int each = a.cap > 256 * 1024 && a.taps <= 8 ? 2 : 1;
+  const unsigned grid = (unsigned)((a.cap + each * kMapThreads - 1) / (each * kMapThreads));
+  const unsigned lds = each * kMapThreads * a.taps * sizeof(int);
+  if (sum && each == 1) hipLaunchKernelGGL((frame_map_kernel<true, 1>), dim3(grid ? grid : 1), dim3(kMapThreads), lds, s, a);
+  else if (sum) hipLaunchKernelGGL((frame_map_kernel<true, 2>), dim3(grid), dim3(kMapThreads), lds, s, a);
+  else if (grid && each == 1) hipLaunchKernelGGL((frame_map_kernel<false, 1>), dim3(grid), dim3(kMapThreads), lds, s, a);
+  else if (grid) hipLaunchKernelGGL((frame_map_kernel<false, 2>), dim3(grid), dim3(kMapThreads), lds, s, a);
 }
 
 namespace {

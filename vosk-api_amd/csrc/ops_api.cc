@@ -131,10 +131,13 @@ int vamd_op_frame_map(int device, void* stream, const VamdFrameMap* p) {
     Want(p->cap == 0 || p->rows, "frame_map: null pointer");
     FrameMap a{p->lengths, p->first, p->streams, p->table, p->ldt, p->pages, p->page, p->taps, p->step,
                p->clamp ? 1 : 0, p->low, p->high, p->starts, p->rows, p->cap, INT_MIN, {},
-               Divider((uint32_t)p->pages * (uint32_t)p->page), Divider((uint32_t)p->page)};
+               Divider((uint32_t)p->pages * (uint32_t)p->page), Divider((uint32_t)p->page), false, {}};
+    const long long ring = (long long)p->pages * p->page;
     for (int j = 0; j < a.taps; j++) {
       a.offset[j] = p->offsets[j];
       if (a.offset[j] > a.max_offset) a.max_offset = a.offset[j];
+      a.far_offsets = a.far_offsets || a.offset[j] > (1 << 30) || a.offset[j] < -(1 << 30);
+      a.offset_at[j] = (unsigned)(((long long)a.offset[j] % ring + ring) % ring);
     }
     OnDevice guard(device);
     LaunchFrameMap(a, (hipStream_t)stream);

@@ -90,11 +90,11 @@ def _on(t, name):
 
 
 def _vector(t, name, dtype, n, dev):
-    """The address of a vector of n elements (None: 0)."""
+    """The address of n contiguous elements (None: 0)."""
     if t is None:
         return 0
     try:
-        if t.dtype is dtype and t.numel() == n and t.dim() == 1 and t.get_device() == dev and t.is_contiguous():
+        if t.dtype is dtype and t.numel() == n and t.get_device() == dev and t.is_contiguous():
             return t.data_ptr()
     except AttributeError:
         pass
@@ -102,28 +102,29 @@ def _vector(t, name, dtype, n, dev):
         _refuse("%s has to be a tensor of %s" % (name, dtype))
     if t.get_device() != dev:
         _refuse(name + " is on another device")
-    if t.dim() != 1 or t.numel() != n:
+    if t.numel() != n:
         _refuse("%s has to have %d elements" % (name, n))
     _refuse(name + " has to be contiguous")
 
 
 def _matrix(t, name, dev):
     """Address, rows, columns and row stride of a matrix whose rows are contiguous and do not overlap."""
-    if not isinstance(t, torch.Tensor):
-        _refuse(name + " has to be a tensor")
+    try:
+        m, n = t.shape
+        ld, sc = t.stride()
+        if sc == 1 and ld >= n and m > 1 and t.get_device() == dev:
+            return t.data_ptr(), m, n, ld
+    except (AttributeError, TypeError, ValueError):
+        if not isinstance(t, torch.Tensor):
+            _refuse(name + " has to be a tensor")
+        _refuse(name + " has to be a matrix")
     if t.get_device() != dev:
         _refuse(name + " is on another device")
-    if t.dim() != 2:
-        _refuse(name + " has to be a matrix")
-    m, n = t.shape
-    ld, sc = t.stride()
     if sc != 1 and n > 1 and m:
         _refuse("rows of %s have to be contiguous" % name)
-    if m <= 1:  # any stride will do
-        ld = -(-n // 16) * 16
-    elif ld < n:
+    if m > 1 and ld < n:
         _refuse("rows of %s overlap" % name)
-    return t.data_ptr(), m, n, ld
+    return t.data_ptr(), m, n, ld if m > 1 else -(-n // 16) * 16  # (of one row any stride will do)
 
 
 def _no_grad(*ts):
