@@ -34,14 +34,16 @@ int vamd_op_code_bytes(int k);
  * exactly, so code * scale is within scale / 2 of x.  A row of zeros gets
  * scale 0; a row that holds an Inf or a NaN gets scale NaN and codes 0. */
 typedef struct {
-    const void *x;           /* [m][k] of `type`, rows ldx elements apart */
-    const int *rows;         /* or NULL: row i goes to row rows[i] of codes and scales; an entry outside
-                                their cache_rows rows is skipped, those inside have to be distinct */
+    const void *x;           /* rows of k of `type`, ldx elements apart */
+    const int *rows;         /* or NULL: row i goes to row rows[i * ldrows] of codes and scales; an entry
+                                outside their cache_rows rows is skipped, those inside have to be distinct */
+    const int *from;         /* or NULL: row i is row from[i * ldfrom] of the x_rows rows of x; an entry
+                                outside them is skipped */
     const int *count;        /* or NULL: rows from *count on are skipped (what frame_map leaves behind its
                                 last row names old frames) */
     signed char *codes;      /* rows of vamd_op_code_bytes(k) bytes, ldc apart; 16-byte aligned rows */
     float *scales;
-    long long m, ldx, cache_rows, ldc;
+    long long m, ldx, cache_rows, ldc, ldrows, ldfrom, x_rows;
     int type, k;
 } VamdQuantizeRows;
 int vamd_op_quantize_rows(int device, void *stream, const VamdQuantizeRows *args);
@@ -51,7 +53,10 @@ int vamd_op_quantize_rows(int device, void *stream, const VamdQuantizeRows *args
  * n = ceil(lengths[r] / step) output rows, row i at time first[r] + step * i.
  * Entry j of an output row at time t is the cache row of frame
  * f = t + offsets[j]: with ring = pages * page,
- *   table[r][(f mod ring) / page] * page + f mod page     (mod: 0 .. ring-1)
+ *   table[r][(f mod ring) / page] * page_stride + (f mod page) * frame_stride
+ * (mod: 0 .. ring-1; page_stride = page and frame_stride = 1 for pages of
+ * neighbouring rows, page_stride = 1 and frame_stride = streams for a ring of
+ * one page in which the streams' rows of one time are neighbours).
  * low / high are the first and last frame that a stream has: a frame outside
  * them is replaced by the nearest inside (clamp != 0) or has no row.  An entry
  * is -1 where there is no row: no such frame, a negative page number, a frame
@@ -64,7 +69,7 @@ typedef struct {
     int *starts;             /* [streams + 1]: the streams' first output rows, and last the total */
     int *rows;               /* [cap][taps]; rows from the total on, and those past cap, are not written */
     long long ldt, cap;
-    int streams, pages, page, taps, step, clamp;
+    int streams, pages, page, page_stride, frame_stride, taps, step, clamp;
     int offsets[16];
 } VamdFrameMap;
 int vamd_op_frame_map(int device, void *stream, const VamdFrameMap *args);
@@ -83,7 +88,7 @@ int vamd_op_frame_map(int device, void *stream, const VamdFrameMap *args);
 typedef struct {
     const signed char *codes; /* rows of kb bytes, lda apart; 16-byte aligned rows */
     const float *scale;      /* [cache_rows] */
-    const int *rows;         /* [m][taps], or NULL */
+    const int *rows;         /* [m][taps], rows ldrows entries apart, or NULL */
     const int *count;        /* or NULL: output rows from *count on are left as they were */
     const void *x;           /* [m][k] of x_type, rows ldx elements apart, or NULL */
     void *workspace;         /* 16-byte aligned, this call's alone until it has run */
@@ -93,7 +98,11 @@ typedef struct {
     const float *gain, *shift; /* [n], or both NULL */
     const void *residual;    /* [m][n] of residual_type, rows ldr elements apart, or NULL */
     void *out;               /* [m][n] of out_type, rows ldo apart; residual itself, or overlapping no input */
-    long long cache_rows, lda, ldx, ldw, ldr, ldo;
+    const int *out_to;       /* or NULL: output row i goes to row out_to[i * ldout_to] of the out_rows rows of
+                                out; an entry outside is skipped, those inside have to be distinct */
+    const int *res_from;     /* or NULL: row i's residual is row res_from[i * ldres_from] of the res_rows rows;
+                                an entry outside adds nothing (with either, that matrix is below 2^31 bytes) */
+    long long cache_rows, lda, ldx, ldw, ldr, ldo, ldrows, ldout_to, out_rows, ldres_from, res_rows;
     int m, n, k, taps, relu, x_type, residual_type, out_type;
     float residual_scale;
 } VamdLinearInt8;

@@ -28,18 +28,18 @@ _p, _q, _i, _f = C.c_void_p, C.c_longlong, C.c_int, C.c_float
 
 
 class Rows(C.Structure):
-    _fields_ = [(n, _p) for n in "x rows count codes scales".split()] + [(n, _q) for n in "m ldx cache_rows ldc".split()] + \
+    _fields_ = [(n, _p) for n in "x rows from_ count codes scales".split()] + [(n, _q) for n in "m ldx cache_rows ldc ldrows ldfrom x_rows".split()] + \
         [(n, _i) for n in "type k".split()]
 
 
 class Map(C.Structure):
     _fields_ = [(n, _p) for n in "lengths first table low high starts rows".split()] + [("ldt", _q), ("cap", _q)] + \
-        [(n, _i) for n in "streams pages page taps step clamp".split()] + [("offsets", _i * 16)]
+        [(n, _i) for n in "streams pages page page_stride frame_stride taps step clamp".split()] + [("offsets", _i * 16)]
 
 
 class Linear(C.Structure):
-    _fields_ = [(n, _p) for n in "codes scale rows count x workspace w wscale bias gain shift residual out".split()] + \
-        [(n, _q) for n in "cache_rows lda ldx ldw ldr ldo".split()] + \
+    _fields_ = [(n, _p) for n in "codes scale rows count x workspace w wscale bias gain shift residual out out_to res_from".split()] + \
+        [(n, _q) for n in "cache_rows lda ldx ldw ldr ldo ldrows ldout_to out_rows ldres_from res_rows".split()] + \
         [(n, _i) for n in "m n k taps relu x_type residual_type out_type".split()] + [("residual_scale", _f)]
 
 
@@ -61,7 +61,7 @@ def test_structures_are_laid_out_as_the_bindings_have_them(tmp_path):
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "%s"' % HDR, "int main(void) {"]
     for name, kind in kinds.items():
         lines.append('printf("%%zu ", sizeof(%s));' % name)
-        lines += ['printf("%%zu ", offsetof(%s, %s));' % (name, f) for f, _ in kind._fields_]
+        lines += ['printf("%%zu ", offsetof(%s, %s));' % (name, f.rstrip("_")) for f, _ in kind._fields_]
     (tmp_path / "a.c").write_text("\n".join(lines) + "return 0; }\n")
     subprocess.run(["gcc", str(tmp_path / "a.c"), "-o", str(tmp_path / "a")], check=True)
     got = [int(v) for v in subprocess.run([str(tmp_path / "a")], capture_output=True, text=True, check=True).stdout.split()]
@@ -69,12 +69,12 @@ def test_structures_are_laid_out_as_the_bindings_have_them(tmp_path):
     for kind in kinds.values():
         want += [C.sizeof(kind)] + [getattr(kind, f).offset for f, _ in kind._fields_]
     assert got == want
-    assert len(ops._ROWS(*range(11))) == C.sizeof(Rows)
-    assert len(ops._MAP(*range(31))) == C.sizeof(Map)
-    packed = ops._LINEAR(*range(1, 28), 0.5)
+    assert len(ops._ROWS(*range(15))) == C.sizeof(Rows)
+    assert len(ops._MAP(*range(33))) == C.sizeof(Map)
+    packed = ops._LINEAR(*range(1, 35), 0.5)
     assert C.sizeof(Linear) - 8 < len(packed) <= C.sizeof(Linear)
     back = Linear.from_buffer_copy(packed.ljust(C.sizeof(Linear), b"\0"))
-    assert [getattr(back, f) for f, _ in Linear._fields_] == [*range(1, 28), 0.5]
+    assert [getattr(back, f) for f, _ in Linear._fields_] == [*range(1, 35), 0.5]
 
 
 @pytest.mark.parametrize("k,want", [(1, 64), (64, 64), (65, 128), (1 << 17, 1 << 17), (0, -1), (-3, -1), ((1 << 17) + 1, -1)])
@@ -104,7 +104,7 @@ ROWS = dict(x=P, m=4, k=100, ldx=100, cache_rows=4, codes=P, ldc=128, scales=P)
     (dict(type=3), "element type"), (dict(m=-1), "rows"), (dict(k=0), "k has"), (dict(k=(1 << 17) + 1), "k has"),
     (dict(x=None), "null"), (dict(codes=None), "null"), (dict(scales=None), "null"), (dict(ldx=99), "overlap"),
     (dict(x=P + 2), "aligned"), (dict(codes=P + 8), "16-byte"), (dict(ldc=120), "16-byte"), (dict(ldc=64), "shorter"),
-    (dict(cache_rows=3), "fewer"), (dict(rows=P, cache_rows=-1), "fewer"),
+    (dict(cache_rows=3), "fewer"), (dict(rows=P, cache_rows=-1), "fewer"), (dict(m=1, from_=P, ldx=99), "overlap"), (dict(from_=P, x_rows=-1), "rows"),
 ])
 def test_quantize_rows_refuses(lib, change, what):
     assert _call(lib, "vamd_op_quantize_rows", Rows, **{**ROWS, **change}) < 0
@@ -117,21 +117,21 @@ def test_nothing_to_do_is_no_error(lib):
     assert _call(lib, "vamd_op_linear_int8", Linear, **{**FLOAT, "n": 0}) == 0
 
 
-MAP = dict(lengths=P, first=P, streams=2, table=P, ldt=3, pages=3, page=8, taps=2, step=1, clamp=1, starts=P, rows=P, cap=10)
+MAP = dict(lengths=P, first=P, streams=2, table=P, ldt=3, pages=3, page=8, page_stride=8, frame_stride=1, taps=2, step=1, clamp=1, starts=P, rows=P, cap=10)
 
 
 @pytest.mark.parametrize("change,what", [
     (dict(streams=-1), "sizes"), (dict(cap=-1), "sizes"), (dict(cap=1 << 31), "sizes"), (dict(pages=0), "pages"),
     (dict(page=0), "pages"), (dict(pages=1 << 16, page=1 << 15), "pages"), (dict(taps=0), "offsets"), (dict(taps=17), "offsets"),
     (dict(step=0), "step"), (dict(starts=None), "null"), (dict(lengths=None), "null"),
-    (dict(first=None), "null"), (dict(table=None), "null"), (dict(rows=None), "null"), (dict(ldt=2), "overlap"),
+    (dict(first=None), "null"), (dict(table=None), "null"), (dict(rows=None), "null"), (dict(ldt=2), "overlap"), (dict(page_stride=-1), "strides"), (dict(frame_stride=-2), "strides"),
 ])
 def test_frame_map_refuses(lib, change, what):
     assert _call(lib, "vamd_op_frame_map", Map, **{**MAP, **change}) < 0
     assert what in _err(lib)
 
 
-LINEAR = dict(codes=P, lda=128, scale=P, cache_rows=5, rows=P, taps=2, w=P, ldw=256, wscale=P, m=7, n=9, k=100, residual_scale=1.0,
+LINEAR = dict(codes=P, lda=128, scale=P, cache_rows=5, rows=P, ldrows=2, taps=2, w=P, ldw=256, wscale=P, m=7, n=9, k=100, residual_scale=1.0,
               out=P, ldo=9)
 
 
@@ -146,7 +146,9 @@ LINEAR = dict(codes=P, lda=128, scale=P, cache_rows=5, rows=P, taps=2, w=P, ldw=
     (dict(rows=None), "row map"), (dict(rows=None, taps=1, cache_rows=6), "fewer"), (dict(gain=P), "together"),
     (dict(shift=P), "together"), (dict(ldo=8), "overlap"), (dict(out=P + 2), "aligned"),
     (dict(residual=P, residual_type=5), "residual type"), (dict(residual=P + 2, ldr=9), "residual is not aligned"),
-    (dict(x=P), "without codes"),
+    (dict(x=P), "without codes"), (dict(ldrows=1), "row map overlap"), (dict(out_to=P, out_rows=-1), "sizes"),
+    (dict(out_to=P, out_rows=1 << 26), "2^31"), (dict(residual=P, ldr=9, res_from=P, res_rows=1 << 26), "2^31"),
+    (dict(m=1, out_to=P, out_rows=3, ldo=8), "overlap"), (dict(m=1, residual=P, res_from=P, res_rows=3, ldr=8), "overlap"),
 ])
 def test_linear_int8_refuses(lib, change, what):
     assert _call(lib, "vamd_op_linear_int8", Linear, **{**LINEAR, **change}) < 0

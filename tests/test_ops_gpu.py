@@ -124,6 +124,24 @@ def test_quantize_rows_into_a_cache(ops):
     np.testing.assert_array_equal(scales.cpu().numpy(), want_s)
 
 
+def test_quantize_rows_from_rows(ops):
+    """Rows gathered from a ring and scattered into a cache through columns of one map."""
+    g = _gen(15)
+    x = _randn(g, 300, 96)
+    both = torch.stack([torch.randint(0, 300, (70,), generator=g, device="cuda"), torch.randperm(200, generator=g, device="cuda")[:70]], 1).int()
+    both[3, 0], both[4, 0], both[5, 1] = -1, 300, 200
+    codes = torch.full((200, 128), 9, dtype=torch.int8, device="cuda")
+    scales = torch.full((200,), -1.0, device="cuda")
+    ops.quantize_rows(x, codes, scales, rows=both[:, 1], from_rows=both[:, 0])
+    want_c, want_s = np.full((200, 128), 9, np.int8), np.full(200, -1, np.float32)
+    c, s = ref.codes_of(_np(x))
+    for fr, to in both.tolist():
+        if 0 <= fr < 300 and 0 <= to < 200:
+            want_c[to], want_s[to] = c[fr], s[fr]
+    np.testing.assert_array_equal(codes.cpu().numpy(), want_c)
+    np.testing.assert_array_equal(scales.cpu().numpy(), want_s)
+
+
 @pytest.mark.parametrize("count", [-2, 0, 1, 7, 20, 99])
 def test_quantize_rows_leaves_rows_past_the_count(ops, count):
     x = _randn(_gen(8), 20, 70)
@@ -208,6 +226,29 @@ def test_frame_map_one_limit(ops, only, clamp):
     kw = dict(low=None, high=None)
     kw[only] = limit
     np.testing.assert_array_equal(rows.cpu().numpy(), ref.frame_map(lengths, first, table, 16, (-5, 0, 6), 1, kw["low"], kw["high"], clamp, before)[1])
+
+
+@pytest.mark.parametrize("off", [2**31 - 1, 2**30 + 5, -2**30 - 3, -2**31])
+def test_frame_map_far_offsets(ops, off):
+    """Times and offsets whose sums need more than 32 bits, or nearly."""
+    first = np.array([0, 5, 2**30 - 3, -2**30, 2**31 - 30, -2**31], np.int32)
+    lengths = np.array([4, 7, 9, 3, 11, 5], np.int32)
+    table = np.arange(12, dtype=np.int32).reshape(6, 2)[::-1].copy()
+    before = np.full((39, 2), -9, np.int32)
+    dev = lambda v: torch.from_numpy(v).cuda()  # noqa: E731
+    rows = dev(before)
+    ops.frame_map(dev(lengths), dev(first), dev(table), 37, rows, offsets=(off, -1))
+    np.testing.assert_array_equal(rows.cpu().numpy(), ref.frame_map(lengths, first, table, 37, (off, -1), 1, None, None, True, before)[1])
+
+
+def test_frame_map_of_a_ring_with_streams_side_by_side(ops):
+    """page_stride 1, frame_stride = streams: row (t mod ring) * streams + slot."""
+    lengths, first, slots = [3, 5, 2], [60, -3, 7], [2, 0, 5]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    rows = torch.full((10, 2), -9, dtype=torch.int32, device="cuda")
+    ops.frame_map(i32(lengths), i32(first), i32(slots).view(3, 1), 64, rows, offsets=(0, 3), strides=(1, 6))
+    want = [[((f + i + o) % 64) * 6 + s for o in (0, 3)] for n, f, s in zip(lengths, first, slots) for i in range(n)]
+    assert rows.tolist() == want
 
 
 def test_frame_map_with_less_room_than_rows(ops):
@@ -386,6 +427,35 @@ def test_linear_cache_offsets_past_32_bits(ops):
     _check(ops.linear_int8(codes, w, ws, scale=scales, rows=rows[:5].contiguous()), v[:5], size[:5], 1, "fp32")
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,n,k,taps", [(5, 40, 64, 1), (20, 100, 130, 3), (90, 70, 96, 2), (300, 513, 192, 1), (3000, 2000, 96, 2),
+                                        (2100, 2050, 2100, 1)])
+def test_linear_mapped_rows(ops, m, n, k, taps, t):
+    """Rows read, residual rows and output rows all through one map, as a layer over frame rings has them."""
+    g = _gen(m + n)
+    c, s = ops.quantize_rows(_randn(g, 99, k))
+    w, ws = ops.quantize_weight(_randn(g, n, taps * k) / (taps * k) ** 0.5, taps)
+    res = _randn(g, 80, n).to(TYPES[t])
+    rows = torch.randint(-1, 100, (m, taps + 2), generator=g, device="cuda", dtype=torch.int32)
+    rows[:, taps] = torch.randperm(m + 50, generator=g, device="cuda")[:m].int() - 20    # some outside out
+    rows[:, taps + 1] = torch.randint(-1, 82, (m,), generator=g, device="cuda")          # some outside residual
+    bias = _randn(g, n)
+    out = torch.full((m, n), 7.0, dtype=TYPES[t], device="cuda")
+    count = torch.tensor([m - 2], dtype=torch.int32, device="cuda")
+    ops.linear_int8(c, w, ws, scale=s, rows=rows[:, :taps], count=count, bias=bias, relu=True, residual=res, residual_scale=0.75, out=out,
+                    out_rows=rows[:, taps], residual_rows=rows[:, taps + 1])
+    r = rows.cpu().numpy()[:m - 2]
+    rf = r[:, taps + 1]
+    z = np.where(((rf >= 0) & (rf < 80))[:, None], _np(res)[np.clip(rf, 0, 79)], 0.0)
+    v, size = ref.linear(c.cpu().numpy(), s.cpu().numpy(), r[:, :taps], w.cpu().numpy(), ws.cpu().numpy(), taps, bias=_np(bias), relu=True,
+                         residual=z, residual_scale=0.75)
+    to = r[:, taps]
+    ok = (to >= 0) & (to < m)
+    _check(out[torch.from_numpy(to[ok]).long().cuda()], v[ok], size[ok], taps, t)
+    rest = np.setdiff1d(np.arange(m), to[ok])
+    assert (out[torch.from_numpy(rest).cuda()] == 7.0).all()
+
+
 def test_linear_empty(ops):
     w, ws = ops.quantize_weight(torch.ones(3, 64, device="cuda"))
     assert ops.linear_int8(torch.ones(0, 64, device="cuda"), w, ws).shape == (0, 3)
@@ -413,6 +483,11 @@ def test_refusals(ops):
         (lambda: ops.linear_int8(c, w, ws[:3], scale=s), "elements"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, rows=rows.long()), "int32"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, rows=rows.expand(4, 2)), "contiguous"),
+        (lambda: ops.linear_int8(c, w, ws, scale=s, out_rows=rows[:, 0]), "needs an out"),
+        (lambda: ops.linear_int8(c, w, ws, scale=s, residual_rows=rows[:, 0]), "needs a residual"),
+        (lambda: ops.linear_int8(c, w, ws, scale=s, out=x[:, :8], out_rows=rows[:3, 0]), "elements"),
+        (lambda: ops.quantize_rows(x, from_rows=rows[:, 0]), "codes and scales"),
+        (lambda: ops.quantize_rows(x, c, s, rows=rows[:3, 0], from_rows=rows[:, 0]), "elements"),
         (lambda: ops.linear_int8(x, w, ws, rows=rows), "belong to codes"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, gain=ws), "together"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, bias=ws.cpu()), "another device"),

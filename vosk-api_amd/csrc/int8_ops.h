@@ -31,6 +31,9 @@ struct QuantizeRows {
   int k;
   long long ldx;       // elements
   const int* rows;
+  long long ldrows;    // entries apart
+  const int* from;     // row m is row from[m] of x's `xrows`, skipped outside them (nullptr: m)
+  long long ldfrom, xrows;
   const int* count;    // device: rows from *count on are skipped (or nullptr)
   long long cache_rows;
   int8_t* codes;
@@ -43,7 +46,8 @@ void LaunchQuantizeRows(const QuantizeRows& a, hipStream_t s);
 // new frames from time first[r] on and gives n_r = ceil(lengths[r] / step)
 // output rows, at times first[r] + step * i; output rows are packed stream
 // after stream (starts = exclusive sums of n_r, the total last).  Frame t of
-// stream r lies in cache row table[r][(t mod ring) / page] * page + t mod page,
+// stream r lies in cache row
+//   table[r][(t mod ring) / page] * page_stride + (t mod page) * frame_stride,
 // ring = pages * page.  Entry (row, j) names the row of frame t + offset[j],
 // t limited to [low[r], high[r]] (clamp: the nearest inside, else -1), -1
 // where the page is not assigned or the ring cannot hold the frame beside
@@ -76,6 +80,7 @@ struct FrameMap {
   const int* table;    // [streams][pages], rows ldt apart
   long long ldt;
   int pages, page;
+  int page_stride, frame_stride;
   int taps, step, clamp;
   const int* low;      // [streams] or nullptr
   const int* high;
@@ -103,6 +108,7 @@ struct LinearInt8 {
   const float* sa;
   long long arows;
   const int* rows;
+  long long ldrows;    // entries apart
   int taps;
   const int* count;    // device: output rows from *count on are left as they were (or nullptr)
   const int8_t* w;
@@ -120,6 +126,13 @@ struct LinearInt8 {
   void* out;
   long long ldo;       // elements
   int out_type;
+  // Output row m goes to row out_to[m] of out (of out_rows rows; skipped
+  // outside them), and residual row m is row res_from[m] (adds nothing outside
+  // res_rows); nullptr: m.  Such a matrix is smaller than 2^31 bytes.
+  const int* out_to;
+  long long ldout_to, out_rows;
+  const int* res_from;
+  long long ldres_from, res_rows;
 };
 void LaunchLinearInt8(const LinearInt8& a, hipStream_t s);
 // The product of float rows: x's codes and scales are a's (a workspace, not

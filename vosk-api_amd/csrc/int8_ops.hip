@@ -152,10 +152,14 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeRows a) {
   const int tid = threadIdx.x % TPR;
   const long long m = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
   long long to = -1;
-  if (m < a.m && !(a.count && m >= *a.count)) to = a.rows ? a.rows[m] : m;
-  if (to < 0 || to >= a.cache_rows) return;  // the same in all threads of the row
+  long long from = m;
+  if (m < a.m && !(a.count && m >= *a.count)) {
+    to = a.rows ? a.rows[m * a.ldrows] : m;
+    if (a.from) from = a.from[m * a.ldfrom];
+  }
+  if (to < 0 || to >= a.cache_rows || from < 0 || from >= a.xrows) return;  // the same in all threads of the row
   const int kp = (a.k + kInt8Pad - 1) / kInt8Pad * kInt8Pad;
-  const long long row0 = m * a.ldx;
+  const long long row0 = from * a.ldx;
   Chunk<TYPE> c[NV ? NV : 1];
   uint32_t top = 0;
   if (NV) {
@@ -409,7 +413,7 @@ __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a) {
         held = held && t >= oldest[i] && t <= high[i];
         const unsigned q = a.pages == 1 ? 0u : a.by_page.div(u);
         const int pg = held ? a.table[r[i] * a.ldt + q] : -1;
-        if (pg >= 0) to[i][j] = (pg - (int)q) * a.page + (int)u;
+        if (pg >= 0) to[i][j] = pg * a.page_stride + (int)(u - q * (unsigned)a.page) * a.frame_stride;
       }
 #pragma unroll
     for (int i = 0; i < ROWS; i++)
@@ -478,27 +482,31 @@ struct BlockRows {
                                                (int)min(max((long long)end - first, 0ll) * ldx * size, 32 * ldx * size),
                                                0x00020000)),
         ld((uint32_t)ldx * size) {}
+  // all `rows` rows of a matrix smaller than 2^31 bytes
+  __device__ __forceinline__ BlockRows(const void* p, int size, long long ldx, long long count)
+      : rows(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)(count * ldx * size), 0x00020000)),
+        ld((uint32_t)ldx * size) {}
 };
 template <class F>
-__device__ __forceinline__ void each_16(uint32_t off, uint32_t ld, F f) {
+__device__ __forceinline__ void each_16(const uint32_t (&at)[16], F f) {
 #pragma unroll
-  for (int i = 0; i < 16; i++) f(i, off + ((i & 3) + 8 * (i >> 2)) * ld);
+  for (int i = 0; i < 16; i++) f(i, at[i]);
 }
-__device__ __forceinline__ void load_16(const BlockRows& b, int type, uint32_t off, float (&z)[16]) {
+__device__ __forceinline__ void load_16(const BlockRows& b, int type, const uint32_t (&at)[16], float (&z)[16]) {
   if (type == kFloat32)
-    each_16(off, b.ld, [&](int i, uint32_t o) { z[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b.rows, o, 0, 0)); });
+    each_16(at, [&](int i, uint32_t o) { z[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b.rows, o, 0, 0)); });
   else if (type == kFloat16)
-    each_16(off, b.ld, [&](int i, uint32_t o) { z[i] = __half2float(__ushort_as_half(__builtin_amdgcn_raw_buffer_load_b16(b.rows, o, 0, 0))); });
+    each_16(at, [&](int i, uint32_t o) { z[i] = __half2float(__ushort_as_half(__builtin_amdgcn_raw_buffer_load_b16(b.rows, o, 0, 0))); });
   else
-    each_16(off, b.ld, [&](int i, uint32_t o) { z[i] = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(b.rows, o, 0, 0) << 16); });
+    each_16(at, [&](int i, uint32_t o) { z[i] = __uint_as_float((uint32_t)__builtin_amdgcn_raw_buffer_load_b16(b.rows, o, 0, 0) << 16); });
 }
-__device__ __forceinline__ void store_16(const BlockRows& b, int type, uint32_t off, const float (&v)[16]) {
+__device__ __forceinline__ void store_16(const BlockRows& b, int type, const uint32_t (&at)[16], const float (&v)[16]) {
   if (type == kFloat32)
-    each_16(off, b.ld, [&](int i, uint32_t o) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[i]), b.rows, o, 0, 0); });
+    each_16(at, [&](int i, uint32_t o) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[i]), b.rows, o, 0, 0); });
   else if (type == kFloat16)
-    each_16(off, b.ld, [&](int i, uint32_t o) { __builtin_amdgcn_raw_buffer_store_b16(__half_as_ushort(__float2half(v[i])), b.rows, o, 0, 0); });
+    each_16(at, [&](int i, uint32_t o) { __builtin_amdgcn_raw_buffer_store_b16(__half_as_ushort(__float2half(v[i])), b.rows, o, 0, 0); });
   else
-    each_16(off, b.ld, [&](int i, uint32_t o) { __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (__bf16)v[i]), b.rows, o, 0, 0); });
+    each_16(at, [&](int i, uint32_t o) { __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (__bf16)v[i]), b.rows, o, 0, 0); });
 }
 
 struct Column {  // a column's constants
@@ -546,9 +554,11 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   constexpr int LOADS = (TM + TN) / 16 / NW;           // load instructions of a wave for a part of K
   constexpr int PART = (TM + TN) * kPartBytes;         // LDS bytes of those
   static_assert((TM + TN) % (16 * NW) == 0, "every wave has the same number of loads");
-  extern __shared__ char smem[];                       // ST x KB x [TM + TN][64], scales [taps][TM], rows [taps][TM]
+  extern __shared__ char smem[];                       // ST x KB x [TM + TN][64], scales [taps][TM], row tables
   float* const sscale = (float*)(smem + ST * KB * PART);
   int* const srow = (int*)(sscale + a.taps * TM);
+  uint32_t* const sout = (uint32_t*)(srow + (MULTI ? a.taps * TM : 0));  // mapped rows of out and residual: their bytes
+  uint32_t* const sres = sout + (a.out_to ? TM : 0);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // workgroups b, b + 8, ... run on one XCD: each XCD gets neighbouring tiles
@@ -560,7 +570,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   const int m0 = (g0 + gt % gm) * TM, n0 = gt / gm * TN;
   // which row each output row reads; those past the count, which is not known yet, as well
   auto row_of = [&](int m, int tap) {  // -1: adds nothing
-    const int row = m < a.m ? a.rows ? a.rows[(long long)m * a.taps + tap] : m : -1;
+    const int row = m < a.m ? a.rows ? a.rows[m * a.ldrows + tap] : m : -1;
     return row < a.arows ? row : -1;
   };
   const int kt = a.k / kPartBytes, parts = kt * a.taps, steps = (parts + KB - 1) / KB;
@@ -605,6 +615,17 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
     const int row = MULTI ? srow[i] : row_of(m0 + i, 0);
     sscale[i] = row >= 0 ? a.sa[row] : 0.0f;
   }
+  const int rsize = a.res_type == kFloat32 ? 4 : 2, osize = a.out_type == kFloat32 ? 4 : 2;
+  auto bytes_of = [&](const int* map, long long ld, long long rows, uint32_t row_bytes, int m) {
+    const int row = m < mrows ? map[m * ld] : -1;
+    return row >= 0 && row < rows ? (uint32_t)row * row_bytes : kOutside;
+  };
+  if (a.out_to || a.res_from) {
+    for (int i = tid; i < TM; i += NT) {
+      if (a.out_to) sout[i] = bytes_of(a.out_to, a.ldout_to, a.out_rows, (uint32_t)(a.ldo * osize), m0 + i);
+      if (a.res_from) sres[i] = bytes_of(a.res_from, a.ldres_from, a.res_rows, (uint32_t)(a.ldr * rsize), m0 + i);
+    }
+  }
 
   const int r32 = lane & 31, h = lane >> 5;
   const int wm = wave / WN * (TM / WM), wn = wave % WN * (TN / WN);
@@ -612,18 +633,33 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   Column col[BN];
 #pragma unroll
   for (int y = 0; y < BN; y++) col[y] = column(a, min(n0 + wn + y * 32 + r32, a.n - 1));
-  const int rsize = a.res_type == kFloat32 ? 4 : 2, osize = a.out_type == kFloat32 ? 4 : 2;
-  // a lane's offset in a block's rows
-  auto place = [&](int y, uint32_t ld, int size) {
+  // where a lane's 16 values of a block lie
+  auto place = [&](int x, int y, uint32_t ld, int size, const uint32_t* map, uint32_t (&at)[16]) {
     const int n = n0 + wn + y * 32 + r32;
-    return n < a.n ? 4 * h * ld + (uint32_t)(n * size) : kOutside;
+    const uint32_t col = n < a.n ? (uint32_t)(n * size) : kOutside;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      if (map) {
+        const uint4 f = *reinterpret_cast<const uint4*>(&map[wm + x * 32 + 4 * h + 8 * q]);
+        at[4 * q] = max(f.x, f.x + col);  // (a column and a row that are both outside: no wrap to inside)
+        at[4 * q + 1] = max(f.y, f.y + col);
+        at[4 * q + 2] = max(f.z, f.z + col);
+        at[4 * q + 3] = max(f.w, f.w + col);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) at[4 * q + i] = col + (4 * h + 8 * q + i) * ld;
+      }
+    }
   };
   auto residual = [&](int x, int y, float (&z)[16]) {
-    const BlockRows b(a.residual, rsize, a.ldr, m0 + wm + x * 32, mrows);
-    load_16(b, a.res_type, place(y, b.ld, rsize), z);
+    const BlockRows b = a.res_from ? BlockRows(a.residual, rsize, a.ldr, a.res_rows)
+                                   : BlockRows(a.residual, rsize, a.ldr, m0 + wm + x * 32, mrows);
+    uint32_t at[16];
+    place(x, y, b.ld, rsize, a.res_from ? sres : nullptr, at);
+    load_16(b, a.res_type, at, z);
   };
   float z[16];
-  if (BM * BN == 1 && a.residual) residual(0, 0, z);
+  if (BM * BN == 1 && a.residual && !a.res_from) residual(0, 0, z);
   const int f0 = (h ^ ((r32 >> 1) & 3)) << 4, f1 = ((2 + h) ^ ((r32 >> 1) & 3)) << 4;
   intx16 acc[BM][BN];
   float v[MULTI ? BM : 1][MULTI ? BN : 1][16];
@@ -699,10 +735,13 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
       float w[16];
 #pragma unroll
       for (int i = 0; i < 16; i++) w[i] = MULTI ? v[x][y][i] : fmaf((float)acc[x][y][i], sc[i], 0.0f);
-      if (BM * BN > 1 && a.residual) residual(x, y, z);
+      if ((BM * BN > 1 || a.res_from) && a.residual) residual(x, y, z);
       finish_16(a, w, col[y], z);
-      const BlockRows b(a.out, osize, a.ldo, m0 + wm + x * 32, mrows);
-      store_16(b, a.out_type, place(y, b.ld, osize), w);
+      const BlockRows b = a.out_to ? BlockRows(a.out, osize, a.ldo, a.out_rows)
+                                   : BlockRows(a.out, osize, a.ldo, m0 + wm + x * 32, mrows);
+      uint32_t at[16];
+      place(x, y, b.ld, osize, a.out_to ? sout : nullptr, at);
+      store_16(b, a.out_type, at, w);
     }
   }
 }
@@ -782,7 +821,7 @@ __global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, Q
     const int chunks = a.k / 16, all = mrows * a.taps * chunks;
     for (int i = tid; i < all; i += kFewThreads) {
       const int q = i / chunks, e = (i - q * chunks) * 16, m = q / a.taps, j = q - m * a.taps;
-      long long row = a.rows ? a.rows[q] : m;
+      long long row = a.rows ? a.rows[m * a.ldrows + j] : m;
       const bool there = row >= 0 && row < a.arows;
       if (!there) row = 0;
       *reinterpret_cast<intx4*>(smem + m * ldl + j * a.k + e) = *reinterpret_cast<const intx4*>(a.a + row * a.lda + e);
@@ -857,8 +896,14 @@ __global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, Q
     if (a.bias) y = y + col.bias;
     if (a.relu) y = y < 0.0f ? 0.0f : y;
     if (a.gain) y = y * col.gain + col.shift;
-    if (a.residual) y = a.res_scale * load_float(a.residual, a.res_type, m * a.ldr + n) + y;
-    store_float(a.out, a.out_type, m * a.ldo + n, y);
+    if (a.residual) {
+      const int from = a.res_from ? a.res_from[m * a.ldres_from] : m;
+      const bool there = from >= 0 && from < a.res_rows;
+      const float z = load_float(a.residual, a.res_type, (there ? from : 0) * a.ldr + n);
+      y = a.res_scale * (there ? z : 0.0f) + y;
+    }
+    const int to = a.out_to ? a.out_to[m * a.ldout_to] : m;
+    if (to >= 0 && to < a.out_rows) store_float(a.out, a.out_type, to * a.ldo + n, y);
   }
 }
 
@@ -904,7 +949,7 @@ template <int TM, int TN, int WM, int WN, int ST, int KB, bool MULTI>
 void LaunchTile(const LinearInt8& a, hipStream_t s) {
   const long long tm = ((long long)a.m + TM - 1) / TM, tn = ((long long)a.n + TN - 1) / TN;
   if (tm * tn > INT_MAX) VAMD_ERR("too many tiles for one launch: " << a.m << " x " << a.n);
-  const size_t lds = ST * KB * (TM + TN) * kPartBytes + (size_t)a.taps * TM * 8;
+  const size_t lds = ST * KB * (TM + TN) * kPartBytes + (size_t)TM * 4 * (a.taps * (MULTI ? 2 : 1) + (a.out_to ? 1 : 0) + (a.res_from ? 1 : 0));
   auto kernel = linear_tile_kernel<TM, TN, WM, WN, ST, KB, MULTI>;
   AskLds((const void*)kernel, lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, s, a, (int)tm, (int)tn);

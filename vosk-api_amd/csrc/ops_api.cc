@@ -62,7 +62,8 @@ void CheckRows(const QuantizeRows& a) {
   Want(a.k >= 1 && a.k <= kInt8MaxK, "quantize_rows: k has to be in [1, 131072]");
   if (a.m == 0) return;
   Want(a.x && a.codes && a.scales, "quantize_rows: null pointer");
-  Want(a.m == 1 || a.ldx >= a.k, "quantize_rows: rows of x overlap");
+  Want((a.m == 1 && !a.from) || a.ldx >= a.k, "quantize_rows: rows of x overlap");
+  Want(a.xrows >= 0, "quantize_rows: bad number of rows");
   Want(Aligned(a.x, Bytes(a.type)), "quantize_rows: x is not aligned to its elements");
   Want(Aligned(a.codes, 16) && a.ldc % 16 == 0, "quantize_rows: code rows have to be 16-byte aligned");
   Want(a.ldc >= Int8Padded(a.k), "quantize_rows: code rows are shorter than vamd_op_code_bytes(k)");
@@ -82,13 +83,19 @@ void CheckLinear(const LinearInt8& a) {
   Want(a.rows || a.taps == 1, "linear_int8: more than one tap needs a row map");
   Want(a.rows || a.arows >= a.m, "linear_int8: fewer code rows than output rows");
   Want(!a.gain == !a.shift, "linear_int8: gain and shift go together");
-  Want(a.ldo >= a.n || a.m == 1, "linear_int8: output rows overlap");
-  Want(a.ldo <= kInt8MaxStride || a.m == 1, "linear_int8: rows of out may be 2^23 elements apart at most");
+  Want(!a.rows || a.m == 1 || a.ldrows >= a.taps, "linear_int8: rows of the row map overlap");
+  Want(a.ldo >= a.n || (a.m == 1 && !a.out_to), "linear_int8: output rows overlap");
+  Want(a.out_rows >= 0 && a.res_rows >= 0, "linear_int8: bad sizes");
+  Want(!a.out_to || a.out_rows * a.ldo * Bytes(a.out_type) < (1ll << 31),
+       "linear_int8: out has to be below 2^31 bytes where out_to maps its rows");
+  Want(a.ldo <= kInt8MaxStride || (a.m == 1 && !a.out_to), "linear_int8: rows of out may be 2^23 elements apart at most");
   Want(Aligned(a.out, Bytes(a.out_type)), "linear_int8: out is not aligned to its elements");
   if (a.residual) {
     Want(FloatTypeOk(a.res_type), "linear_int8: unknown residual type");
-    Want(a.ldr >= a.n || a.m == 1, "linear_int8: residual rows overlap");
-    Want(a.ldr <= kInt8MaxStride || a.m == 1, "linear_int8: rows of residual may be 2^23 elements apart at most");
+    Want(a.ldr >= a.n || (a.m == 1 && !a.res_from), "linear_int8: residual rows overlap");
+    Want(!a.res_from || a.res_rows * a.ldr * Bytes(a.res_type) < (1ll << 31),
+         "linear_int8: residual has to be below 2^31 bytes where res_from maps its rows");
+    Want(a.ldr <= kInt8MaxStride || (a.m == 1 && !a.res_from), "linear_int8: rows of residual may be 2^23 elements apart at most");
     Want(Aligned(a.residual, Bytes(a.res_type)), "linear_int8: residual is not aligned to its elements");
   }
 }
@@ -108,8 +115,8 @@ int vamd_op_code_bytes(int k) {
 int vamd_op_quantize_rows(int device, void* stream, const VamdQuantizeRows* p) {
   return Guarded([&] {
     Want(p != nullptr, "quantize_rows: null pointer");
-    const QuantizeRows a{p->x, p->type, p->m, p->k, p->ldx, p->rows, p->count, p->cache_rows,
-                         (int8_t*)p->codes, p->ldc, p->scales};
+    const QuantizeRows a{p->x, p->type, p->m, p->k, p->ldx, p->rows, p->ldrows, p->from, p->ldfrom,
+                         p->from ? p->x_rows : p->m, p->count, p->cache_rows, (int8_t*)p->codes, p->ldc, p->scales};
     CheckRows(a);
     if (a.m == 0) return;
     OnDevice guard(device);
@@ -129,7 +136,9 @@ int vamd_op_frame_map(int device, void* stream, const VamdFrameMap* p) {
     Want(p->streams == 0 || (p->lengths && p->first && p->table), "frame_map: null pointer");
     Want(p->streams <= 1 || p->ldt >= p->pages, "frame_map: table rows overlap");
     Want(p->cap == 0 || p->rows, "frame_map: null pointer");
-    FrameMap a{p->lengths, p->first, p->streams, p->table, p->ldt, p->pages, p->page, p->taps, p->step,
+    Want(p->page_stride >= 0 && p->frame_stride >= 0, "frame_map: bad strides");
+    FrameMap a{p->lengths, p->first, p->streams, p->table, p->ldt, p->pages, p->page,
+               p->page_stride, p->frame_stride, p->taps, p->step,
                p->clamp ? 1 : 0, p->low, p->high, p->starts, p->rows, p->cap, INT_MIN, {},
                Divider((uint32_t)p->pages * (uint32_t)p->page), Divider((uint32_t)p->page), false, {}};
     const long long ring = (long long)p->pages * p->page;
@@ -150,9 +159,11 @@ int vamd_op_linear_int8(int device, void* stream, const VamdLinearInt8* p) {
     Want(p != nullptr, "linear_int8: null pointer");
     Want(p->m >= 0 && p->n >= 0 && p->m <= kInt8MaxRows && p->n <= kInt8MaxCols, "linear_int8: bad sizes");
     Want(p->k >= 1 && p->k <= kInt8MaxK, "linear_int8: k has to be in [1, 131072]");
-    LinearInt8 a{(const int8_t*)p->codes, p->lda, p->scale, p->cache_rows, p->rows, p->taps, p->count,
+    LinearInt8 a{(const int8_t*)p->codes, p->lda, p->scale, p->cache_rows, p->rows, p->ldrows, p->taps, p->count,
                  (const int8_t*)p->w, p->ldw, p->wscale, p->m, p->n, p->k, p->bias, p->gain, p->shift,
-                 p->residual, p->ldr, p->residual_type, p->residual_scale, p->relu ? 1 : 0, p->out, p->ldo, p->out_type};
+                 p->residual, p->ldr, p->residual_type, p->residual_scale, p->relu ? 1 : 0, p->out, p->ldo, p->out_type,
+                 p->out_to, p->ldout_to, p->out_to ? p->out_rows : p->m, p->res_from, p->ldres_from,
+                 p->res_from ? p->res_rows : p->m};
     QuantizeRows q{};
     if (p->x) {
       Want(!p->codes && !p->scale && !p->rows && p->taps == 1, "linear_int8: x comes without codes, scale and rows");
@@ -161,7 +172,8 @@ int vamd_op_linear_int8(int device, void* stream, const VamdLinearInt8* p) {
       a.lda = kb;
       a.sa = (const float*)(a.a + (long long)p->m * kb);
       a.arows = p->m;
-      q = QuantizeRows{p->x, p->x_type, p->m, p->k, p->ldx, nullptr, p->count, p->m, (int8_t*)p->workspace, kb, (float*)a.sa};
+      q = QuantizeRows{p->x, p->x_type, p->m, p->k, p->ldx, nullptr, 0, nullptr, 0, p->m, p->count, p->m,
+                       (int8_t*)p->workspace, kb, (float*)a.sa};
       if (p->m && p->n) {
         if (LinearFloatFused(p->m, kb)) {  // no workspace: the checks below want addresses
           static char none[16] __attribute__((aligned(16)));
@@ -176,7 +188,8 @@ int vamd_op_linear_int8(int device, void* stream, const VamdLinearInt8* p) {
     CheckLinear(a);
     if (a.m == 0 || a.n == 0) return;
     a.k = Int8Padded(a.k);
-    if (a.m == 1) a.ldo = a.ldr = a.n;  // one row: any stride was right
+    if (a.m == 1 && !a.out_to) a.ldo = a.n;  // one row: any stride was right
+    if (a.m == 1 && !a.res_from) a.ldr = a.n;
     OnDevice guard(device);
     if (p->x) LaunchLinearFloat(a, q, (hipStream_t)stream);
     else LaunchLinearInt8(a, (hipStream_t)stream);

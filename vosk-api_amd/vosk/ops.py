@@ -55,9 +55,9 @@ for _name, (_res, _args) in _SIGS.items():
 
 # the structures of vosk_amd_ops.h, packed in one call (a ctypes argument
 # costs 0.1 us, and the smallest operators take three)
-_ROWS = struct.Struct("@5P4q2i").pack
-_MAP = struct.Struct("@7P2q6i16i").pack
-_LINEAR = struct.Struct("@13P6q8if").pack
+_ROWS = struct.Struct("@6P7q2i").pack
+_MAP = struct.Struct("@7P2q8i16i").pack
+_LINEAR = struct.Struct("@15P11q8if").pack
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 PAD = 64          # code rows are a multiple of this many bytes
@@ -127,6 +127,19 @@ def _matrix(t, name, dev):
     return t.data_ptr(), m, n, ld if m > 1 else -(-n // 16) * 16  # (of one row any stride will do)
 
 
+def _ints(t, name, n, dev):
+    """Address and stride of a vector of n int32, any stride (None: 0, 0)."""
+    if t is None:
+        return 0, 0
+    if not isinstance(t, torch.Tensor) or t.dtype is not _i32:
+        _refuse(name + " has to be a tensor of torch.int32")
+    if t.get_device() != dev:
+        _refuse(name + " is on another device")
+    if t.dim() != 1 or t.shape[0] != n:
+        _refuse("%s has to have %d elements" % (name, n))
+    return t.data_ptr(), t.stride(0)
+
+
 def _no_grad(*ts):
     if torch.is_grad_enabled():
         for t in ts:
@@ -139,7 +152,7 @@ def code_bytes(k):
     return _chk(_c.vamd_op_code_bytes(k))
 
 
-def quantize_rows(x, codes=None, scales=None, rows=None, count=None):
+def quantize_rows(x, codes=None, scales=None, rows=None, count=None, from_rows=None):
     """Codes and scales of the rows of x (float32, float16 or bfloat16 [M, K];
     contiguous rows, any row stride):
 
@@ -155,7 +168,9 @@ def quantize_rows(x, codes=None, scales=None, rows=None, count=None):
     to be distinct (frame_map's are, without limits), rows not named are left
     as they were.  count (int32, one element, on the GPU): rows of x from there
     on are skipped; what frame_map leaves behind its last row names old frames,
-    so a map's total belongs here.
+    so a map's total belongs here.  from_rows, int32 [M]: row i is row
+    from_rows[i] of x (skipped outside x), with rows as long; codes and scales
+    are then given.
     """
     dev = _on(x, "x")
     t = _TYPES.get(x.dtype)
@@ -169,11 +184,12 @@ def quantize_rows(x, codes=None, scales=None, rows=None, count=None):
     if codes is None or scales is None:
         if codes is not scales:
             _refuse("codes and scales go together")
-        if rows is not None:
-            _refuse("rows needs codes and scales to write into")
+        if rows is not None or from_rows is not None:
+            _refuse("rows and from_rows need codes and scales to write into")
+        xr = m
         codes = torch.empty(m, kb, dtype=_i8, device=x.device)
         scales = torch.empty(m, dtype=_f32, device=x.device)
-        cp, sp, c, ldc, rp = codes.data_ptr(), scales.data_ptr(), m, kb, 0
+        cp, sp, c, ldc, rp, ldi, fp, ldf = codes.data_ptr(), scales.data_ptr(), m, kb, 0, 0, 0, 0
     else:
         cp, c, cols, ldc = _matrix(codes, "codes", dev)
         if codes.dtype is not _i8:
@@ -181,9 +197,13 @@ def quantize_rows(x, codes=None, scales=None, rows=None, count=None):
         if cols < kb:
             _refuse("codes has to have %d columns" % kb)
         sp = _vector(scales, "scales", _f32, c, dev)
-        rp = _vector(rows, "rows", _i32, m, dev)
-    if _c.vamd_op_quantize_rows(dev, _raw_stream(dev), _ROWS(xp, rp, _vector(count, "count", _i32, 1, dev), cp, sp,
-                                                             m, ldx, c, ldc, t, k)) < 0:
+        xr = m
+        if from_rows is not None:
+            m = from_rows.numel()
+        fp, ldf = _ints(from_rows, "from_rows", m, dev)
+        rp, ldi = _ints(rows, "rows", m, dev)
+    if _c.vamd_op_quantize_rows(dev, _raw_stream(dev), _ROWS(xp, rp, fp, _vector(count, "count", _i32, 1, dev), cp, sp,
+                                                             m, ldx, c, ldc, ldi, ldf, xr, t, k)) < 0:
         _chk(-1)
     return codes, scales
 
@@ -204,7 +224,8 @@ def quantize_weight(w, taps=1):
     return out.view(n, taps * kb), scales
 
 
-def frame_map(lengths, first, table, page, rows, starts=None, offsets=(0,), step=1, low=None, high=None, clamp=True):
+def frame_map(lengths, first, table, page, rows, starts=None, offsets=(0,), step=1, low=None, high=None, clamp=True,
+              strides=None):
     """Which rows of a frame cache the output rows of a step read.
 
     lengths, first: int32 [R], every stream's new frames and the time of the
@@ -221,6 +242,8 @@ def frame_map(lengths, first, table, page, rows, starts=None, offsets=(0,), step
     Entry -1: absent, a negative page number, or a frame the ring cannot hold
     beside the newest one that the stream's rows name.  Rows from the total
     on are left as they were; rows past cap are not written.
+    strides = (page_stride, frame_stride), by default (page, 1): frame t lies in
+    row table[...] * page_stride + (t mod page) * frame_stride.
     Returns (starts, rows).
     """
     dev = _on(lengths, "lengths")
@@ -241,17 +264,18 @@ def frame_map(lengths, first, table, page, rows, starts=None, offsets=(0,), step
         starts = torch.empty(r + 1, dtype=_i32, device=lengths.device)
     try:
         args = _MAP(lp, fp, tp, _vector(low, "low", _i32, r, dev), _vector(high, "high", _i32, r, dev),
-                    _vector(starts, "starts", _i32, r + 1, dev), rp, ldt, cap, r, pages, page, taps, step, 1 if clamp else 0,
+                    _vector(starts, "starts", _i32, r + 1, dev), rp, ldt, cap, r, pages, page, *(strides or (page, 1)), taps, step,
+                    1 if clamp else 0,
                     *offsets, *_ZEROS[taps:])
     except struct.error:
-        _refuse("offsets, page and step have to be 32-bit whole numbers")
+        _refuse("offsets, page, step and strides have to be 32-bit whole numbers")
     if _c.vamd_op_frame_map(dev, _raw_stream(dev), args) < 0:
         _chk(-1)
     return starts, rows
 
 
 def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, bias=None, relu=False, gain=None,
-                shift=None, residual=None, residual_scale=1.0, out=None, dtype=None):
+                shift=None, residual=None, residual_scale=1.0, out=None, dtype=None, out_rows=None, residual_rows=None):
     """Matrix product in 8-bit codes, with a scale for each row and column:
 
       out[i, n] = weight_scale[n] * sum_j scale[r(i, j)] * sum_k x[r(i, j), k] * weight[n, j, k]
@@ -269,7 +293,11 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     are left as they were (or, where the call makes out, have no value).
 
     out [M, N] may be given, else it is made, of `dtype` (float32).  It may be
-    residual itself; it must not overlap another input.
+    residual itself; it must not overlap another input.  out_rows (int32 [M]):
+    output row i goes to row out_rows[i] of a given out [O, N], skipped outside
+    it; entries inside have to be distinct.  residual_rows (int32 [M]): its
+    residual is row residual_rows[i] of residual [R, N], none outside it.  (A
+    matrix with mapped rows is smaller than 2^31 bytes.)
     """
     dev = _on(x, "x")
     xp, m, k, ldx = _matrix(x, "x", dev)
@@ -279,7 +307,7 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     if not 1 <= k <= MAX_K:
         _refuse("x has to have 1 to %d columns" % MAX_K)
     kb = -(-k // PAD) * PAD
-    taps, rp, wsp, c = 1, 0, 0, m
+    taps, rp, ldi, wsp, c = 1, 0, 0, 0, m
     if x.dtype is _i8:
         if scale is None:
             _refuse("codes need their scales")
@@ -287,9 +315,9 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
             _refuse("codes have to have a multiple of %d columns" % PAD)
         xt, sp, cp, lda, xp, ldx = 0, _vector(scale, "scale", _f32, m, dev), xp, ldx, 0, 0
         if rows is not None:
-            rp, m, taps, ldr = _matrix(rows, "rows", dev)
-            if rows.dtype is not _i32 or (m > 1 and ldr != taps):
-                _refuse("rows has to be contiguous int32 [M, J]")
+            rp, m, taps, ldi = _matrix(rows, "rows", dev)
+            if rows.dtype is not _i32:
+                _refuse("rows has to be int32 [M, J]")
             if not 1 <= taps <= MAX_TAPS:
                 _refuse("rows has to have 1 to %d columns" % MAX_TAPS)
     else:
@@ -302,21 +330,34 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     if wk != taps * kb:
         _refuse("weight has to have %d columns" % (taps * kb))
     _no_grad(x, residual, out, bias, gain, shift)
-    qp = ldr = rt = 0
+    qp = ldr = rt = ep = lde = rr = 0
     if residual is not None:
         qp, rm, rn, ldr = _matrix(residual, "residual", dev)
         rt = _TYPES.get(residual.dtype)
+        rr = rm
+        if residual_rows is not None:
+            ep, lde = _ints(residual_rows, "residual_rows", m, dev)
+            rm = m
         if rt is None or rm != m or rn != n:
             _refuse("residual has to be [%d, %d] floats" % (m, n))
+    elif residual_rows is not None:
+        _refuse("residual_rows needs a residual")
+    tp = ldto = 0
     if out is None:
+        if out_rows is not None:
+            _refuse("out_rows needs an out to write into")
         if dtype is None:
             dtype = _f32
         if dtype not in _TYPES:
             _refuse("dtype has to be float32, float16 or bfloat16")
         out = torch.empty(m, n, dtype=dtype, device=x.device)
-        op, ldo = out.data_ptr(), n
+        op, ldo, orows = out.data_ptr(), n, m
     else:
         op, om, on, ldo = _matrix(out, "out", dev)
+        orows = om
+        if out_rows is not None:
+            tp, ldto = _ints(out_rows, "out_rows", m, dev)
+            om = m
         if om != m or on != n or out.dtype not in _TYPES or (dtype is not None and dtype is not out.dtype):
             _refuse("out has to be [%d, %d] float32, float16 or bfloat16" % (m, n))
     if m == 0 or n == 0:
@@ -329,7 +370,7 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     if _c.vamd_op_linear_int8(dev, _raw_stream(dev), _LINEAR(
             cp, sp, rp, _vector(count, "count", _i32, 1, dev), xp, wsp, wp,
             _vector(weight_scale, "weight_scale", _f32, n, dev), _vector(bias, "bias", _f32, n, dev),
-            _vector(gain, "gain", _f32, n, dev), _vector(shift, "shift", _f32, n, dev), qp, op,
-            c, lda, ldx, ldw, ldr, ldo, m, n, k, taps, 1 if relu else 0, xt, rt, _TYPES[out.dtype], residual_scale)) < 0:
+            _vector(gain, "gain", _f32, n, dev), _vector(shift, "shift", _f32, n, dev), qp, op, tp, ep,
+            c, lda, ldx, ldw, ldr, ldo, ldi, ldto, orows, lde, rr, m, n, k, taps, 1 if relu else 0, xt, rt, _TYPES[out.dtype], residual_scale)) < 0:
         _chk(-1)
     return out
