@@ -138,7 +138,9 @@ int vamd_device_count(void);
  *            i; decoder results lag one step, vamd_engine_flush drains),
  *       16 = lattice generation (vamd_stream_lattice),
  *       32 = order-independent token passing (the BatchModel lanes' form)
- *            instead of Kaldi's sequential order (VOSK_AMD_DEC_ORDER overrides). */
+ *            instead of Kaldi's sequential order (VOSK_AMD_DEC_ORDER overrides),
+ *        64 = the acoustic model's affine layers as 8-bit products with a scale
+ *            for each frame and each output (VOSK_AMD_NNET=int8|fp32 overrides). */
 VamdEngine *vamd_engine_new(const char *model_dir, int frames_per_chunk, int max_streams,
                             int flags);
 void vamd_engine_free(VamdEngine *e);
@@ -174,6 +176,10 @@ long long vamd_stream_llh(VamdEngine *e, int stream, float *out, long long cap);
  * copies up to cap floats, returns the count; ivector dim 0 = no i-vector input */
 long long vamd_stream_ivectors(VamdEngine *e, int stream, float *out, long long cap);
 int vamd_engine_ivector_dim(VamdEngine *e);
+/* layers that run as 8-bit products (engine flag 64; 0: none) */
+int vamd_engine_int8_layers(VamdEngine *e);
+/* host-only: which layers those are, and the nodes kept in codes, as text */
+const char *vamd_plan_describe_int8(const char *model_dir, int frames_per_chunk);
 /* state-level lattice of a stream's decoder segment (engine flag 16): call
  * with frame_begin == NULL to build it and get sizes4 = [frames, tokens,
  * links, final costs | overflow << 30], then again with arrays of those sizes

@@ -186,3 +186,28 @@ def test_import_after_vosk_alone_names_the_cause():
     out = subprocess.run(["python3", "-c", code], capture_output=True, text=True, check=True).stdout
     torch_has_its_own = os.path.exists(os.path.join(os.path.dirname(torch.__file__), "lib", "libamdhip64.so"))
     assert ("import torch before vosk" in out) == torch_has_its_own
+
+
+def test_plan_of_the_8_bit_layers(synth_model):
+    """Which layers of the TDNN-F model run as 8-bit products, and through how many maps."""
+    from vosk import engine
+    lines = engine.plan_describe_int8(synth_model, 51).splitlines()
+    assert lines[-1] == "24 products, 5 maps"
+    ops = {ln.split(":")[0]: ln.split(": ", 1)[1] for ln in lines[:-1]}
+    # the spliced bottleneck layer reads two frames of the layer before, the layer after it adds the bypass
+    assert ops["tdnnf2.linear"].startswith("product of tdnn1.dropout x 2 -> codes")
+    assert ops["tdnnf2.noop"].startswith("product of tdnnf2.linear x 2 + 0.75 * tdnn1.dropout -> codes")
+    assert ops["output.affine"].startswith("product of prefinal-chain.batchnorm2 x 1 (")
+    # 32 bits: the layers before and the one that reads the features and the
+    # i-vector, and tdnnf4.linear, whose frames are not evenly spaced
+    assert not {"spec-augment", "delta", "input2", "tdnnf4.linear"} & set(ops)
+    assert ops["tdnn1.dropout"].startswith("-> codes")
+    assert "-> codes" not in ops["tdnnf3.noop"]  # read by tdnnf4.linear and a bypass alone
+    for fpc in (3, 21):
+        assert engine.plan_describe_int8(synth_model, fpc).splitlines()[-1].startswith("24 products")
+
+
+def test_precision_names():
+    from vosk import engine
+    with pytest.raises(ValueError, match="precision"):
+        engine.Engine("nowhere", precision="int4")

@@ -330,6 +330,13 @@ Engine::Engine(std::shared_ptr<const ModelData> md, const EngineConfig& cfg) : m
   cfg_.frames_per_chunk = fpc;
   plan_ = BuildNnetPlan(m.nnet, fpc, fss, m.dcb.acoustic_scale);
   if (LogLevel() > 0) VAMD_LOG(plan_.Describe());
+  if (const char* o = getenv("VOSK_AMD_NNET")) {
+    const std::string v(o);
+    if (v == "int8") cfg_.nnet_int8 = true;
+    else if (v == "fp32") cfg_.nnet_int8 = false;
+    else VAMD_ERR("VOSK_AMD_NNET has to be int8 or fp32, not " << v);
+  }
+  if (cfg_.nnet_int8) int8_ = BuildInt8Plan(plan_);
   for (int pdf : m.tm.tid2pdf)
     if (pdf >= plan_.out_dim) VAMD_ERR("transition model pdf " << pdf << " >= nnet output dim");
 
@@ -361,6 +368,8 @@ Engine::Engine(std::shared_ptr<const ModelData> md, const EngineConfig& cfg) : m
   // the pipelined front end runs one step ahead of the nnet
   ring_ = std::max(ring_, Pow2AtLeast((long long)jobs_per_slot_ * fpc + plan_.left_context +
                                       plan_.right_context + 2 * step_frames + fpc + 16));
+  // the 8-bit layers' maps name the frames of a whole job at once
+  ring_ = std::max(ring_, Pow2AtLeast(int8_.span));
   sample_ring_ = Pow2AtLeast((long long)cfg_.max_step_samples + 2 * L + o.WindowShift() + 64);
   const int S = cfg_.max_slots;
   std::vector<float*> ring_ptrs(plan_.nodes.size());
@@ -566,7 +575,8 @@ Engine::Engine(std::shared_ptr<const ModelData> md, const EngineConfig& cfg) : m
     a.out_ldim = op.out_node >= 0 ? ring_dims[op.out_node] : 0;
     int bk = 64;
     if (op.kind == Op::GEMM) {
-      a.W = Upload(plan_.mats[op.weight].data);
+      const bool product = cfg_.nnet_int8 && int8_.ops[op_args_.size()].product;
+      a.W = product ? nullptr : Upload(plan_.mats[op.weight].data);
       if ((int)op.segs.size() > kMaxSegs) VAMD_ERR("too many input segments in op " << op.name);
       a.nsegs = (int)op.segs.size();
       for (size_t i = 0; i < op.segs.size(); i++) {
@@ -622,6 +632,8 @@ Engine::Engine(std::shared_ptr<const ModelData> md, const EngineConfig& cfg) : m
     op_args_.push_back(a);
     op_bk_.push_back(bk);
   }
+
+  if (cfg_.nnet_int8) BuildInt8(ring_ptrs, vec_ptrs);
 
   // ---- graph: per state {arc_begin, eps_begin, arc_end, final bits}; per arc
   // {nextstate, weight bits, pdf (-1 for epsilon), ilabel}
@@ -831,7 +843,8 @@ Engine::Engine(std::shared_ptr<const ModelData> md, const EngineConfig& cfg) : m
   stage_bytes_ = Align256(sizeof(float) * (size_t)S * cfg_.max_step_samples) +
                  2 * Align256(sizeof(SampleJob) * S) + Align256(sizeof(ResampleJob) * S) +
                  Align256(sizeof(MfccJob) * S) +
-                 Align256(sizeof(DevJob) * max_jobs_) + Align256(sizeof(DecJob) * S) +
+                 Align256(sizeof(DevJob) * max_jobs_) + 2 * Align256(sizeof(int) * max_jobs_) +
+                 Align256(sizeof(DecJob) * S) +
                  Align256(sizeof(IvStreamJob) * S) + Align256(sizeof(IvReq) * max_jobs_) +
                  2 * Align256(sizeof(CmvnJob) * S) +
                  2 * Align256(sizeof(IvFrameBlock) * ((size_t)max_iv_frames_ / kIvFrameBlock + 2 * S)) +
@@ -1472,15 +1485,134 @@ void Engine::FinishDecodeBatch(const DecBatch& b) {
   }
 }
 
+// The 8-bit layers' device side: rings of codes beside the rings of floats (a
+// frame's code row has its float row's index), weights, maps.
+void Engine::BuildInt8(const std::vector<float*>& rings, const std::vector<float*>& vecs) {
+  const int S = cfg_.max_slots, jobs = S * jobs_per_slot_;
+  const long long frames = (long long)ring_ * S;
+  if (frames > INT_MAX) VAMD_ERR("8-bit layers: more than 2^31 ring rows");
+  std::vector<int8_t*> codes(plan_.nodes.size(), nullptr);
+  std::vector<float*> scales(plan_.nodes.size(), nullptr);
+  for (size_t n = 0; n < plan_.nodes.size(); n++) {
+    if (!int8_.coded[n]) continue;
+    const size_t bytes = (size_t)frames * Int8Padded(plan_.nodes[n].dim);
+    codes[n] = (int8_t*)DevAlloc(bytes);
+    scales[n] = (float*)DevAlloc(sizeof(float) * (size_t)frames);
+    HIPCHECK(hipMemset(codes[n], 0, bytes));
+    HIPCHECK(hipMemset(scales[n], 0, sizeof(float) * (size_t)frames));
+  }
+  int* const starts = (int*)DevAlloc(sizeof(int) * ((size_t)jobs + 1));
+  for (const Int8Plan::Map& m : int8_.maps) {
+    FrameMap f{};
+    f.lengths = Upload(std::vector<int>(jobs, m.rows * m.step));
+    f.ldt = 1;
+    f.pages = 1;
+    f.page = ring_;
+    f.page_stride = 1;  // the table holds the jobs' slots
+    f.frame_stride = S;
+    f.taps = (int)m.offsets.size();
+    f.step = m.step;
+    f.starts = starts;
+    f.rows = (int*)DevAlloc(sizeof(int) * (size_t)jobs * m.rows * f.taps);
+    f.per_stream = m.rows;
+    SetOffsets(&f, m.offsets.data());
+    int8_maps_.push_back(f);
+  }
+  int8_args_.resize(plan_.ops.size());
+  int8_codes_.resize(plan_.ops.size());
+  for (size_t i = 0; i < plan_.ops.size(); i++) {
+    const Op& op = plan_.ops[i];
+    const Int8Plan::OpPlan& o = int8_.ops[i];
+    if (!o.product && !o.quantize) continue;
+    const FrameMap& map = int8_maps_[o.map];
+    const int dim = op.out_node >= 0 ? plan_.nodes[op.out_node].dim : op.N;
+    if (o.product) {
+      LinearInt8 l{};
+      l.a = codes[o.node];
+      l.lda = o.k;
+      l.sa = scales[o.node];
+      l.arows = frames;
+      l.rows = map.rows + o.col;
+      l.ldrows = map.taps;
+      l.taps = o.taps;
+      l.w = Upload(o.w);
+      l.ldw = (long long)o.taps * o.k;
+      l.sw = Upload(o.wscale);
+      l.n = op.N;
+      l.k = o.k;
+      l.bias = o.bias >= 0 ? vecs[o.bias] : nullptr;
+      l.gain = o.gain.empty() ? nullptr : Upload(o.gain);
+      l.shift = o.shift.empty() ? nullptr : Upload(o.shift);
+      l.relu = o.relu ? 1 : 0;
+      if (o.res_node >= 0) {
+        l.residual = rings[o.res_node] + o.res_src;
+        l.ldr = plan_.nodes[o.res_node].dim;
+        l.res_type = kFloat32;
+        l.res_scale = o.res_scale;
+        l.res_from = map.rows + o.res_col;
+        l.ldres_from = map.taps;
+        l.res_rows = frames;
+      }
+      l.ldo = dim;
+      l.out_type = kFloat32;
+      if (op.out_node >= 0) {
+        l.out = rings[op.out_node];
+        l.out_to = map.rows + o.out_col;
+        l.ldout_to = map.taps;
+        l.out_rows = frames;
+      }
+      if (frames * std::max(l.ldo, l.ldr) * 4 >= (1ll << 31))
+        VAMD_ERR("8-bit layers: a ring of " << frames << " rows of " << std::max(l.ldo, l.ldr)
+                                            << " floats passes 2^31 bytes (fewer streams an engine)");
+      int8_args_[i] = l;
+    }
+    if (o.quantize) {
+      QuantizeRows q{};
+      q.x = rings[op.out_node];
+      q.type = kFloat32;
+      q.k = dim;
+      q.ldx = dim;
+      q.rows = q.from = map.rows + o.out_col;
+      q.ldrows = q.ldfrom = map.taps;
+      q.xrows = q.cache_rows = frames;
+      q.codes = codes[op.out_node];
+      q.ldc = Int8Padded(dim);
+      q.scales = scales[op.out_node];
+      int8_codes_[i] = q;
+    }
+  }
+}
+
+long long Engine::NnetLaunches() const {
+  long long n = (long long)(plan_.ops.size() + int8_maps_.size());
+  for (const Int8Plan::OpPlan& o : int8_.ops) n += o.quantize;
+  return n;
+}
+
 void Engine::LaunchNnet(const NnetBatch& b, hipStream_t s) {
   if (b.njobs == 0) return;
   const DevJob* dj = (const DevJob*)(d_stage_ + (size_t)b.buf * stage_bytes_ + b.o_dj);
+  for (FrameMap m : int8_maps_) {
+    m.streams = b.njobs;
+    m.first = (const int*)(d_stage_ + (size_t)b.buf * stage_bytes_ + b.o_t);
+    m.table = (const int*)(d_stage_ + (size_t)b.buf * stage_bytes_ + b.o_slot);
+    m.cap = (long long)b.njobs * m.per_stream;
+    LaunchFrameMap(m, s);
+  }
   for (size_t i = 0; i < plan_.ops.size(); i++) {
     NnetOpArgs a = op_args_[i];
     a.M = b.njobs * a.P;
     a.jobs = dj;
     a.llh = d_llh_buf_[b.par];
-    if (plan_.ops[i].kind == Op::GEMM) {
+    if (cfg_.nnet_int8 && int8_.ops[i].product) {
+      LinearInt8 l = int8_args_[i];
+      l.m = a.M;
+      if (plan_.ops[i].out_node < 0) {
+        l.out = a.llh;
+        l.out_rows = a.M;
+      }
+      LaunchLinearInt8(l, s);
+    } else if (plan_.ops[i].kind == Op::GEMM) {
       LaunchNnetGemm(a, op_bk_[i], s);
     } else {
       for (int k = 0; k < a.nparts; k++)
@@ -1488,8 +1620,13 @@ void Engine::LaunchNnet(const NnetBatch& b, hipStream_t s) {
           if (a.instr[j].op == GInstr::PUSH_JOB) a.instr[j].base = d_ivec_buf_[b.par];
       LaunchNnetGather(a, s);
     }
+    if (cfg_.nnet_int8 && int8_.ops[i].quantize) {
+      QuantizeRows q = int8_codes_[i];
+      q.m = a.M;
+      LaunchQuantizeRows(q, s);
+    }
   }
-  counters_.launches += (long long)plan_.ops.size();
+  counters_.launches += NnetLaunches();
 }
 
 // One engine step.  Front end (staging copy, samples, MFCC, i-vectors) of the
@@ -1525,6 +1662,15 @@ void Engine::RunStep(bool allow_pipeline) {
   NnetBatch cur;
   cur.njobs = (int)st_jobs_.size();
   cur.o_dj = put(st_jobs_.data(), sizeof(DevJob) * st_jobs_.size());
+  if (cfg_.nnet_int8) {  // the jobs' times and slots, as the row maps take them
+    std::vector<int> t, slot;
+    for (const DevJob& j : st_jobs_) {
+      t.push_back(j.base_t);
+      slot.push_back(j.slot);
+    }
+    cur.o_t = put(t.data(), sizeof(int) * t.size());
+    cur.o_slot = put(slot.data(), sizeof(int) * slot.size());
+  }
   cur.buf = buf;
   cur.par = par;
   size_t o_ivj = put(st_iv_jobs_.data(), sizeof(IvStreamJob) * st_iv_jobs_.size());
@@ -1621,7 +1767,7 @@ void Engine::RunStep(bool allow_pipeline) {
     times_.ms[0] += a; times_.ms[1] += b; times_.ms[2] += c;
     times_.ms[3] += std::max(t1, std::max(t2, t3));
     times_.launches[0] += lf;
-    times_.launches[1] += nb && nb->njobs ? (long long)plan_.ops.size() : 0;
+    times_.launches[1] += nb && nb->njobs ? NnetLaunches() : 0;
     times_.launches[2] += db && !db->jobs.empty() ? 1 : 0;
     times_.launches[3] += 1;
   }

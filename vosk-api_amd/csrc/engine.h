@@ -26,6 +26,8 @@
 
 #include "engine_dev.h"
 #include "model_io.h"
+#include "int8_ops.h"
+#include "nnet_int8.h"
 #include "nnet_plan.h"
 #include "resample.h"
 #include "lattice.h"
@@ -114,6 +116,9 @@ struct EngineConfig {
   // deterministic form of the reference's batch CudaDecoder, BatchModel's
   // default); env VOSK_AMD_DEC_ORDER=kaldi|parallel overrides
   bool kaldi_order = true;
+  // the acoustic model's affine layers as 8-bit products (nnet_int8.h) instead
+  // of 32-bit ones; env VOSK_AMD_NNET=int8|fp32 overrides
+  bool nnet_int8 = false;
 };
 
 // HIP-event times accumulated on the engine stream (time_kernels).
@@ -377,6 +382,9 @@ class Engine {
   bool Step(const std::vector<int>& slots, bool allow_pipeline = true);
   void SetStepSamples(int n) { cfg_.max_step_samples = n; }
   const StageTimes& stage_times() const { return times_; }
+  // layers that run as 8-bit products (0: a 32-bit engine)
+  long long NnetLaunches() const;  // of one pass
+  int Int8Layers() const { return cfg_.nnet_int8 ? int8_.products : 0; }
   bool kaldi_order() const { return dec_.kaldi != 0; }  // the decoder's token-passing order
   void ResetStageTimes() { times_ = StageTimes(); }
   void InputFinished(int slot);
@@ -545,7 +553,7 @@ class Engine {
   };
   struct NnetBatch {  // one nnet pass: chunk jobs staged in one staging buffer
     int njobs = 0;
-    size_t o_dj = 0;
+    size_t o_dj = 0, o_t = 0, o_slot = 0;
     int buf = 0;
     int par = 0;  // LLH / i-vector buffer
     DecBatch dec;
@@ -553,6 +561,7 @@ class Engine {
   bool BuildStep(const std::vector<int>& slots);
   void RunStep(bool allow_pipeline = true);
   void LaunchNnet(const NnetBatch& b, hipStream_t s);
+  void BuildInt8(const std::vector<float*>& rings, const std::vector<float*>& vecs);
   void LaunchDecodeBatch(const DecBatch& b, hipStream_t s);
   void FinishDecodeBatch(const DecBatch& b);
   void DrainOnce();  // pipeline tail: the pending nnet and decoder passes
@@ -585,6 +594,10 @@ class Engine {
   size_t dev_bytes_ = 0;  // DevAlloc total (logged at construction)
   long long arena_hwm_ = 0, links_hwm_ = 0;  // MemoryStats
   std::vector<NnetOpArgs> op_args_;
+  Int8Plan int8_;                        // nnet_int8: empty otherwise
+  std::vector<LinearInt8> int8_args_;    // per op (products)
+  std::vector<QuantizeRows> int8_codes_; // per op (quantised rows)
+  std::vector<FrameMap> int8_maps_;
   std::vector<int> op_bk_;
   float** d_ring_ptrs_ = nullptr;
   int* d_ring_dims_ = nullptr;

@@ -90,9 +90,12 @@ struct FrameMap {
   int max_offset;
   int offset[kMaxTaps];
   Divider by_ring, by_page;
+  int per_stream;                 // (the engine's: output rows of each stream)
   bool far_offsets;               // an offset past +-2^30
   unsigned offset_at[kMaxTaps];   // offset mod ring, 0 .. ring - 1
 };
+// Sets the a->taps offsets and what follows from them and from the pages.
+void SetOffsets(FrameMap* a, const int* offsets);
 void LaunchFrameMap(const FrameMap& a, hipStream_t s);
 
 // out[m][n] = epi(sw[n] * sum_j sa[r(m,j)] * sum_k a[r(m,j)][k] * w[n][j * K + k])

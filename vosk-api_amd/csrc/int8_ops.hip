@@ -930,6 +930,20 @@ void LaunchQuantizeRows(const QuantizeRows& a, hipStream_t s) {
   else LaunchQuantize<kBFloat16>(a, rows4, s);
 }
 
+void SetOffsets(FrameMap* a, const int* offsets) {
+  const long long ring = (long long)a->pages * a->page;
+  a->by_ring = Divider((uint32_t)ring);
+  a->by_page = Divider((uint32_t)a->page);
+  a->max_offset = INT_MIN;
+  a->far_offsets = false;
+  for (int j = 0; j < a->taps; j++) {
+    a->offset[j] = offsets[j];
+    a->max_offset = offsets[j] > a->max_offset ? offsets[j] : a->max_offset;
+    a->far_offsets = a->far_offsets || offsets[j] > (1 << 30) || offsets[j] < -(1 << 30);
+    a->offset_at[j] = (unsigned)(((long long)offsets[j] % ring + ring) % ring);
+  }
+}
+
 void LaunchFrameMap(const FrameMap& a, hipStream_t s) {
   const bool sum = a.streams <= kMapStreams;
   if (!sum) hipLaunchKernelGGL(frame_starts_kernel, dim3(1), dim3(kMapThreads), 0, s, a);

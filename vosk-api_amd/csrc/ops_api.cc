@@ -137,17 +137,25 @@ int vamd_op_frame_map(int device, void* stream, const VamdFrameMap* p) {
     Want(p->streams <= 1 || p->ldt >= p->pages, "frame_map: table rows overlap");
     Want(p->cap == 0 || p->rows, "frame_map: null pointer");
     Want(p->page_stride >= 0 && p->frame_stride >= 0, "frame_map: bad strides");
-    FrameMap a{p->lengths, p->first, p->streams, p->table, p->ldt, p->pages, p->page,
-               p->page_stride, p->frame_stride, p->taps, p->step,
-               p->clamp ? 1 : 0, p->low, p->high, p->starts, p->rows, p->cap, INT_MIN, {},
-               Divider((uint32_t)p->pages * (uint32_t)p->page), Divider((uint32_t)p->page), false, {}};
-    const long long ring = (long long)p->pages * p->page;
-    for (int j = 0; j < a.taps; j++) {
-      a.offset[j] = p->offsets[j];
-      if (a.offset[j] > a.max_offset) a.max_offset = a.offset[j];
-      a.far_offsets = a.far_offsets || a.offset[j] > (1 << 30) || a.offset[j] < -(1 << 30);
-      a.offset_at[j] = (unsigned)(((long long)a.offset[j] % ring + ring) % ring);
-    }
+    FrameMap a{};
+    a.lengths = p->lengths;
+    a.first = p->first;
+    a.streams = p->streams;
+    a.table = p->table;
+    a.ldt = p->ldt;
+    a.pages = p->pages;
+    a.page = p->page;
+    a.page_stride = p->page_stride;
+    a.frame_stride = p->frame_stride;
+    a.taps = p->taps;
+    a.step = p->step;
+    a.clamp = p->clamp ? 1 : 0;
+    a.low = p->low;
+    a.high = p->high;
+    a.starts = p->starts;
+    a.rows = p->rows;
+    a.cap = p->cap;
+    SetOffsets(&a, p->offsets);
     OnDevice guard(device);
     LaunchFrameMap(a, (hipStream_t)stream);
     OnDevice::Check(hipGetLastError());

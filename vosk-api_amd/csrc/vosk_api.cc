@@ -299,6 +299,7 @@ VamdEngine* vamd_engine_new(const char* model_dir, int fpc, int max_streams, int
   cfg.pipeline = (flags & 8) != 0;
   cfg.lattice = (flags & 16) != 0;
   cfg.kaldi_order = (flags & 32) == 0;
+  cfg.nnet_int8 = (flags & 64) != 0;
   const char* d = getenv("VOSK_AMD_DEVICE");
   cfg.device = d ? atoi(d) : 0;
   const char* at = getenv("VOSK_AMD_ARENA_TOKENS");
@@ -816,6 +817,24 @@ int vamd_stream_lattice(VamdEngine* e, int s, int use_final, int* sizes4, int* f
   }
   return 0;
   API_CATCH(-1)
+}
+
+int vamd_engine_int8_layers(VamdEngine* e) {
+  API_TRY
+  return e->eng->Int8Layers();
+  API_CATCH(-1)
+}
+
+const char* vamd_plan_describe_int8(const char* model_dir, int fpc) {
+  static thread_local std::string out;
+  API_TRY
+  ModelData md;
+  md.Load(model_dir);
+  const NnetPlan p = BuildNnetPlan(md.nnet, fpc > 0 ? fpc : md.dcb.frames_per_chunk,
+                                   md.dcb.frame_subsampling_factor, md.dcb.acoustic_scale);
+  out = BuildInt8Plan(p).Describe(p);
+  return out.c_str();
+  API_CATCH(nullptr)
 }
 
 int vamd_engine_ivector_dim(VamdEngine* e) {

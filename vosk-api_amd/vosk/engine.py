@@ -35,6 +35,8 @@ _SIGS = {
     "vamd_stream_llh": (C.c_longlong, [_vp, C.c_int, _vp, C.c_longlong]),
     "vamd_stream_ivectors": (C.c_longlong, [_vp, C.c_int, _vp, C.c_longlong]),
     "vamd_engine_ivector_dim": (C.c_int, [_vp]),
+    "vamd_engine_int8_layers": (C.c_int, [_vp]),
+    "vamd_plan_describe_int8": (C.c_char_p, [C.c_char_p, C.c_int]),
     "vamd_stream_update_silence_weights": (C.c_int, [_vp, C.c_int, C.c_int]),
     "vamd_stream_lattice": (C.c_int, [_vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                       _vp, _vp, _vp]),
@@ -270,6 +272,14 @@ def plan_describe(model_dir, frames_per_chunk=0):
     return r.decode()
 
 
+def plan_describe_int8(model_dir, frames_per_chunk=0):
+    """Host-only: the layers that precision="int8" runs as 8-bit products."""
+    r = _c.vamd_plan_describe_int8(str(model_dir).encode(), frames_per_chunk)
+    if r is None:
+        raise RuntimeError("vamd_plan_describe_int8 failed: " + _err())
+    return r.decode()
+
+
 def plan_info(model_dir, frames_per_chunk=0):
     info = np.zeros(8, np.int32)
     fl = C.c_double(0)
@@ -287,14 +297,19 @@ def device_count():
 
 class Engine:
     def __init__(self, model_dir, frames_per_chunk=0, max_streams=8, stats=False, keep_llh=False,
-                 time_kernels=False, pipeline=False, lattice=False, order="kaldi"):
+                 time_kernels=False, pipeline=False, lattice=False, order="kaldi", precision="fp32"):
         """order: "kaldi" (LatticeFasterDecoder's sequential token passing,
         the KaldiRecognizer path) or "parallel" (the order-independent form
-        the BatchModel lanes run); VOSK_AMD_DEC_ORDER overrides either."""
+        the BatchModel lanes run); VOSK_AMD_DEC_ORDER overrides either.
+        precision: "fp32", or "int8" for the acoustic model's affine layers as
+        8-bit products (the operators of vosk.ops); VOSK_AMD_NNET overrides."""
         if order not in ("kaldi", "parallel"):
             raise ValueError("order: 'kaldi' or 'parallel'")
+        if precision not in ("fp32", "int8"):
+            raise ValueError("precision: 'fp32' or 'int8'")
         flags = ((1 if stats else 0) | (2 if keep_llh else 0) | (4 if time_kernels else 0)
-                 | (8 if pipeline else 0) | (16 if lattice else 0) | (32 if order == "parallel" else 0))
+                 | (8 if pipeline else 0) | (16 if lattice else 0) | (32 if order == "parallel" else 0)
+                 | (64 if precision == "int8" else 0))
         h = _c.vamd_engine_new(str(model_dir).encode(), frames_per_chunk, max_streams, flags)
         if not h:
             raise RuntimeError("vamd_engine_new failed: " + _err())
@@ -306,6 +321,7 @@ class Engine:
         (self.fpc, self.fss, self.left_context, self.right_context, self.priming,
          self.out_dim, self.num_ops, _) = [int(x) for x in info]
         self.flops_per_chunk = fl.value
+        self.int8_layers = _chk(_c.vamd_engine_int8_layers(h))
 
     def close(self):
         if self.h:
