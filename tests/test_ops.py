@@ -204,8 +204,8 @@ def test_plan_of_the_8_bit_layers(synth_model):
     assert ops["tdnn1.dropout"].startswith("-> codes")
     assert "-> codes" not in ops["tdnnf3.noop"]  # read by tdnnf4.linear and a bypass alone
     assert engine.plan_describe_int8(synth_model, 21).splitlines()[-1].startswith("24 products")
-    # chunks of one output frame: two frames of tdnnf4.linear a chunk, evenly spaced as two always are
-    assert engine.plan_describe_int8(synth_model, 3).splitlines()[-1].startswith("25 products")
+    # chunks of one output frame: tdnnf4.linear has two frames a chunk, evenly spaced as two always are, and tdnnf4.noop reads it
+    assert engine.plan_describe_int8(synth_model, 3).splitlines()[-1].startswith("26 products")
 
 
 def test_precision_names():
