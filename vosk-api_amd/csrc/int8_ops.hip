@@ -436,8 +436,10 @@ __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a) {
 // straight from global memory into a ring of ST LDS buffers, so ST - 1 steps
 // of loads are in flight behind the matrix instructions and one barrier a step
 // is enough.  A part's rows are 64 bytes in LDS, their four 16-byte chunks
-// permuted by (row >> 1) & 3 (on the global side of the load: LDS takes lane
-// after lane), which spreads the rows that a read covers over the banks.
+// permuted by (row >> 2) & 3 (on the global side of the load: LDS takes lane
+// after lane), so that the sixteen lanes which a 16-byte-a-lane read serves
+// together, four runs of four rows, lie in different banks ((row >> 1) & 3,
+// right for eight neighbouring rows, cost 1.5 times the reads' cycles).
 constexpr int kPartBytes = 64;
 
 // lane l's 16 bytes at p go to LDS byte `to` + 16 * l (to: the same in all lanes).
@@ -576,7 +578,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   const int kt = a.k / kPartBytes, parts = kt * a.taps, steps = (parts + KB - 1) / KB;
   // this wave's loads: LOADS groups of 16 rows (the tile's rows of A, then of
   // W), lane l row l >> 2, chunk slot l & 3; absent rows read row 0
-  const int lrow = lane >> 2, chunk = (lane & 3) ^ ((lrow >> 1) & 3);
+  const int lrow = lane >> 2, chunk = (lane & 3) ^ ((lrow >> 2) & 3);
   const int8_t* p[LOADS];
 #pragma unroll
   for (int g = 0; g < LOADS; g++) {
@@ -660,7 +662,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   };
   float z[16];
   if (BM * BN == 1 && a.residual && !a.res_from) residual(0, 0, z);
-  const int f0 = (h ^ ((r32 >> 1) & 3)) << 4, f1 = ((2 + h) ^ ((r32 >> 1) & 3)) << 4;
+  const int f0 = (h ^ ((r32 >> 2) & 3)) << 4, f1 = ((2 + h) ^ ((r32 >> 2) & 3)) << 4;
   intx16 acc[BM][BN];
   float v[MULTI ? BM : 1][MULTI ? BN : 1][16];
 #pragma unroll
@@ -1067,7 +1069,7 @@ void LaunchLinearInt8(const LinearInt8& a, hipStream_t s) {
   } else if (!wide || a.k < 256) {
     LaunchSmallTiles<false>(a, tiles(64, 64), s);
   } else if (a.k >= 2048 && tiles(256, 256) >= 128) {
-    LaunchTile<256, 256, 4, 4, 2, 2, false>(a, s);
+    LaunchTile<256, 256, 4, 2, 2, 2, false>(a, s);
   } else if (tiles(128, 256) >= 256) {
     LaunchTile<128, 256, 2, 4, 3, 1, false>(a, s);
   } else {
