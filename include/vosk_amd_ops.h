@@ -81,16 +81,17 @@ int vamd_op_frame_map(int device, void *stream, const VamdFrameMap *args);
  * the rest is 32-bit floats:  v = v + bias[n];  v = max(v, 0) if relu;
  * v = v * gain[n] + shift[n];  v = residual_scale * residual[i][n] + v;
  * rounded to out_type.
- * With x (and codes, scale, rows NULL, one tap) the m rows of floats are
- * quantised as by vamd_op_quantize_rows and multiplied in one call;
- * vamd_op_linear_workspace() says whether that takes a workspace.  m is at
+ * With x (and codes and scale NULL) rows of floats take the place of codes:
+ * they are quantised as by vamd_op_quantize_rows in the call, which may take a
+ * workspace (vamd_op_linear_workspace).  rows then maps the cache_rows rows of
+ * x; without it x has m rows.  m is at
  * most 2^30, n and the row strides ldr and ldo at most 2^23. */
 typedef struct {
     const signed char *codes; /* rows of kb bytes, lda apart; 16-byte aligned rows */
     const float *scale;      /* [cache_rows] */
     const int *rows;         /* [m][taps], rows ldrows entries apart, or NULL */
     const int *count;        /* or NULL: output rows from *count on are left as they were */
-    const void *x;           /* [m][k] of x_type, rows ldx elements apart, or NULL */
+    const void *x;           /* rows of k of x_type, ldx elements apart, or NULL */
     void *workspace;         /* 16-byte aligned, this call's alone until it has run */
     const signed char *w;    /* [n][taps * kb] codes, rows ldw apart; 16-byte aligned rows */
     const float *wscale;     /* [n] */
@@ -107,8 +108,9 @@ typedef struct {
     float residual_scale;
 } VamdLinearInt8;
 int vamd_op_linear_int8(int device, void *stream, const VamdLinearInt8 *args);
-/* Bytes of workspace for m rows of k floats and n columns: may be 0; < 0 for bad sizes. */
-long long vamd_op_linear_workspace(int m, int n, int k);
+/* Bytes of workspace for m output rows, n columns and x_rows rows of k floats
+ * (x_rows = m without a map): may be 0; < 0 for bad sizes. */
+long long vamd_op_linear_workspace(int m, int n, int k, int taps, long long x_rows);
 
 #ifdef __cplusplus
 }

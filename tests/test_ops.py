@@ -83,12 +83,17 @@ def test_code_bytes(lib, k, want):
 
 
 def test_workspace(lib):
-    assert lib.vamd_op_linear_workspace(1000, 500, 65) == 1000 * (128 + 4)
-    assert lib.vamd_op_linear_workspace(0, 5, 65) == 0
-    assert lib.vamd_op_linear_workspace(-1, 5, 65) < 0
-    assert lib.vamd_op_linear_workspace(1, -5, 65) < 0
-    assert lib.vamd_op_linear_workspace(1, 5, 0) < 0
-    assert lib.vamd_op_linear_workspace((1 << 30) + 1, 5, 64) < 0
+    assert lib.vamd_op_linear_workspace(1000, 500, 65, 1, 1000) == 1000 * (128 + 4)
+    assert lib.vamd_op_linear_workspace(1000, 500, 65, 3, 77) == 77 * (128 + 4)
+    assert lib.vamd_op_linear_workspace(1, 500, 65, 3, 77) == 0
+    assert lib.vamd_op_linear_workspace(0, 5, 65, 1, 0) == 0
+    assert lib.vamd_op_linear_workspace(-1, 5, 65, 1, 4) < 0
+    assert lib.vamd_op_linear_workspace(1, -5, 65, 1, 4) < 0
+    assert lib.vamd_op_linear_workspace(1, 5, 65, 0, 4) < 0
+    assert lib.vamd_op_linear_workspace(1, 5, 65, 17, 4) < 0
+    assert lib.vamd_op_linear_workspace(1, 5, 65, 1, -4) < 0
+    assert lib.vamd_op_linear_workspace(1, 5, 0, 1, 4) < 0
+    assert lib.vamd_op_linear_workspace((1 << 30) + 1, 5, 64, 1, 4) < 0
 
 
 def test_no_arguments(lib):
@@ -161,7 +166,8 @@ FLOAT = dict(x=P, ldx=100, workspace=P, w=P, ldw=128, wscale=P, m=700, n=9, k=10
 @pytest.mark.parametrize("change,what", [
     (dict(k=0), "k has"), (dict(x_type=7), "element type"), (dict(ldx=50), "overlap"), (dict(x=P + 1), "aligned"),
     (dict(workspace=None), "null"), (dict(workspace=P + 4), "16-byte"), (dict(ldw=64), "shorter"), (dict(m=-2), "sizes"),
-    (dict(rows=P), "without codes"), (dict(taps=2), "without codes"),
+    (dict(codes=P), "without codes"), (dict(scale=P), "without codes"), (dict(taps=2, ldw=256), "row map"), (dict(taps=0), "taps"),
+    (dict(rows=P, ldrows=1), "bad number"),
 ])
 def test_linear_of_floats_refuses(lib, change, what):
     assert _call(lib, "vamd_op_linear_int8", Linear, **{**FLOAT, **change}) < 0

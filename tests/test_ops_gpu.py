@@ -456,6 +456,31 @@ def test_linear_mapped_rows(ops, m, n, k, taps, t):
     assert (out[torch.from_numpy(rest).cuda()] == 7.0).all()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,n,k,taps", [(1, 17, 5, 1), (1, 96, 512, 2), (17, 96, 512, 2), (17, 512, 96, 2), (32, 40, 100, 3), (9, 50, 64, 16), (3, 33, 4096, 2),
+                                        (33, 40, 100, 3), (300, 96, 512, 2)])
+def test_linear_float_rows_through_a_map(ops, m, n, k, taps, t):
+    """Quantised in the call or beforehand: the same bits; absent rows, one row under several taps."""
+    g = _gen(m + n + k)
+    x = (_randn(g, 50, k) * torch.exp(_randn(g, 50, 1))).to(TYPES[t])
+    x[7] = 0
+    x[8, 0] = float("inf")
+    w, ws = ops.quantize_weight(_randn(g, n, taps * k) / (taps * k) ** 0.5, taps)
+    rows = torch.randint(-1, 51, (m, taps), generator=g, device="cuda", dtype=torch.int32)
+    rows[0] = 3
+    if m > 2:
+        rows[1], rows[2, 0] = -1, 7
+    c, s = ops.quantize_rows(x)
+    want = ops.linear_int8(c, w, ws, scale=s, rows=rows)
+    got = ops.linear_int8(x, w, ws, rows=rows)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    fine = ~(rows == 8).any(1)
+    assert not torch.isnan(got[fine]).any() and torch.isnan(got[~fine]).all()
+    v, size = ref.linear(*(a[:len(a)] for a in ref.codes_of(np.where(np.isfinite(_np(x)), _np(x), 0))), rows.cpu().numpy(), w.cpu().numpy(), ws.cpu().numpy(), taps)
+    f = fine.cpu().numpy()
+    _check(got[fine], v[f], size[f], taps, "fp32")
+
+
 def test_linear_empty(ops):
     w, ws = ops.quantize_weight(torch.ones(3, 64, device="cuda"))
     assert ops.linear_int8(torch.ones(0, 64, device="cuda"), w, ws).shape == (0, 3)
@@ -488,7 +513,7 @@ def test_refusals(ops):
         (lambda: ops.linear_int8(c, w, ws, scale=s, out=x[:, :8], out_rows=rows[:3, 0]), "elements"),
         (lambda: ops.quantize_rows(x, from_rows=rows[:, 0]), "codes and scales"),
         (lambda: ops.quantize_rows(x, c, s, rows=rows[:3, 0], from_rows=rows[:, 0]), "elements"),
-        (lambda: ops.linear_int8(x, w, ws, rows=rows), "belong to codes"),
+        (lambda: ops.linear_int8(x, w, ws, scale=s), "belongs to codes"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, gain=ws), "together"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, bias=ws.cpu()), "another device"),
         (lambda: ops.linear_int8(c, w, ws, scale=s, residual=x), "residual"),

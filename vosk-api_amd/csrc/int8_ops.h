@@ -138,9 +138,10 @@ struct LinearInt8 {
   long long ldres_from, res_rows;
 };
 void LaunchLinearInt8(const LinearInt8& a, hipStream_t s);
-// The product of float rows: x's codes and scales are a's (a workspace, not
-// used where LinearFloatFused(a.m, a.k): one launch then quantises in LDS).
-bool LinearFloatFused(int m, int k);
+// The product of float rows x, gathered through a's row map: x's codes and
+// scales (of all its rows) are a's, a workspace that is not used where
+// LinearFloatFused: one launch then quantises the rows it reads in LDS, to the
+// same codes.
+bool LinearFloatFused(int m, int k, int taps);
 void LaunchLinearFloat(const LinearInt8& a, const QuantizeRows& x, hipStream_t s);
-
 }  // namespace vamd

@@ -268,17 +268,20 @@ __global__ __launch_bounds__(kMapThreads) void frame_starts_kernel(FrameMap a) {
   if (tid == 0) a.starts[a.streams] = saturated(total);
 }
 
-// SUM: the workgroup sums the streams itself.  A lane makes ROWS rows, 64
-// apart, of the ROWS * 64 of its wave, their loads in flight together.
-template <bool SUM, int ROWS>
+// The workgroup sums the streams itself, EACH a thread (0: `starts` is there
+// already).  A lane makes ROWS rows, 64 apart, of the ROWS * 64 of its wave,
+// their loads in flight together.
+template <int EACH, int ROWS>
 __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a) {
-  constexpr int EACH = kMapStreams / kMapThreads;
+  constexpr bool SUM = EACH > 0;
+  constexpr int GAP = EACH > 1 ? EACH : 1 << 30;
   // starts; a gap every EACH so that a thread's lie in other banks than its neighbours'
-  __shared__ int sums[SUM ? kMapStreams + kMapThreads : 1];
+  __shared__ int sums[SUM ? (EACH + 1) * kMapThreads : 1];
   const int tid = threadIdx.x;
-  auto at = [](int r) { return r + r / EACH; };
+  auto at = [](int r) { return r + r / GAP; };
   unsigned total;
-  if (SUM) {
+  if constexpr (SUM) {
+    constexpr int STRIDE = EACH > 1 ? EACH + 1 : 1;
     unsigned n[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
@@ -293,7 +296,7 @@ __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a) {
     if (any) {
 #pragma unroll
       for (int i = 0; i < EACH; i++) {
-        n[i] = (unsigned)sums[tid * (EACH + 1) + i];
+        n[i] = (unsigned)sums[tid * STRIDE + i];
         sum = add_sat(sum, n[i]);
       }
     }
@@ -301,7 +304,7 @@ __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a) {
     if (any) {
 #pragma unroll
       for (int i = 0; i < EACH; i++) {
-        sums[tid * (EACH + 1) + i] = saturated(v);
+        sums[tid * STRIDE + i] = saturated(v);
         v = add_sat(v, n[i]);
       }
     }
@@ -549,7 +552,9 @@ __device__ __forceinline__ void finish_16(const LinearInt8& a, float (&v)[16], c
 
 // (two waves a SIMD leave 256 registers a wave: the accumulators then stay
 // where the products and the epilogue both use them, without a copy a step)
-template <int TM, int TN, int WM, int WN, int ST, int KB, bool MULTI>
+// MAPPED: rows of out or of the residual go through maps (in a kernel of its
+// own: the choice at run time cost the others 5 %).
+template <int TM, int TN, int WM, int WN, int ST, int KB, bool MULTI, bool MAPPED>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2))) void linear_tile_kernel(LinearInt8 a, int tiles_m, int tiles_n) {
   constexpr int NW = WM * WN, NT = 64 * NW;
   constexpr int BM = TM / WM / 32, BN = TN / WN / 32;  // 32 x 32 blocks of a wave
@@ -560,7 +565,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   float* const sscale = (float*)(smem + ST * KB * PART);
   int* const srow = (int*)(sscale + a.taps * TM);
   uint32_t* const sout = (uint32_t*)(srow + (MULTI ? a.taps * TM : 0));  // mapped rows of out and residual: their bytes
-  uint32_t* const sres = sout + (a.out_to ? TM : 0);
+  uint32_t* const sres = sout + (MAPPED && a.out_to ? TM : 0);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // workgroups b, b + 8, ... run on one XCD: each XCD gets neighbouring tiles
@@ -622,7 +627,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
     const int row = m < mrows ? map[m * ld] : -1;
     return row >= 0 && row < rows ? (uint32_t)row * row_bytes : kOutside;
   };
-  if (a.out_to || a.res_from) {
+  if (MAPPED) {
     for (int i = tid; i < TM; i += NT) {
       if (a.out_to) sout[i] = bytes_of(a.out_to, a.ldout_to, a.out_rows, (uint32_t)(a.ldo * osize), m0 + i);
       if (a.res_from) sres[i] = bytes_of(a.res_from, a.ldres_from, a.res_rows, (uint32_t)(a.ldr * rsize), m0 + i);
@@ -641,7 +646,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
     const uint32_t col = n < a.n ? (uint32_t)(n * size) : kOutside;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-      if (map) {
+      if (MAPPED && map) {
         const uint4 f = *reinterpret_cast<const uint4*>(&map[wm + x * 32 + 4 * h + 8 * q]);
         at[4 * q] = max(f.x, f.x + col);  // (a column and a row that are both outside: no wrap to inside)
         at[4 * q + 1] = max(f.y, f.y + col);
@@ -654,14 +659,15 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
     }
   };
   auto residual = [&](int x, int y, float (&z)[16]) {
-    const BlockRows b = a.res_from ? BlockRows(a.residual, rsize, a.ldr, a.res_rows)
+    const BlockRows b = MAPPED && a.res_from ? BlockRows(a.residual, rsize, a.ldr, a.res_rows)
                                    : BlockRows(a.residual, rsize, a.ldr, m0 + wm + x * 32, mrows);
     uint32_t at[16];
-    place(x, y, b.ld, rsize, a.res_from ? sres : nullptr, at);
+    place(x, y, b.ld, rsize, MAPPED && a.res_from ? sres : nullptr, at);
     load_16(b, a.res_type, at, z);
   };
   float z[16];
-  if (BM * BN == 1 && a.residual && !a.res_from) residual(0, 0, z);
+  const bool late = BM * BN > 1 || (MAPPED && a.res_from);  // (its rows' table is read behind the loop)
+  if (!late && a.residual) residual(0, 0, z);
   const int f0 = (h ^ ((r32 >> 2) & 3)) << 4, f1 = ((2 + h) ^ ((r32 >> 2) & 3)) << 4;
   intx16 acc[BM][BN];
   float v[MULTI ? BM : 1][MULTI ? BN : 1][16];
@@ -737,12 +743,12 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
       float w[16];
 #pragma unroll
       for (int i = 0; i < 16; i++) w[i] = MULTI ? v[x][y][i] : fmaf((float)acc[x][y][i], sc[i], 0.0f);
-      if ((BM * BN > 1 || a.res_from) && a.residual) residual(x, y, z);
+      if (late && a.residual) residual(x, y, z);
       finish_16(a, w, col[y], z);
-      const BlockRows b = a.out_to ? BlockRows(a.out, osize, a.ldo, a.out_rows)
+      const BlockRows b = MAPPED && a.out_to ? BlockRows(a.out, osize, a.ldo, a.out_rows)
                                    : BlockRows(a.out, osize, a.ldo, m0 + wm + x * 32, mrows);
       uint32_t at[16];
-      place(x, y, b.ld, osize, a.out_to ? sout : nullptr, at);
+      place(x, y, b.ld, osize, MAPPED && a.out_to ? sout : nullptr, at);
       store_16(b, a.out_type, at, w);
     }
   }
@@ -758,12 +764,12 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
 // workgroup itself, each workgroup for itself, which costs less than a launch
 // before this one.  A first batch of weight loads is on its way meanwhile.
 constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
-constexpr int kFusedValues = 16384;  // float values (rows x padded columns) that a workgroup quantises itself
+constexpr int kFusedValues = 16384;  // float values (rows x taps x padded columns) that a workgroup quantises itself
 
-template <int TYPE, int RT>  // TYPE < 0: codes; RT blocks of 16 rows
+template <int TYPE, int RT, int VALUES>  // TYPE < 0: codes, else up to VALUES float values; RT blocks of 16 rows
 __global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, QuantizeRows x) {
-  constexpr int R = 16 * RT, AHEAD = 8;
-  extern __shared__ char smem[];  // codes [R][ldl], partial sums [8][RT][256], scales [taps][R], maxima [R]
+  constexpr int R = 16 * RT, AHEAD = 4;
+  extern __shared__ char smem[];  // codes [R][ldl], partial sums [8][RT][256], scales [taps][R], maxima [taps][R]
   const int kk = a.k * a.taps, ldl = kk + 16;  // 16 bytes on: rows in other banks
   int* const part = (int*)(smem + R * ldl);
   float* const sscale = (float*)(part + kFewWaves * RT * 256);
@@ -779,50 +785,60 @@ __global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, Q
 #pragma unroll
   for (int i = 0; i < AHEAD; i++) {
     const int s = wave + kFewWaves * i;
-    w[i] = *reinterpret_cast<const intx4*>(wp + 64 * (s < steps ? s : 0));
+    if (s < steps) w[i] = *reinterpret_cast<const intx4*>(wp + 64 * s);
   }
 
   const Column col = column(a, min(n0 + (tid & 15), a.n - 1));  // of the values below
+  auto row_of = [&](int q) { return a.taps == 1 ? q : q / a.taps; };  // of tap q of all rows
   if constexpr (TYPE >= 0) {
     constexpr int N = Chunk<TYPE < 0 ? 0 : TYPE>::N;
-    // all chunks of all rows (LinearFloatFused: HELD a thread) stay in registers
-    const int chunks = a.k / N, all = mrows * chunks;  // past a row's end: zeros
-    constexpr int HELD = kFusedValues / (kFewThreads * N);
+    // all chunks of all rows of all taps stay in registers (LinearFloatFused)
+    const int chunks = a.k / N, all = mrows * a.taps * chunks;  // past a row's end: zeros
+    constexpr int HELD = VALUES / (kFewThreads * N);
     Chunk<TYPE < 0 ? 0 : TYPE> c[HELD];
-    int mm[HELD];
+    int place[HELD];  // tap * R + row; -1: the row is absent
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
-      const int q = tid + i * kFewThreads;
-      mm[i] = q / chunks;
-      if (q < all) c[i].load(x.x, mm[i] * x.ldx, (q - mm[i] * chunks) * N, x.k);
+      const int u = tid + i * kFewThreads, q = u / chunks, m = row_of(q), j = q - m * a.taps;
+      place[i] = -1;
+      if (u >= all) continue;
+      const int row = a.rows ? a.rows[m * a.ldrows + j] : m;
+      if (row >= 0 && row < a.arows) {
+        place[i] = j * R + m;
+        c[i].load(x.x, row * x.ldx, (u - q * chunks) * N, x.k);
+      }
     }
-    if (tid < R) smax[tid] = 0;
+    for (int i = tid; i < a.taps * R; i += kFewThreads) smax[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
-      if (tid + i * kFewThreads >= all) break;
-      uint32_t top = c[i].top_bits(c[i].top(0));
-      if (__all(mm[i] == __builtin_amdgcn_readfirstlane(mm[i]))) {  // one atomic a wave where it holds one row
+      uint32_t top = place[i] >= 0 ? c[i].top_bits(c[i].top(0)) : 0u;
+      const int one = __builtin_amdgcn_readfirstlane(place[i]);
+      if (__all(place[i] == one)) {  // one atomic a wave where it holds one row
+        if (one < 0) continue;
         top = wave_max(top);
-        if (lane == 0) atomicMax(&smax[mm[i]], top);
-      } else {
-        atomicMax(&smax[mm[i]], top);
+        if (lane == 0) atomicMax(&smax[one], top);
+      } else if (place[i] >= 0) {
+        atomicMax(&smax[place[i]], top);
       }
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
-      const int q = tid + i * kFewThreads;
-      if (q >= all) break;
-      const int e = (q - mm[i] * chunks) * N;
-      const RowScale r = row_scale(smax[mm[i]]);
-      c[i].store((int8_t*)smem + mm[i] * ldl + e, r);
-      if (e == 0) sscale[mm[i]] = r.scale;
+      const int u = tid + i * kFewThreads, q = u / chunks, m = row_of(q), j = q - m * a.taps, e = (u - q * chunks) * N;
+      if (u >= all) break;
+      if (place[i] >= 0) {
+        const RowScale r = row_scale(smax[place[i]]);
+        c[i].store((int8_t*)smem + m * ldl + j * a.k + e, r);
+        if (e == 0) sscale[place[i]] = r.scale;
+      } else if (e == 0) {
+        sscale[j * R + m] = 0.0f;  // (whatever its codes: the sum of them is finite)
+      }
     }
   } else {
     const int chunks = a.k / 16, all = mrows * a.taps * chunks;
     for (int i = tid; i < all; i += kFewThreads) {
-      const int q = i / chunks, e = (i - q * chunks) * 16, m = q / a.taps, j = q - m * a.taps;
+      const int q = i / chunks, e = (i - q * chunks) * 16, m = row_of(q), j = q - m * a.taps;
       long long row = a.rows ? a.rows[m * a.ldrows + j] : m;
       const bool there = row >= 0 && row < a.arows;
       if (!there) row = 0;
@@ -953,10 +969,14 @@ void LaunchFrameMap(const FrameMap& a, hipStream_t s) {
   const int each = a.cap > 256 * 1024 && a.taps <= 8 ? 2 : 1;
   const unsigned grid = (unsigned)((a.cap + each * kMapThreads - 1) / (each * kMapThreads));
   const unsigned lds = each * kMapThreads * a.taps * sizeof(int);
-  if (sum && each == 1) hipLaunchKernelGGL((frame_map_kernel<true, 1>), dim3(grid ? grid : 1), dim3(kMapThreads), lds, s, a);
-  else if (sum) hipLaunchKernelGGL((frame_map_kernel<true, 2>), dim3(grid), dim3(kMapThreads), lds, s, a);
-  else if (grid && each == 1) hipLaunchKernelGGL((frame_map_kernel<false, 1>), dim3(grid), dim3(kMapThreads), lds, s, a);
-  else if (grid) hipLaunchKernelGGL((frame_map_kernel<false, 2>), dim3(grid), dim3(kMapThreads), lds, s, a);
+  const dim3 blocks(grid ? grid : 1), threads(kMapThreads);
+  if (!sum && !grid) return;
+  if (!sum && each == 1) hipLaunchKernelGGL((frame_map_kernel<0, 1>), blocks, threads, lds, s, a);
+  else if (!sum) hipLaunchKernelGGL((frame_map_kernel<0, 2>), blocks, threads, lds, s, a);
+  else if (a.streams <= kMapThreads && each == 1) hipLaunchKernelGGL((frame_map_kernel<1, 1>), blocks, threads, lds, s, a);
+  else if (a.streams <= kMapThreads) hipLaunchKernelGGL((frame_map_kernel<1, 2>), blocks, threads, lds, s, a);
+  else if (each == 1) hipLaunchKernelGGL((frame_map_kernel<kMapStreams / kMapThreads, 1>), blocks, threads, lds, s, a);
+  else hipLaunchKernelGGL((frame_map_kernel<kMapStreams / kMapThreads, 2>), blocks, threads, lds, s, a);
 }
 
 namespace {
@@ -966,7 +986,9 @@ void LaunchTile(const LinearInt8& a, hipStream_t s) {
   const long long tm = ((long long)a.m + TM - 1) / TM, tn = ((long long)a.n + TN - 1) / TN;
   if (tm * tn > INT_MAX) VAMD_ERR("too many tiles for one launch: " << a.m << " x " << a.n);
   const size_t lds = ST * KB * (TM + TN) * kPartBytes + (size_t)TM * 4 * (a.taps * (MULTI ? 2 : 1) + (a.out_to ? 1 : 0) + (a.res_from ? 1 : 0));
-  auto kernel = linear_tile_kernel<TM, TN, WM, WN, ST, KB, MULTI>;
+  const bool mapped = a.out_to || a.res_from;
+  auto kernel = mapped ? linear_tile_kernel<TM, TN, WM, WN, ST, KB, MULTI, true>
+                       : linear_tile_kernel<TM, TN, WM, WN, ST, KB, MULTI, false>;
   AskLds((const void*)kernel, lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, s, a, (int)tm, (int)tn);
 }
@@ -988,12 +1010,12 @@ void LaunchSmallTiles(const LinearInt8& a, long long tiles, hipStream_t s) {
 
 size_t FewLds(int m, int k, int taps) {
   const size_t rt = m <= 16 ? 1 : 2;
-  return rt * 16 * ((size_t)k * taps + 16) + kFewWaves * rt * 1024 + rt * 16 * 4 * (taps + 1);
+  return rt * 16 * ((size_t)k * taps + 16) + kFewWaves * rt * 1024 + rt * 16 * 4 * 2 * taps;
 }
 
-template <int TYPE, int RT>
+template <int TYPE, int RT, int VALUES>
 void LaunchFew(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
-  auto kernel = linear_few_kernel<TYPE, RT>;
+  auto kernel = linear_few_kernel<TYPE, RT, VALUES>;
   const size_t lds = FewLds(a.m, a.k, a.taps);
   AskLds((const void*)kernel, lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)((a.n + 15) / 16)), dim3(kFewThreads), lds, s, a, x);
@@ -1001,25 +1023,33 @@ void LaunchFew(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
 
 template <int TYPE>
 void LaunchFewRows(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
-  if (a.m <= 16) LaunchFew<TYPE, 1>(a, x, s);
-  else LaunchFew<TYPE, 2>(a, x, s);
+  const bool more = (long long)a.m * a.taps * a.k > kFusedValues / 4;
+  if (a.m <= 16 && more) LaunchFew<TYPE, 1, kFusedValues>(a, x, s);
+  else if (a.m <= 16) LaunchFew<TYPE, 1, kFusedValues / 4>(a, x, s);
+  else if (more) LaunchFew<TYPE, 2, kFusedValues>(a, x, s);
+  else LaunchFew<TYPE, 2, kFusedValues / 4>(a, x, s);
 }
 
 }  // namespace
 
-// Up to 32 rows: with 64 the tiles take as long (us, few / tiles, k x n: 192 x
-// 2000 4.1 / 4.5, 1024 x 96 7.0 / 6.5, 4096 x 4096 15.3 / 15.3), with 32 they
-// take longer (3.3 / 4.4, 4.9 / 6.7, 14.1 / 15.4).
-bool LinearFewRows(int m, int k, int taps) { return m <= 32 && FewLds(m, k, taps) <= 160 * 1024; }
+// Up to 32 rows (us in a graph, few / tiles, rows x k x n: 32 x 192 x 2000 3.2 /
+// 4.4, 32 x 1024 x 96 4.4 / 6.0, 64 x 512 x 512 5.5 / 3.9), as long as copying
+// them to LDS in every workgroup is little beside the weights: 17 x 4096 x 4096
+// 8.6 / 11.2, but 32 x 4096 x 4096 13.4 / 11.2.
+bool LinearFewRows(int m, int k, int taps) {
+  return m <= 32 && (long long)m * k * taps <= 96 * 1024 && FewLds(m, k, taps) <= 160 * 1024;
+}
 
-// Each workgroup quantises all rows: worth it up to 16384 values (us, fused /
-// two launches: 4 rows of 4096 10.7 / 12.4, 17 of 512 6.5 / 7.0, 32 of 192
-// 5.0 / 6.3; but 16 of 1024 8.4 / 7.2, 32 of 512 8.6 / 7.1).
-bool LinearFloatFused(int m, int k) { return LinearFewRows(m, k, 1) && (long long)m * k <= kFusedValues; }
+// Each workgroup quantises all rows: one launch up to 16384 values, which a
+// program that calls it from Python gets back (us, one call / two: 4 x 4096 x
+// 4096 10.1 / 16.0, 16 x 1024 x 1024 8.2 / 15.7), and which costs little in a
+// graph (4 x 4096 10.0 / 9.1, 17 x 512 5.8 / 5.9, 32 x 192 5.5 / 5.9, 16 x 1024
+// 7.5 / 6.9).
+bool LinearFloatFused(int m, int k, int taps) { return LinearFewRows(m, k, taps) && (long long)m * k * taps <= kFusedValues; }
 
 void LaunchLinearFloat(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
   if (a.m <= 0 || a.n <= 0) return;
-  if (LinearFloatFused(a.m, a.k)) {
+  if (LinearFloatFused(a.m, a.k, a.taps)) {
     if (x.type == kFloat32) LaunchFewRows<kFloat32>(a, x, s);
     else if (x.type == kFloat16) LaunchFewRows<kFloat16>(a, x, s);
     else LaunchFewRows<kBFloat16>(a, x, s);

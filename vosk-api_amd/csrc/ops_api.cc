@@ -70,6 +70,8 @@ void CheckRows(const QuantizeRows& a) {
   Want(a.cache_rows >= (a.rows ? 0 : a.m), "quantize_rows: fewer code rows than rows");
 }
 
+alignas(16) char kNoWorkspace[16];
+
 void CheckLinear(const LinearInt8& a) {
   Want(a.taps >= 1 && a.taps <= kMaxTaps, "linear_int8: 1 to 16 taps");
   Want(FloatTypeOk(a.out_type), "linear_int8: unknown output type");
@@ -174,24 +176,18 @@ int vamd_op_linear_int8(int device, void* stream, const VamdLinearInt8* p) {
                  p->res_from ? p->res_rows : p->m};
     QuantizeRows q{};
     if (p->x) {
-      Want(!p->codes && !p->scale && !p->rows && p->taps == 1, "linear_int8: x comes without codes, scale and rows");
+      Want(!p->codes && !p->scale, "linear_int8: x comes without codes and scale");
+      Want(p->taps >= 1 && p->taps <= kMaxTaps, "linear_int8: 1 to 16 taps");
+      Want(!p->rows || (p->cache_rows >= 1 && p->cache_rows <= kInt8MaxRows), "linear_int8: bad number of rows of x");
       const int kb = Int8Padded(p->k);
-      a.a = (const int8_t*)p->workspace;
       a.lda = kb;
-      a.sa = (const float*)(a.a + (long long)p->m * kb);
-      a.arows = p->m;
-      q = QuantizeRows{p->x, p->x_type, p->m, p->k, p->ldx, nullptr, 0, nullptr, 0, p->m, p->count, p->m,
-                       (int8_t*)p->workspace, kb, (float*)a.sa};
-      if (p->m && p->n) {
-        if (LinearFloatFused(p->m, kb)) {  // no workspace: the checks below want addresses
-          static char none[16] __attribute__((aligned(16)));
-          q.codes = (int8_t*)none;
-          q.scales = (float*)none;
-          a.a = q.codes;
-          a.sa = q.scales;
-        }
-        CheckRows(q);
-      }
+      a.arows = p->rows ? p->cache_rows : p->m;
+      // (without a workspace the checks below still want addresses)
+      a.a = (const int8_t*)(LinearFloatFused(p->m, kb, p->taps) ? kNoWorkspace : p->workspace);
+      a.sa = (const float*)(a.a + (LinearFloatFused(p->m, kb, p->taps) ? 0 : a.arows * kb));
+      q = QuantizeRows{p->x, p->x_type, a.arows, p->k, p->ldx, nullptr, 0, nullptr, 0, a.arows,
+                       p->rows ? nullptr : p->count, a.arows, (int8_t*)a.a, kb, (float*)a.sa};
+      if (p->m && p->n) CheckRows(q);
     }
     CheckLinear(a);
     if (a.m == 0 || a.n == 0) return;
@@ -205,13 +201,14 @@ int vamd_op_linear_int8(int device, void* stream, const VamdLinearInt8* p) {
   });
 }
 
-long long vamd_op_linear_workspace(int m, int n, int k) {
-  if (m < 0 || m > kInt8MaxRows || n < 0 || n > kInt8MaxCols || k < 1 || k > kInt8MaxK) {
+long long vamd_op_linear_workspace(int m, int n, int k, int taps, long long x_rows) {
+  if (m < 0 || m > kInt8MaxRows || n < 0 || n > kInt8MaxCols || k < 1 || k > kInt8MaxK || taps < 1 || taps > kMaxTaps ||
+      x_rows < 0 || x_rows > kInt8MaxRows) {
     SetLastError("linear_int8: bad sizes");
     return -1;
   }
-  if (n == 0 || LinearFloatFused(m, Int8Padded(k))) return 0;
-  return (long long)m * Int8Padded(k) + 4ll * m;
+  if (m == 0 || n == 0 || LinearFloatFused(m, Int8Padded(k), taps)) return 0;
+  return x_rows * Int8Padded(k) + 4ll * x_rows;
 }
 
 }  // extern "C"

@@ -45,7 +45,7 @@ _SIGS = {
     "vamd_op_quantize_rows": (C.c_int, [C.c_int, C.c_void_p, C.c_char_p]),
     "vamd_op_frame_map": (C.c_int, [C.c_int, C.c_void_p, C.c_char_p]),
     "vamd_op_linear_int8": (C.c_int, [C.c_int, C.c_void_p, C.c_char_p]),
-    "vamd_op_linear_workspace": (C.c_longlong, [C.c_int, C.c_int, C.c_int]),
+    "vamd_op_linear_workspace": (C.c_longlong, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_longlong]),
     "vamd_last_error": (C.c_char_p, []),
 }
 for _name, (_res, _args) in _SIGS.items():
@@ -286,10 +286,10 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
 
     weight: int8 [N, J * code_bytes(K)], weight_scale: float32 [N]
     (quantize_weight).  x is either int8 codes [C, code_bytes(K)] with scale
-    float32 [C] (quantize_rows), or float rows [M, K] that are quantised in
-    the call.  With codes, rows (int32 [M, J], frame_map) says which code rows
-    are read; an entry outside [0, C) adds nothing.  Without it row i reads
-    row i.  count (int32, one element, on the GPU): output rows from there on
+    float32 [C] (quantize_rows), or float rows [C, K] that are quantised in
+    the call, to the same codes.  rows (int32 [M, J], frame_map) says which
+    rows of x are read; an entry outside [0, C) adds nothing.  Without it row
+    i reads row i.  count (int32, one element, on the GPU): output rows from there on
     are left as they were (or, where the call makes out, have no value).
 
     out [M, N] may be given, else it is made, of `dtype` (float32).  It may be
@@ -314,19 +314,19 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
         if k != kb:
             _refuse("codes have to have a multiple of %d columns" % PAD)
         xt, sp, cp, lda, xp, ldx = 0, _vector(scale, "scale", _f32, m, dev), xp, ldx, 0, 0
-        if rows is not None:
-            rp, m, taps, ldi = _matrix(rows, "rows", dev)
-            if rows.dtype is not _i32:
-                _refuse("rows has to be int32 [M, J]")
-            if not 1 <= taps <= MAX_TAPS:
-                _refuse("rows has to have 1 to %d columns" % MAX_TAPS)
     else:
         xt = _TYPES.get(x.dtype)
         if xt is None:
             _refuse("x has to be int8 codes, float32, float16 or bfloat16")
-        if scale is not None or rows is not None:
-            _refuse("scale and rows belong to codes")
+        if scale is not None:
+            _refuse("scale belongs to codes")
         sp = cp = lda = 0
+    if rows is not None:
+        rp, m, taps, ldi = _matrix(rows, "rows", dev)
+        if rows.dtype is not _i32:
+            _refuse("rows has to be int32 [M, J]")
+        if not 1 <= taps <= MAX_TAPS:
+            _refuse("rows has to have 1 to %d columns" % MAX_TAPS)
     if wk != taps * kb:
         _refuse("weight has to have %d columns" % (taps * kb))
     _no_grad(x, residual, out, bias, gain, shift)
@@ -363,7 +363,7 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     if m == 0 or n == 0:
         return out
     if xp:
-        size = _chk(_c.vamd_op_linear_workspace(m, n, k))
+        size = _chk(_c.vamd_op_linear_workspace(m, n, k, taps, c))
         if size:
             ws = torch.empty(size, dtype=_i8, device=x.device)
             wsp = ws.data_ptr()
