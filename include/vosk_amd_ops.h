@@ -61,7 +61,7 @@ int vamd_op_quantize_rows(int device, void *stream, const VamdQuantizeRows *args
  * them is replaced by the nearest inside (clamp != 0) or has no row.  An entry
  * is -1 where there is no row: no such frame, a negative page number, a frame
  * `ring` or more before the newest one that the stream's rows name (the ring
- * cannot hold both), or a time outside 32 bits. */
+ * cannot hold both), a time outside 32 bits, a row past 2^31 - 1. */
 typedef struct {
     const int *lengths, *first; /* [streams] */
     const int *table;        /* [streams][pages] page numbers, rows ldt entries apart */
@@ -76,7 +76,7 @@ int vamd_op_frame_map(int device, void *stream, const VamdFrameMap *args);
 
 /* The matrix product over codes:
  *   out[i][n] = epi(wscale[n] * sum_j scale[r(i,j)] * sum_k codes[r(i,j)][k] * w[n][j * kb + k])
- * with kb = vamd_op_code_bytes(k) and r(i,j) = rows[i][j] (rows NULL: i, one
+ * with kb = vamd_op_code_bytes(k), codes and w in -127 .. 127, and r(i,j) = rows[i][j] (rows NULL: i, one
  * tap); an entry outside [0, cache_rows) adds nothing.  Inner sums are exact,
  * the rest is 32-bit floats:  v = v + bias[n];  v = max(v, 0) if relu;
  * v = v * gain[n] + shift[n];  v = residual_scale * residual[i][n] + v;

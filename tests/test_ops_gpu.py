@@ -744,3 +744,83 @@ def test_another_device_than_the_current_one(ops):
         want = ops.linear_int8(x, w, ws)
     with torch.cuda.device(0):
         assert torch.equal(ops.linear_int8(x, w, ws), want)
+
+
+# ---- largest launches
+
+
+def test_quantize_rows_of_more_rows_than_a_dimension_of_the_grid(ops):
+    m = (1 << 26) + 5  # a launch has less than 2^32 threads a dimension: 64 threads a row here
+    x = (torch.arange(m, device="cuda", dtype=torch.int32) % 251 - 125).float()[:, None]
+    codes = torch.full((m, 64), 3, dtype=torch.int8, device="cuda")
+    scales = torch.full((m,), -1.0, device="cuda")
+    ops.quantize_rows(x, codes, scales)
+    want = x[:251].abs().cpu()[:, 0].numpy() / np.float32(127)
+    assert torch.equal(scales, torch.from_numpy(want).cuda()[torch.arange(m, device="cuda") % 251])
+    assert torch.equal(codes[:, 0].float(), 127 * torch.sign(x[:, 0]))
+    assert not codes[:, 1:].any()
+
+
+def test_linear_of_more_rows_than_a_dimension_of_the_grid(ops):
+    m, c, g = 1 << 30, 1009, _gen(81)  # 2^24 tiles of 64 rows by 256 threads: 2^32
+    codes, scales = ops.quantize_rows(_randn(g, c, 40))
+    w, ws = ops.quantize_weight(_randn(g, 1, 40))
+    few = ops.linear_int8(codes, w, ws, scale=scales, dtype=torch.float16)
+    rows = torch.arange(c, device="cuda", dtype=torch.int32).repeat(-(-m // c))[:m, None]
+    out = torch.full((m, 1), 7.0, dtype=torch.float16, device="cuda")
+    ops.linear_int8(codes, w, ws, scale=scales, rows=rows, out=out)
+    whole = m // c * c
+    assert (out[:whole].view(-1, c) == few.view(1, c)).all()
+    assert torch.equal(out[whole:], few[:m - whole])
+
+
+def test_frame_map_rows_past_31_bits_have_no_entry(ops):
+    """Pages so high that a cache row's number passes 2^31 - 1."""
+    page = 1 << 20
+    table = torch.tensor([[2047, 2048, 2047, 1 << 30], [2**31 - 1, 0, 1, 4096]], dtype=torch.int32, device="cuda")
+    first = torch.tensor([0, 0], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([4, 4], dtype=torch.int32, device="cuda")
+    rows = torch.full((8, 2), 9, dtype=torch.int32, device="cuda")
+    ops.frame_map(lengths, first, table, page, rows, offsets=(0, 1), step=1)
+    assert rows[:4].tolist() == [[2047 * page + i, 2047 * page + i + 1] for i in range(4)]
+    assert (rows[4:] == -1).all()
+    for q, want in ((1, -1), (2, 2047 * page), (3, -1)):
+        ops.frame_map(lengths[:1], torch.tensor([q * page], dtype=torch.int32, device="cuda"), table[:1], page, rows[:4],
+                      offsets=(0, page - 1))
+        assert rows[:4, 0].tolist() == [want + i if want >= 0 else -1 for i in range(4)]
+    # page * frame_stride past 32 bits as well
+    ops.frame_map(lengths[:1], first[:1], table[:1], page, rows[:4], offsets=(5, page - 4), strides=(1, 4096))
+    assert rows[:4, 0].tolist() == [2047 + (5 + i) * 4096 for i in range(4)]
+    assert (rows[:4, 1] == -1).all()
+
+
+def test_captured_map_of_many_streams(ops):
+    """More streams than a workgroup sums by itself (two launches), replayed with other lengths."""
+    g, r = _gen(82), 5000
+    lengths = torch.randint(0, 9, (r,), generator=g, device="cuda", dtype=torch.int32)
+    first = torch.randint(0, 4000, (r,), generator=g, device="cuda", dtype=torch.int32)
+    table = torch.randint(0, 99999, (r, 3), generator=g, device="cuda", dtype=torch.int32)
+    rows = torch.full((9 * r, 2), -7, dtype=torch.int32, device="cuda")
+    starts = torch.empty(r + 1, dtype=torch.int32, device="cuda")
+    ops.frame_map(lengths, first, table, 32, rows, starts=starts, offsets=(-3, 0))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.frame_map(lengths, first, table, 32, rows, starts=starts, offsets=(-3, 0))
+    for i in range(4):
+        lengths.copy_(torch.randint(0, 9, (r,), generator=g, device="cuda", dtype=torch.int32))
+        rows.fill_(-7)
+        graph.replay()
+        want = torch.full_like(rows, -7)
+        want_starts, _ = ops.frame_map(lengths, first, table, 32, want, offsets=(-3, 0))
+        assert torch.equal(starts, want_starts) and torch.equal(rows, want), i
+
+
+def test_numbers_that_do_not_fit_are_refused(ops):
+    g = _gen(83)
+    codes, scales = ops.quantize_rows(_randn(g, 3, 64))
+    w, ws = ops.quantize_weight(_randn(g, 5, 64))
+    for bad in ("1", 1e39, None):
+        with pytest.raises(ValueError, match="residual_scale"):
+            ops.linear_int8(codes, w, ws, scale=scales, residual_scale=bad)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.linear_int8(codes, w, ws.clone().requires_grad_(), scale=scales)

@@ -42,16 +42,6 @@ struct QuantizeRows {
 };
 void LaunchQuantizeRows(const QuantizeRows& a, hipStream_t s);
 
-// Which cache rows the output rows of a step read.  Stream r has lengths[r]
-// new frames from time first[r] on and gives n_r = ceil(lengths[r] / step)
-// output rows, at times first[r] + step * i; output rows are packed stream
-// after stream (starts = exclusive sums of n_r, the total last).  Frame t of
-// stream r lies in cache row
-//   table[r][(t mod ring) / page] * page_stride + (t mod page) * frame_stride,
-// ring = pages * page.  Entry (row, j) names the row of frame t + offset[j],
-// t limited to [low[r], high[r]] (clamp: the nearest inside, else -1), -1
-// where the page is not assigned or the ring cannot hold the frame beside
-// the newest that the stream's rows name.
 // Division by a number that is fixed for the launch: the high word of a
 // product with a rounded reciprocal (Granlund and Montgomery, "Division by
 // invariant integers using multiplication", 1994; exact for all 32-bit n).
@@ -73,6 +63,16 @@ struct Divider {
   __host__ __device__ uint32_t mod(uint32_t n) const { return n - div(n) * d; }
 };
 
+// Which cache rows the output rows of a step read.  Stream r has lengths[r]
+// new frames from time first[r] on and gives n_r = ceil(lengths[r] / step)
+// output rows, at times first[r] + step * i; output rows are packed stream
+// after stream (starts = exclusive sums of n_r, the total last).  Frame t of
+// stream r lies in cache row
+//   table[r][(t mod ring) / page] * page_stride + (t mod page) * frame_stride,
+// ring = pages * page.  Entry (row, j) names the row of frame t + offset[j],
+// t limited to [low[r], high[r]] (clamp: the nearest inside, else -1), -1
+// where the page is not assigned, the ring cannot hold the frame beside the
+// newest that the stream's rows name, or the row's number passes 31 bits.
 struct FrameMap {
   const int* lengths;
   const int* first;

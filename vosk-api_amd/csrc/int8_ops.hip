@@ -56,6 +56,15 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top) {  // top: the large
   return r;
 }
 
+// A launch has less than 2^32 threads a dimension: more workgroups than kGridX
+// go into the next (a multiple of 8, which keeps block_id & 7 the XCD).
+constexpr long long kGridX = 1 << 22;
+__device__ __forceinline__ long long block_id() { return blockIdx.y * kGridX + blockIdx.x; }
+dim3 Grid(long long blocks) {
+  if (blocks > INT_MAX) VAMD_ERR("too many workgroups for one launch: " << blocks);
+  return blocks <= kGridX ? dim3((unsigned)blocks) : dim3((unsigned)kGridX, (unsigned)((blocks + kGridX - 1) / kGridX));
+}
+
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -150,7 +159,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeRows a) {
   constexpr int N = Chunk<TYPE>::N;
   __shared__ uint32_t part[4];
   const int tid = threadIdx.x % TPR;
-  const long long m = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const long long m = block_id() * (256 / TPR) + threadIdx.x / TPR;
   long long to = -1;
   long long from = m;
   if (m < a.m && !(a.count && m >= *a.count)) {
@@ -197,19 +206,20 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeRows a) {
 }
 
 template <int TYPE>
-void LaunchQuantize(const QuantizeRows& a, unsigned rows4, hipStream_t s) {
+void LaunchQuantize(const QuantizeRows& a, hipStream_t s) {
   constexpr int N = Chunk<TYPE>::N;
   const int kp = Int8Padded(a.k);
+  const dim3 rows4 = Grid((a.m + 3) / 4), rows1 = Grid(a.m);
   // a wave a row as long as it fits its registers; with too few rows to fill
   // the chip so, four waves share the longer ones
-  if (kp <= 64 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 1>), dim3(rows4), dim3(256), 0, s, a);
-  else if (kp <= 64 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 2>), dim3(rows4), dim3(256), 0, s, a);
-  else if (kp <= 64 * 4 * N && a.m > 2048) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 4>), dim3(rows4), dim3(256), 0, s, a);
-  else if (kp <= 64 * 8 * N && a.m > 2048) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 8>), dim3(rows4), dim3(256), 0, s, a);
-  else if (kp <= 256 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 2>), dim3((unsigned)a.m), dim3(256), 0, s, a);
-  else if (kp <= 256 * 4 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 4>), dim3((unsigned)a.m), dim3(256), 0, s, a);
-  else if (kp <= 256 * 8 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 8>), dim3((unsigned)a.m), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 0>), dim3((unsigned)a.m), dim3(256), 0, s, a);
+  if (kp <= 64 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 1>), rows4, dim3(256), 0, s, a);
+  else if (kp <= 64 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 2>), rows4, dim3(256), 0, s, a);
+  else if (kp <= 64 * 4 * N && a.m > 2048) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 4>), rows4, dim3(256), 0, s, a);
+  else if (kp <= 64 * 8 * N && a.m > 2048) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 8>), rows4, dim3(256), 0, s, a);
+  else if (kp <= 256 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 2>), rows1, dim3(256), 0, s, a);
+  else if (kp <= 256 * 4 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 4>), rows1, dim3(256), 0, s, a);
+  else if (kp <= 256 * 8 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 8>), rows1, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 0>), rows1, dim3(256), 0, s, a);
 }
 
 // ---- row maps
@@ -416,7 +426,9 @@ __global__ __launch_bounds__(kMapThreads) void frame_map_kernel(FrameMap a) {
         held = held && t >= oldest[i] && t <= high[i];
         const unsigned q = a.pages == 1 ? 0u : a.by_page.div(u);
         const int pg = held ? a.table[r[i] * a.ldt + q] : -1;
-        if (pg >= 0) to[i][j] = pg * a.page_stride + (int)(u - q * (unsigned)a.page) * a.frame_stride;
+        const uint64_t row = (uint64_t)(unsigned)pg * (unsigned)a.page_stride +
+                             (uint64_t)(u - q * (unsigned)a.page) * (unsigned)a.frame_stride;
+        if (pg >= 0 && row <= INT_MAX) to[i][j] = (int)row;
       }
 #pragma unroll
     for (int i = 0; i < ROWS; i++)
@@ -571,8 +583,11 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   // workgroups b, b + 8, ... run on one XCD: each XCD gets neighbouring tiles
   // (GROUP rows of tiles, column after column), whose rows its L2 reads once
   constexpr int GROUP = 4;
-  const int tiles = tiles_m * tiles_n, xcd = blockIdx.x & 7;
-  const int t = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (blockIdx.x >> 3);
+  const int tiles = tiles_m * tiles_n;
+  const long long block = block_id();
+  if (block >= tiles) return;
+  const int xcd = (int)(block & 7);
+  const int t = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (int)(block >> 3);
   const int g0 = t / (GROUP * tiles_n) * GROUP, gm = min(GROUP, tiles_m - g0), gt = t - g0 * tiles_n;
   const int m0 = (g0 + gt % gm) * TM, n0 = gt / gm * TN;
   // which row each output row reads; those past the count, which is not known yet, as well
@@ -932,20 +947,13 @@ void AskLds(const void* kernel, size_t bytes) {
     VAMD_ERR("the device does not give a workgroup " << bytes << " bytes of LDS");
 }
 
-unsigned Blocks(long long n, long long per) {
-  const long long b = (n + per - 1) / per;
-  if (b > INT_MAX) VAMD_ERR("too many rows for one launch: " << n);
-  return (unsigned)b;
-}
-
 }  // namespace
 
 void LaunchQuantizeRows(const QuantizeRows& a, hipStream_t s) {
   if (a.m <= 0) return;
-  const unsigned rows4 = Blocks(a.m, 4);
-  if (a.type == kFloat32) LaunchQuantize<kFloat32>(a, rows4, s);
-  else if (a.type == kFloat16) LaunchQuantize<kFloat16>(a, rows4, s);
-  else LaunchQuantize<kBFloat16>(a, rows4, s);
+  if (a.type == kFloat32) LaunchQuantize<kFloat32>(a, s);
+  else if (a.type == kFloat16) LaunchQuantize<kFloat16>(a, s);
+  else LaunchQuantize<kBFloat16>(a, s);
 }
 
 void SetOffsets(FrameMap* a, const int* offsets) {
@@ -984,13 +992,12 @@ namespace {
 template <int TM, int TN, int WM, int WN, int ST, int KB, bool MULTI>
 void LaunchTile(const LinearInt8& a, hipStream_t s) {
   const long long tm = ((long long)a.m + TM - 1) / TM, tn = ((long long)a.n + TN - 1) / TN;
-  if (tm * tn > INT_MAX) VAMD_ERR("too many tiles for one launch: " << a.m << " x " << a.n);
   const size_t lds = ST * KB * (TM + TN) * kPartBytes + (size_t)TM * 4 * (a.taps * (MULTI ? 2 : 1) + (a.out_to ? 1 : 0) + (a.res_from ? 1 : 0));
   const bool mapped = a.out_to || a.res_from;
   auto kernel = mapped ? linear_tile_kernel<TM, TN, WM, WN, ST, KB, MULTI, true>
                        : linear_tile_kernel<TM, TN, WM, WN, ST, KB, MULTI, false>;
   AskLds((const void*)kernel, lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, s, a, (int)tm, (int)tn);
+  hipLaunchKernelGGL(kernel, Grid(tm * tn), dim3(64 * WM * WN), lds, s, a, (int)tm, (int)tn);
 }
 
 }  // namespace

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <climits>
+#include <cmath>
 
 #include "common.h"
 #include "int8_ops.h"
@@ -75,6 +76,7 @@ alignas(16) char kNoWorkspace[16];
 void CheckLinear(const LinearInt8& a) {
   Want(a.taps >= 1 && a.taps <= kMaxTaps, "linear_int8: 1 to 16 taps");
   Want(FloatTypeOk(a.out_type), "linear_int8: unknown output type");
+  Want(std::isfinite(a.res_scale), "linear_int8: residual_scale has to be finite");
   if (a.m == 0 || a.n == 0) return;
   const long long kb = Int8Padded(a.k);
   Want(a.a && a.sa && a.w && a.sw && a.out, "linear_int8: null pointer");

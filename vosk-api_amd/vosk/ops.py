@@ -239,8 +239,8 @@ def frame_map(lengths, first, table, page, rows, starts=None, offsets=(0,), step
 
     low, high (int32 [R], optional): the first and last frame a stream has; a
     frame outside is replaced by the nearest one inside (clamp) or is absent.
-    Entry -1: absent, a negative page number, or a frame the ring cannot hold
-    beside the newest one that the stream's rows name.  Rows from the total
+    Entry -1: absent, a negative page number, a frame the ring cannot hold
+    beside the newest one that the stream's rows name, a row past 2^31 - 1.  Rows from the total
     on are left as they were; rows past cap are not written.
     strides = (page_stride, frame_stride), by default (page, 1): frame t lies in
     row table[...] * page_stride + (t mod page) * frame_stride.
@@ -284,7 +284,7 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     optional.  The inner sums are exact, the rest is 32-bit floats, rounded
     once to out's type.
 
-    weight: int8 [N, J * code_bytes(K)], weight_scale: float32 [N]
+    weight: int8 [N, J * code_bytes(K)] in -127 .. 127, weight_scale: float32 [N]
     (quantize_weight).  x is either int8 codes [C, code_bytes(K)] with scale
     float32 [C] (quantize_rows), or float rows [C, K] that are quantised in
     the call, to the same codes.  rows (int32 [M, J], frame_map) says which
@@ -329,7 +329,7 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
             _refuse("rows has to have 1 to %d columns" % MAX_TAPS)
     if wk != taps * kb:
         _refuse("weight has to have %d columns" % (taps * kb))
-    _no_grad(x, residual, out, bias, gain, shift)
+    _no_grad(x, scale, weight_scale, residual, out, bias, gain, shift)
     qp = ldr = rt = ep = lde = rr = 0
     if residual is not None:
         qp, rm, rn, ldr = _matrix(residual, "residual", dev)
@@ -367,10 +367,14 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
         if size:
             ws = torch.empty(size, dtype=_i8, device=x.device)
             wsp = ws.data_ptr()
-    if _c.vamd_op_linear_int8(dev, _raw_stream(dev), _LINEAR(
-            cp, sp, rp, _vector(count, "count", _i32, 1, dev), xp, wsp, wp,
-            _vector(weight_scale, "weight_scale", _f32, n, dev), _vector(bias, "bias", _f32, n, dev),
-            _vector(gain, "gain", _f32, n, dev), _vector(shift, "shift", _f32, n, dev), qp, op, tp, ep,
-            c, lda, ldx, ldw, ldr, ldo, ldi, ldto, orows, lde, rr, m, n, k, taps, 1 if relu else 0, xt, rt, _TYPES[out.dtype], residual_scale)) < 0:
+    try:
+        args = _LINEAR(cp, sp, rp, _vector(count, "count", _i32, 1, dev), xp, wsp, wp,
+                       _vector(weight_scale, "weight_scale", _f32, n, dev), _vector(bias, "bias", _f32, n, dev),
+                       _vector(gain, "gain", _f32, n, dev), _vector(shift, "shift", _f32, n, dev), qp, op, tp, ep,
+                       c, lda, ldx, ldw, ldr, ldo, ldi, ldto, orows, lde, rr, m, n, k, taps, 1 if relu else 0, xt, rt,
+                       _TYPES[out.dtype], residual_scale)
+    except struct.error:
+        _refuse("residual_scale has to be a number")
+    if _c.vamd_op_linear_int8(dev, _raw_stream(dev), args) < 0:
         _chk(-1)
     return out
