@@ -481,6 +481,13 @@ __device__ __forceinline__ void wait_last(int behind) {
   }
 }
 
+// a wave's own loads alone: until `behind` <= B steps of LOADS loads are left
+template <int B, int LOADS>
+__device__ __forceinline__ void wait_own(int behind) {
+  if (B == 0 || behind >= B) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(B * LOADS) : "memory");
+  else wait_own<(B > 0 ? B - 1 : 0), LOADS>(behind);
+}
+
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
@@ -560,6 +567,22 @@ __device__ __forceinline__ void finish_16(const LinearInt8& a, float (&v)[16], c
 #pragma unroll
     for (int i = 0; i < 16; i++) v[i] = a.res_scale * z[i] + v[i];
   }
+}
+
+// The same for one value
+__device__ __forceinline__ void finish_one(const LinearInt8& a, float v, const Column& c, int m, int n) {
+  float y = v * c.sw;
+  if (a.bias) y = y + c.bias;
+  if (a.relu) y = y < 0.0f ? 0.0f : y;
+  if (a.gain) y = y * c.gain + c.shift;
+  if (a.residual) {
+    const int from = a.res_from ? a.res_from[m * a.ldres_from] : m;
+    const bool there = from >= 0 && from < a.res_rows;
+    const float z = load_float(a.residual, a.res_type, (there ? from : 0) * a.ldr + n);
+    y = a.res_scale * (there ? z : 0.0f) + y;
+  }
+  const int to = a.out_to ? a.out_to[m * a.ldout_to] : m;
+  if (to >= 0 && to < a.out_rows) store_float(a.out, a.out_type, to * a.ldo + n, y);
 }
 
 // (two waves a SIMD leave 256 registers a wave: the accumulators then stay
@@ -769,61 +792,116 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   }
 }
 
-// ---- few rows
+// ---- narrow tiles
 //
-// The weights are what there is to read: a workgroup takes 16 columns, its
-// eight waves share the K steps (64 bytes of 16 weight rows each, straight
-// into v_mfma_i32_16x16x64_i8: lane l holds row / column l & 15, bytes
-// 16 * (l >> 4) of the step) and their integer sums are joined in LDS.  The
-// rows of codes lie in LDS whole; float rows are quantised there by the
-// workgroup itself, each workgroup for itself, which costs less than a launch
-// before this one.  A first batch of weight loads is on its way meanwhile.
-constexpr int kFewWaves = 8, kFewThreads = 64 * kFewWaves;
+// Few columns a workgroup, so that the chip is full where 64 x 64 tiles are
+// few: a tile of 16 * RT rows and 16 * CT columns in 16 x 16 blocks of
+// v_mfma_i32_16x16x64_i8 (lane l holds row / column l & 15, bytes 16 * (l >> 4)
+// of a step), whose K steps of 64 bytes the eight waves share.  No two waves
+// read the same bytes, so each has a ring of ST steps in LDS of its own and
+// waits for nobody until the waves' integer sums are joined, tap by tap.
+// (Loaded straight into registers as the matrix instruction takes them, four
+// neighbouring lanes read four rows, and a CU takes in 13 bytes a cycle instead
+// of 21: 64 x 4096 x 4096 10.8 us against 7.6.)
+// Rows of floats (TYPE >= 0; RT blocks cover all rows then) are quantised in
+// LDS by the workgroup itself, each for itself, while its first weights are on
+// their way.
+constexpr int kNarrowWaves = 8, kNarrowThreads = 64 * kNarrowWaves;
 constexpr int kFusedValues = 16384;  // float values (rows x taps x padded columns) that a workgroup quantises itself
 
-template <int TYPE, int RT, int VALUES>  // TYPE < 0: codes, else up to VALUES float values; RT blocks of 16 rows
-__global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, QuantizeRows x) {
-  constexpr int R = 16 * RT, AHEAD = 4;
-  extern __shared__ char smem[];  // codes [R][ldl], partial sums [8][RT][256], scales [taps][R], maxima [taps][R]
-  const int kk = a.k * a.taps, ldl = kk + 16;  // 16 bytes on: rows in other banks
-  int* const part = (int*)(smem + R * ldl);
-  float* const sscale = (float*)(part + kFewWaves * RT * 256);
-  uint32_t* const smax = (uint32_t*)(sscale + a.taps * R);
+template <int TYPE, int RT, int CT, int ST, int VALUES>  // TYPE < 0: codes, else up to VALUES float values
+__global__ __launch_bounds__(kNarrowThreads) void linear_narrow_kernel(LinearInt8 a, QuantizeRows x, int tiles_m, int tiles_n) {
+  constexpr bool FLOATS = TYPE >= 0;
+  constexpr int R = 16 * RT, BLOCKS = RT * CT, LOADS = (FLOATS ? 0 : RT) + CT;
+  // rings [8][ST][LOADS][16][64], sums [8][BLOCKS][256], scales [taps][R], codes: rows [taps][R]; floats: maxima
+  // [taps][R] as bits, codes [m][ldl]
+  extern __shared__ char smem[];
+  int* const part = (int*)(smem + kNarrowWaves * ST * LOADS * 1024);
+  float* const sscale = (float*)(part + kNarrowWaves * BLOCKS * 256);
+  int* const srow = (int*)(sscale + a.taps * R);
+  uint32_t* const smax = (uint32_t*)srow;
+  char* const scode = (char*)(smax + a.taps * R);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int mrows = a.count ? min(a.m, *a.count) : a.m;
-  const int n0 = blockIdx.x * 16;
-  if (mrows <= 0) return;
-
-  const int steps = kk / 64;
-  const int8_t* const wp = a.w + (long long)min(n0 + (lane & 15), a.n - 1) * a.ldw + 16 * (lane >> 4);
-  intx4 w[AHEAD];
+  // an XCD's tiles are neighbours, the rows of a column first: its L2 reads the weights once
+  const int tiles = tiles_m * tiles_n;
+  const long long block = block_id();
+  if (block >= tiles) return;
+  const int xcd = (int)(block & 7), t = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (int)(block >> 3);
+  const int m0 = t % tiles_m * R, n0 = t / tiles_m * 16 * CT;
+  auto row_of = [&](int m, int tap) {  // -1: adds nothing
+    const int row = m < a.m ? a.rows ? a.rows[m * a.ldrows + tap] : m : -1;
+    return row < a.arows ? row : -1;
+  };
+  const int kt = a.k / kPartBytes, steps = kt * a.taps;
+  // a load: 16 rows, lane l row l >> 2, chunk slot l & 3; absent rows read row 0
+  const int lrow = lane >> 2, chunk = 16 * ((lane & 3) ^ ((lrow >> 2) & 3));
+  const int8_t* wp[CT];
 #pragma unroll
-  for (int i = 0; i < AHEAD; i++) {
-    const int s = wave + kFewWaves * i;
-    if (s < steps) w[i] = *reinterpret_cast<const intx4*>(wp + 64 * s);
+  for (int c = 0; c < CT; c++) wp[c] = a.w + (long long)min(n0 + 16 * c + lrow, a.n - 1) * a.ldw + chunk;
+  const int8_t* p[RT];  // of the tap of the last load
+  int itap = 0;
+  if (!FLOATS) {
+    while ((itap + 1) * kt <= wave) itap++;
+#pragma unroll
+    for (int b = 0; b < RT; b++)
+      p[b] = a.a + max(row_of(m0 + 16 * b + lrow, min(itap, a.taps - 1)), 0) * a.lda + chunk;
   }
+  const int mrows = a.count ? min(a.m, *a.count) : a.m;
+  if (m0 >= mrows) return;
+  if (!FLOATS && a.taps > 1) {
+    for (int i = tid; i < a.taps * R; i += kNarrowThreads) srow[i] = max(row_of(m0 + i % R, i / R), 0);
+    __syncthreads();
+  }
+  const uint32_t ring = lds_address(smem) + wave * ST * LOADS * 1024;
+  int is = wave, ibuf = 0, issued = 0;
+  auto issue = [&] {
+    const uint32_t to = ring + ibuf * LOADS * 1024;
+    if (!FLOATS) {
+      if (is >= (itap + 1) * kt) {
+        do itap++;
+        while (is >= (itap + 1) * kt);
+#pragma unroll
+        for (int b = 0; b < RT; b++) p[b] = a.a + (long long)srow[itap * R + 16 * b + lrow] * a.lda + chunk;
+      }
+#pragma unroll
+      for (int b = 0; b < RT; b++) load_to_lds(p[b] + kPartBytes * (is - itap * kt), to + (CT + b) * 1024);
+    }
+#pragma unroll
+    for (int c = 0; c < CT; c++) load_to_lds(wp[c] + kPartBytes * is, to + c * 1024);
+    ibuf = ibuf + 1 == ST ? 0 : ibuf + 1;
+    is += kNarrowWaves;
+    issued++;
+  };
+  for (int i = 0; i < ST - 1 && is < steps; i++) issue();
+  // value i of a thread: t = tid + 512 * i of the blocks' 256 each, row t >> 4, column t & 15
+  constexpr int EACH = (BLOCKS * 256 + kNarrowThreads - 1) / kNarrowThreads;
+  auto row_in = [&](int i) { return ((tid + i * kNarrowThreads) >> 8) / CT * 16 + (tid >> 4 & 15); };
+  auto col_in = [&](int i) { return ((tid + i * kNarrowThreads) >> 8) % CT * 16 + (tid & 15); };
+  Column col[CT > 1 ? EACH : 1];
+#pragma unroll
+  for (int i = 0; i < (CT > 1 ? EACH : 1); i++) col[i] = column(a, min(n0 + col_in(i), a.n - 1));
 
-  const Column col = column(a, min(n0 + (tid & 15), a.n - 1));  // of the values below
-  auto row_of = [&](int q) { return a.taps == 1 ? q : q / a.taps; };  // of tap q of all rows
-  if constexpr (TYPE >= 0) {
-    constexpr int N = Chunk<TYPE < 0 ? 0 : TYPE>::N;
+  const int ldl = steps * kPartBytes + 16;  // 16 bytes on: rows in other banks
+  if constexpr (FLOATS) {
+    constexpr int N = Chunk<TYPE>::N;
     // all chunks of all rows of all taps stay in registers (LinearFloatFused)
     const int chunks = a.k / N, all = mrows * a.taps * chunks;  // past a row's end: zeros
-    constexpr int HELD = VALUES / (kFewThreads * N);
-    Chunk<TYPE < 0 ? 0 : TYPE> c[HELD];
+    constexpr int HELD = VALUES / (kNarrowThreads * N);
+    auto row_of_tap = [&](int q) { return a.taps == 1 ? q : q / a.taps; };  // of tap q of all rows
+    Chunk<TYPE> c[HELD];
     int place[HELD];  // tap * R + row; -1: the row is absent
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
-      const int u = tid + i * kFewThreads, q = u / chunks, m = row_of(q), j = q - m * a.taps;
+      const int u = tid + i * kNarrowThreads, q = u / chunks, m = row_of_tap(q), j = q - m * a.taps;
       place[i] = -1;
       if (u >= all) continue;
-      const int row = a.rows ? a.rows[m * a.ldrows + j] : m;
-      if (row >= 0 && row < a.arows) {
+      const int row = row_of(m, j);
+      if (row >= 0) {
         place[i] = j * R + m;
         c[i].load(x.x, row * x.ldx, (u - q * chunks) * N, x.k);
       }
     }
-    for (int i = tid; i < a.taps * R; i += kFewThreads) smax[i] = 0;
+    for (int i = tid; i < a.taps * R; i += kNarrowThreads) smax[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
@@ -840,103 +918,87 @@ __global__ __launch_bounds__(kFewThreads) void linear_few_kernel(LinearInt8 a, Q
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
-      const int u = tid + i * kFewThreads, q = u / chunks, m = row_of(q), j = q - m * a.taps, e = (u - q * chunks) * N;
+      const int u = tid + i * kNarrowThreads, q = u / chunks, m = row_of_tap(q), j = q - m * a.taps, e = (u - q * chunks) * N;
       if (u >= all) break;
       if (place[i] >= 0) {
         const RowScale r = row_scale(smax[place[i]]);
-        c[i].store((int8_t*)smem + m * ldl + j * a.k + e, r);
+        c[i].store((int8_t*)scode + m * ldl + j * a.k + e, r);
         if (e == 0) sscale[place[i]] = r.scale;
       } else if (e == 0) {
         sscale[j * R + m] = 0.0f;  // (whatever its codes: the sum of them is finite)
       }
     }
+    __syncthreads();
   } else {
-    const int chunks = a.k / 16, all = mrows * a.taps * chunks;
-    for (int i = tid; i < all; i += kFewThreads) {
-      const int q = i / chunks, e = (i - q * chunks) * 16, m = row_of(q), j = q - m * a.taps;
-      long long row = a.rows ? a.rows[m * a.ldrows + j] : m;
-      const bool there = row >= 0 && row < a.arows;
-      if (!there) row = 0;
-      *reinterpret_cast<intx4*>(smem + m * ldl + j * a.k + e) = *reinterpret_cast<const intx4*>(a.a + row * a.lda + e);
-      if (e == 0) sscale[j * R + m] = there ? a.sa[row] : 0.0f;
+    for (int i = tid; i < a.taps * R; i += kNarrowThreads) {  // read behind a join's barrier
+      const int row = row_of(m0 + i % R, i / R);
+      sscale[i] = row >= 0 ? a.sa[row] : 0.0f;
     }
   }
-  __syncthreads();
 
-  // element t of the 16 x 16 blocks: row t >> 4, column t & 15
-  constexpr int EACH = (RT * 256 + kFewThreads - 1) / kFewThreads;
   float v[EACH];
 #pragma unroll
   for (int i = 0; i < EACH; i++) v[i] = 0.0f;
-  intx4 acc[RT];
+  intx4 acc[RT][CT];
 #pragma unroll
-  for (int t = 0; t < RT; t++) acc[t] = intx4{0, 0, 0, 0};
-  const int kt = a.k / 64;
-  const char* const ap = smem + (lane & 15) * ldl + 16 * (lane >> 4);
+  for (int b = 0; b < RT; b++)
+#pragma unroll
+    for (int c = 0; c < CT; c++) acc[b][c] = intx4{0, 0, 0, 0};
   int tap = 0, end = kt;  // the tap's steps end there
   auto join = [&] {       // the tap's integer sums, then the row's scale
     if (tap) __syncthreads();
 #pragma unroll
-    for (int t = 0; t < RT; t++)
+    for (int b = 0; b < RT; b++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        part[(wave * RT + t) * 256 + ((lane >> 4) * 4 + i) * 16 + (lane & 15)] = acc[t][i];
-        acc[t][i] = 0;
-      }
+      for (int c = 0; c < CT; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          part[((wave * RT + b) * CT + c) * 256 + ((lane >> 4) * 4 + i) * 16 + (lane & 15)] = acc[b][c][i];
+          acc[b][c][i] = 0;
+        }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
-      const int t = tid + i * kFewThreads;
-      if (t < RT * 256) {
+      const int e = tid + i * kNarrowThreads;
+      if (e < BLOCKS * 256) {
         int sum = 0;
 #pragma unroll
-        for (int u = 0; u < kFewWaves; u++) sum += part[u * RT * 256 + t];
-        v[i] = fmaf((float)sum, sscale[tap * R + (t >> 4)], v[i]);
+        for (int u = 0; u < kNarrowWaves; u++) sum += part[u * BLOCKS * 256 + e];
+        v[i] = fmaf((float)sum, sscale[tap * R + row_in(i)], v[i]);
       }
     }
     tap++;
     end += kt;
   };
-  for (int s0 = wave; s0 < steps; s0 += kFewWaves * AHEAD) {
+  const int r16 = lane & 15;
+  const char* const own = smem + wave * ST * LOADS * 1024 + r16 * kPartBytes + 16 * ((lane >> 4) ^ ((r16 >> 2) & 3));
+  const char* held[RT];  // floats: a lane's row, one that is not there the last one (its sums are not used)
+#pragma unroll
+  for (int b = 0; b < RT; b++) held[b] = scode + min(16 * b + r16, mrows - 1) * ldl + 16 * (lane >> 4);
+  int buf = 0, done = 0;
+  for (int s = wave; s < steps; s += kNarrowWaves) {
     // (a wave joins a tap when it is past it: every wave joins every tap once, in order)
-    intx4 u[AHEAD];
+    while (s >= end) join();
+    wait_own<ST - 2, LOADS>(issued - ++done);
+    if (is < steps) issue();  // over the step before, whose reads are done
+    const char* const at = own + buf * LOADS * 1024;
+    intx4 fa[RT], fb[CT];
 #pragma unroll
-    for (int i = 0; i < AHEAD; i++) {
-      u[i] = w[i];
-      const int s = s0 + kFewWaves * (AHEAD + i);
-      if (s < steps) w[i] = *reinterpret_cast<const intx4*>(wp + 64 * s);
-    }
+    for (int b = 0; b < RT; b++)
+      fa[b] = *reinterpret_cast<const intx4*>(FLOATS ? held[b] + kPartBytes * s : at + (CT + b) * 1024);
 #pragma unroll
-    for (int i = 0; i < AHEAD; i++) {
-      const int s = s0 + kFewWaves * i;
-      while (tap < a.taps && s >= end) join();
-      if (s < steps) {
+    for (int c = 0; c < CT; c++) fb[c] = *reinterpret_cast<const intx4*>(at + c * 1024);
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-          const intx4 f = *reinterpret_cast<const intx4*>(ap + t * 16 * ldl + 64 * s);
-          acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, u[i], acc[t], 0, 0, 0);
-        }
-      }
-    }
+    for (int b = 0; b < RT; b++)
+#pragma unroll
+      for (int c = 0; c < CT; c++) acc[b][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[b], fb[c], acc[b][c], 0, 0, 0);
+    buf = buf + 1 == ST ? 0 : buf + 1;
   }
   while (tap < a.taps) join();
-
 #pragma unroll
   for (int i = 0; i < EACH; i++) {
-    const int t = tid + i * kFewThreads, m = t >> 4, n = n0 + (t & 15);
-    if (t >= RT * 256 || m >= mrows || n >= a.n) continue;
-    float y = v[i] * col.sw;
-    if (a.bias) y = y + col.bias;
-    if (a.relu) y = y < 0.0f ? 0.0f : y;
-    if (a.gain) y = y * col.gain + col.shift;
-    if (a.residual) {
-      const int from = a.res_from ? a.res_from[m * a.ldres_from] : m;
-      const bool there = from >= 0 && from < a.res_rows;
-      const float z = load_float(a.residual, a.res_type, (there ? from : 0) * a.ldr + n);
-      y = a.res_scale * (there ? z : 0.0f) + y;
-    }
-    const int to = a.out_to ? a.out_to[m * a.ldout_to] : m;
-    if (to >= 0 && to < a.out_rows) store_float(a.out, a.out_type, to * a.ldo + n, y);
+    const int m = m0 + row_in(i), n = n0 + col_in(i);
+    if (tid + i * kNarrowThreads < BLOCKS * 256 && m < mrows && n < a.n) finish_one(a, v[i], col[CT > 1 ? i : 0], m, n);
   }
 }
 
@@ -1004,10 +1066,10 @@ void LaunchTile(const LinearInt8& a, hipStream_t s) {
 
 namespace {
 
-// 64 x 64 tiles: the longer K is, the more of it a step (us, 1 / 2 / 4 parts):
-// 4352 x 512 x 96 5.6 / 5.5 / 6.8, 128 x 96 x 1024 6.2 / 5.6 / 5.2; four parts
-// take 64 KB of LDS, which more than two tiles a CU miss: 4352 x 512 x 1024
-// (544 tiles) 9.1 / 8.6 / 10.4.
+// 64 x 64 tiles: the longer K is, the more of it a step (us in a graph, 1 / 2 /
+// 4 parts): 4352 x 512 x 96 5.6 / 5.6 / 7.0, 2048 x 512 x 1024 6.8 / 6.6 / 6.1;
+// four parts take 64 KB of LDS, which more than two tiles a CU miss: 4352 x 512
+// x 1024 (544 tiles) 9.1 / 8.6 / 10.5.
 template <bool MULTI>
 void LaunchSmallTiles(const LinearInt8& a, long long tiles, hipStream_t s) {
   if (a.k * a.taps < 512) LaunchTile<64, 64, 2, 2, 3, 1, MULTI>(a, s);
@@ -1015,51 +1077,40 @@ void LaunchSmallTiles(const LinearInt8& a, long long tiles, hipStream_t s) {
   else LaunchTile<64, 64, 2, 2, 3, 2, MULTI>(a, s);
 }
 
-size_t FewLds(int m, int k, int taps) {
-  const size_t rt = m <= 16 ? 1 : 2;
-  return rt * 16 * ((size_t)k * taps + 16) + kFewWaves * rt * 1024 + rt * 16 * 4 * 2 * taps;
-}
-
-template <int TYPE, int RT, int VALUES>
-void LaunchFew(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
-  auto kernel = linear_few_kernel<TYPE, RT, VALUES>;
-  const size_t lds = FewLds(a.m, a.k, a.taps);
+template <int TYPE, int RT, int CT, int ST, int VALUES>
+void LaunchNarrow(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
+  const long long tm = ((long long)a.m + 16 * RT - 1) / (16 * RT), tn = ((long long)a.n + 16 * CT - 1) / (16 * CT);
+  const size_t lds = kNarrowWaves * (RT * CT + ST * ((TYPE < 0 ? RT : 0) + CT)) * 1024 + 16 * RT * a.taps * 8 +
+                     (TYPE < 0 ? 0 : (size_t)a.m * ((size_t)a.k * a.taps + 16));
+  auto kernel = linear_narrow_kernel<TYPE, RT, CT, ST, VALUES>;
   AskLds((const void*)kernel, lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((a.n + 15) / 16)), dim3(kFewThreads), lds, s, a, x);
+  hipLaunchKernelGGL(kernel, Grid(tm * tn), dim3(kNarrowThreads), lds, s, a, x, (int)tm, (int)tn);
 }
 
 template <int TYPE>
-void LaunchFewRows(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
+void LaunchFused(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
   const bool more = (long long)a.m * a.taps * a.k > kFusedValues / 4;
-  if (a.m <= 16 && more) LaunchFew<TYPE, 1, kFusedValues>(a, x, s);
-  else if (a.m <= 16) LaunchFew<TYPE, 1, kFusedValues / 4>(a, x, s);
-  else if (more) LaunchFew<TYPE, 2, kFusedValues>(a, x, s);
-  else LaunchFew<TYPE, 2, kFusedValues / 4>(a, x, s);
+  if (a.m <= 16 && more) LaunchNarrow<TYPE, 1, 1, 4, kFusedValues>(a, x, s);
+  else if (a.m <= 16) LaunchNarrow<TYPE, 1, 1, 4, kFusedValues / 4>(a, x, s);
+  else if (more) LaunchNarrow<TYPE, 2, 1, 4, kFusedValues>(a, x, s);
+  else LaunchNarrow<TYPE, 2, 1, 4, kFusedValues / 4>(a, x, s);
 }
 
 }  // namespace
 
-// Up to 32 rows (us in a graph, few / tiles, rows x k x n: 32 x 192 x 2000 3.2 /
-// 4.4, 32 x 1024 x 96 4.4 / 6.0, 64 x 512 x 512 5.5 / 3.9), as long as copying
-// them to LDS in every workgroup is little beside the weights: 17 x 4096 x 4096
-// 8.6 / 11.2, but 32 x 4096 x 4096 13.4 / 11.2.
-bool LinearFewRows(int m, int k, int taps) {
-  return m <= 32 && (long long)m * k * taps <= 96 * 1024 && FewLds(m, k, taps) <= 160 * 1024;
-}
-
 // Each workgroup quantises all rows: one launch up to 16384 values, which a
-// program that calls it from Python gets back (us, one call / two: 4 x 4096 x
-// 4096 10.1 / 16.0, 16 x 1024 x 1024 8.2 / 15.7), and which costs little in a
-// graph (4 x 4096 10.0 / 9.1, 17 x 512 5.8 / 5.9, 32 x 192 5.5 / 5.9, 16 x 1024
-// 7.5 / 6.9).
-bool LinearFloatFused(int m, int k, int taps) { return LinearFewRows(m, k, taps) && (long long)m * k * taps <= kFusedValues; }
+// program that calls it from Python gets back (us a call, one launch / two: 1 x
+// 4096 x 4096 7.1 / 11.6, 4 x 4096 x 4096 9.1 / 11.5, 16 x 1024 x 96 8.3 / 11.7)
+// and which costs little in a graph (1 x 4096 x 4096 5.6 / 6.9, 16 x 512 x 512
+// 5.6 / 5.6, 4 x 4096 x 4096 8.6 / 7.7, 32 x 512 x 512 7.7 / 5.7).
+bool LinearFloatFused(int m, int k, int taps) { return m <= 32 && (long long)m * k * taps <= kFusedValues; }
 
 void LaunchLinearFloat(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
   if (a.m <= 0 || a.n <= 0) return;
   if (LinearFloatFused(a.m, a.k, a.taps)) {
-    if (x.type == kFloat32) LaunchFewRows<kFloat32>(a, x, s);
-    else if (x.type == kFloat16) LaunchFewRows<kFloat16>(a, x, s);
-    else LaunchFewRows<kBFloat16>(a, x, s);
+    if (x.type == kFloat32) LaunchFused<kFloat32>(a, x, s);
+    else if (x.type == kFloat16) LaunchFused<kFloat16>(a, x, s);
+    else LaunchFused<kBFloat16>(a, x, s);
     return;
   }
   LaunchQuantizeRows(x, s);
@@ -1068,47 +1119,44 @@ void LaunchLinearFloat(const LinearInt8& a, const QuantizeRows& x, hipStream_t s
 
 void LaunchLinearInt8(const LinearInt8& a, hipStream_t s) {
   if (a.m <= 0 || a.n <= 0) return;
-  if (LinearFewRows(a.m, a.k, a.taps)) {
-    LaunchFewRows<-1>(a, QuantizeRows{}, s);
-    return;
-  }
-  // Tiles as large as leaves every CU one (us, 64 x 64 / 128 x 128 / 128 x 256 /
-  // 256 x 256 tiles, m x n x k):
-  //   1999 x 777 x 1001   6.8 /   8.9 /  11.7 /  16.6
-  //   4352 x 512 x 512    6.9 /   7.7 /   9.4 /  12.0
-  //   2048 x 2000 x 1024 13.3 /  12.2 /  14.4 /  19.1
-  //   4352 x 4096 x 1024 51.4 /  36.8 /  35.1 /  40.7
-  //   8192 x 4096 x 4096  278 /   187 /   157 /   130
-  //   4096 x 4096 x 4096  146 /    97 /    81 /    71
-  // but short products, which the stores bound, in the smallest:
-  //   13056 x 2000 x 96  21.0 /  22.5 /  23.2 /  22.8
-  // Several taps hold a second set of accumulators, which the larger tiles
-  // have no registers for; theirs gain from 128 x 128 at short K too
-  //   13056 x 512 x 2 * 96  12.4 / 10.5
-  // Tiles as large as leaves every CU one or more (us in a graph, 64 x 64 / 128 x
-  // 128 / 128 x 256 / 256 x 256 tiles, m x n x k):
-  //   1999 x 777 x 1001    7.3 /  9.6 / 13.0 / 18.6
-  //   4352 x 512 x 1024    8.6 /  9.6 / 12.9 / 18.0
-  //   2048 x 2000 x 512    9.4 /  9.0 / 10.8 / 13.3
-  //   13056 x 4096 x 1024  120 / 84.6 / 80.7 / 87.3
-  //   4352 x 2000 x 4096  67.4 / 58.9 / 63.5 / 54.8
-  //   8192 x 4096 x 4096   232 /  162 /  148 /  132
-  // but short products, which the stores bound, in the smallest:
-  //   4352 x 2000 x 192   10.5 / 13.5 / 12.3 / 12.2
-  // Several taps hold a second set of accumulators, for which the larger
-  // tiles have no registers; theirs gain from 128 x 128 at short K too:
-  //   13056 x 512 x 2 * 96  14.5 / 13.5
+  // Narrow tiles as long as no CU gets two, the smallest first (us in a graph,
+  // 16 x 16 / 32 x 16 / 32 x 32 / 64 x 64 tiles, m x n x k):
+  //   16 x 4096 x 4096    5.0 /  5.4 / 5.7 / 11.2
+  //   64 x 4096 x 4096   10.6 / 10.0 / 7.8 / 11.4
+  //   128 x 512 x 512     3.6 /  3.8 / 4.2 /  4.4
+  //   1088 x 96 x 1024    4.5 /  4.1 / 4.5 /  5.4
+  //   1088 x 512 x 512   10.0 / 10.5 / 8.7 /  4.9
+  const QuantizeRows none{};
   auto tiles = [&](int tm, int tn) { return (((long long)a.m + tm - 1) / tm) * (((long long)a.n + tn - 1) / tn); };
+  if (tiles(16, 16) <= 256) return LaunchNarrow<-1, 1, 1, 3, 0>(a, none, s);
+  if (tiles(32, 16) <= 256) return LaunchNarrow<-1, 2, 1, 4, 0>(a, none, s);
+  if (tiles(32, 32) <= 256) return LaunchNarrow<-1, 2, 2, 3, 0>(a, none, s);
+  // Else tiles as large as leaves every CU one (us in a graph, 64 x 64 / 128 x
+  // 128 / 256 x 256 tiles):
+  //   1999 x 777 x 1001    7.3 /  9.5 / 19.1
+  //   4352 x 512 x 512     6.8 /  7.5 / 13.2
+  //   2048 x 2000 x 1024  13.0 / 11.1 / 20.5
+  //   13056 x 512 x 512   13.1 / 11.5 / 15.8
+  //   13056 x 4096 x 1024  119 / 82.6 / 94.7
+  //   4096 x 4096 x 2048  69.0 / 46.6 / 45.7
+  //   8192 x 4096 x 4096   231 /  160 /  140
+  // but short products, which the stores bound, in the smallest:
+  //   4352 x 2000 x 192   11.0 / 13.9 / 13.4
+  // and the largest, of which a CU holds one, only where the last round of
+  // them is nearly full: 5000 x 5000 x 5000 (400 tiles) 176 / 154, but 4864 x
+  // 4096 x 4096 (304) 98.5 / 126.
+  // Several taps hold a second set of accumulators, for which the largest
+  // tiles have no registers; theirs gain from 128 x 128 at short K too:
+  //   13056 x 512 x 2 * 96  15.2 / 13.8
   const bool wide = tiles(128, 128) >= 256;
+  const long long big = tiles(256, 256), rounds = (big + 255) / 256;
   if (a.taps > 1) {
     if (wide) LaunchTile<128, 128, 4, 2, 2, 2, true>(a, s);
     else LaunchSmallTiles<true>(a, tiles(64, 64), s);
   } else if (!wide || a.k < 256) {
     LaunchSmallTiles<false>(a, tiles(64, 64), s);
-  } else if (a.k >= 2048 && tiles(256, 256) >= 128) {
+  } else if (a.k >= 2048 && 4 * big >= 3 * 256 * rounds) {
     LaunchTile<256, 256, 4, 2, 2, 2, false>(a, s);
-  } else if (tiles(128, 256) >= 256) {
-    LaunchTile<128, 256, 2, 4, 3, 1, false>(a, s);
   } else {
     LaunchTile<128, 128, 4, 2, 2, 2, false>(a, s);
   }

@@ -20,6 +20,7 @@ is imported first; importing this module after vosk alone raises ImportError.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import struct
 
 import torch
@@ -145,6 +146,11 @@ def _no_grad(*ts):
         for t in ts:
             if getattr(t, "requires_grad", False):
                 _refuse("a tensor requires a gradient: the 8-bit operators have no backward")
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(m, n, k, taps, rows):
+    return _chk(_c.vamd_op_linear_workspace(m, n, k, taps, rows))
 
 
 def code_bytes(k):
@@ -363,7 +369,7 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     if m == 0 or n == 0:
         return out
     if xp:
-        size = _chk(_c.vamd_op_linear_workspace(m, n, k, taps, c))
+        size = _workspace(m, n, k, taps, c)
         if size:
             ws = torch.empty(size, dtype=_i8, device=x.device)
             wsp = ws.data_ptr()
