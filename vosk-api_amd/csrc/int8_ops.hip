@@ -734,44 +734,71 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   };
 
   int buf = 0, k = 0, tap = 0;
+  // half a part of the step in buf: what the wave reads of it, its products
+  constexpr int AHEAD = BM * BN == 1 ? 4 : 1;
+  intx4 fa[AHEAD][BM], fb[AHEAD][BN];
+  auto fetch = [&](int i) {
+    const char* const at = smem + (buf * KB + i / 2) * PART + (i & 1 ? f1 : f0);
+#pragma unroll
+    for (int x = 0; x < BM; x++) fa[i % AHEAD][x] = *reinterpret_cast<const intx4*>(at + (wm + r32 + x * 32) * kPartBytes);
+#pragma unroll
+    for (int y = 0; y < BN; y++) fb[i % AHEAD][y] = *reinterpret_cast<const intx4*>(at + (TM + wn + r32 + y * 32) * kPartBytes);
+  };
+  auto multiply = [&](int i, int keep) {
+#pragma unroll
+    for (int x = 0; x < BM; x++) fa[i % AHEAD][x] &= keep;
+#pragma unroll
+    for (int x = 0; x < BM; x++)
+#pragma unroll
+      for (int y = 0; y < BN; y++)
+        acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i % AHEAD][x], fb[i % AHEAD][y], acc[x][y], 0, 0, 0);
+  };
+  auto join = [&](int u) {  // u more parts of the tap are done: is it?
+    if (!MULTI || (k += u) < kt) return;
+    k = 0;
+#pragma unroll
+    for (int x = 0; x < BM; x++) {
+      float sc[16];
+      row_scales(tap, x, sc);
+#pragma unroll
+      for (int y = 0; y < BN; y++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          v[x][y][i] = fmaf((float)acc[x][y][i], sc[i], v[x][y][i]);
+          acc[x][y][i] = 0;
+        }
+    }
+    tap++;
+  };
   for (int s = 0; s < steps; s++) {
     const int behind = issued - s - 1;  // steps in flight after this one
     if (behind >= ST - 2) wait_step<(ST - 2) * KB * LOADS>();
     else wait_last<ST - 3, KB * LOADS>(behind);
     if (issued < steps) issue();  // into the buffer that every wave left before the barrier
+    if (BM * BN == 1 && KB >= (MULTI ? 4 : 2) && (!MULTI || k + KB <= kt)) {
+      // A wave with one block waits for its reads of LDS: they go ahead of the products (2048 x 512 x 1024 6.3 -> 6.0
+      // us, 1999 x 777 x 2 * 1001 12.4 -> 11.8).  With more blocks the products hide them (8192 x 4096 x 4096 1 %
+      // slower so), and where two paths share both sets of accumulators they are copied.
 #pragma unroll
-    for (int u = 0; u < KB; u++) {
-      if (KB > 1 && s * KB + u >= parts) break;
-      const char* const sa = smem + (buf * KB + u) * PART + (wm + r32) * kPartBytes;
-      const char* const sb = smem + (buf * KB + u) * PART + (TM + wn + r32) * kPartBytes;
+      for (int i = 0; i < AHEAD - 1 && i < 2 * KB; i++) fetch(i);
 #pragma unroll
-      for (int q = 0; q < 2; q++) {
-        const int f = q ? f1 : f0;
-        intx4 fa[BM], fb[BN];
-#pragma unroll
-        for (int x = 0; x < BM; x++) fa[x] = *reinterpret_cast<const intx4*>(sa + x * 32 * kPartBytes + f);
-#pragma unroll
-        for (int y = 0; y < BN; y++) fb[y] = *reinterpret_cast<const intx4*>(sb + y * 32 * kPartBytes + f);
-#pragma unroll
-        for (int x = 0; x < BM; x++)
-#pragma unroll
-          for (int y = 0; y < BN; y++) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[x], fb[y], acc[x][y], 0, 0, 0);
+      for (int i = 0; i < 2 * KB; i++) {
+        if (i + AHEAD - 1 < 2 * KB) fetch(i + AHEAD - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(i, MULTI || s * KB + i / 2 < parts ? -1 : 0);  // (a part behind the last one adds nothing)
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (MULTI && ++k == kt) {
-        k = 0;
+      join(KB);
+    } else {  // part after part: a tap may end within the step
 #pragma unroll
-        for (int x = 0; x < BM; x++) {
-          float sc[16];
-          row_scales(tap, x, sc);
+      for (int u = 0; u < KB; u++) {
+        if (s * KB + u >= parts) break;
 #pragma unroll
-          for (int y = 0; y < BN; y++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              v[x][y][i] = fmaf((float)acc[x][y][i], sc[i], v[x][y][i]);
-              acc[x][y][i] = 0;
-            }
+        for (int i = 2 * u; i < 2 * u + 2; i++) {
+          fetch(i);
+          multiply(i, -1);
         }
-        tap++;
+        join(1);
       }
     }
     buf = buf + 1 == ST ? 0 : buf + 1;
