@@ -824,3 +824,31 @@ def test_numbers_that_do_not_fit_are_refused(ops):
             ops.linear_int8(codes, w, ws, scale=scales, residual_scale=bad)
     with pytest.raises(ValueError, match="gradient"):
         ops.linear_int8(codes, w, ws.clone().requires_grad_(), scale=scales)
+
+
+@pytest.mark.parametrize("m,k,t", [(1030, 1000, "fp32"), (2051, 2041, "fp32"), (4099, 2041, "bf16"), (4099, 1500, "fp16")])
+def test_quantize_rows_of_many_long_rows(ops, m, k, t):
+    """So many that a wave takes a row of its own."""
+    g = _gen(84)
+    x = (_randn(g, m, k) * torch.exp(_randn(g, m, 1))).to(TYPES[t])
+    codes, scales = ops.quantize_rows(x)
+    _same_codes(codes, scales, x)
+    few, few_s = ops.quantize_rows(x[:5].contiguous())
+    assert torch.equal(codes[:5], few) and torch.equal(scales[:5], few_s)
+
+
+@pytest.mark.parametrize("m,n,k,taps", [(40, 300, 576, 1), (64, 4096, 64, 1), (200, 600, 192, 3), (257, 520, 448, 2), (15, 33, 64, 16),
+                                        (500, 512, 640, 1), (2049, 520, 1088, 1), (2049, 130, 320, 5), (1999, 300, 832, 2)])
+def test_linear_tiles_of_every_size_agree(ops, m, n, k, taps):
+    """A row's result is the same in whichever tile it lies: all rows at once, and its own few."""
+    g = _gen(m + n)
+    codes, scales = ops.quantize_rows(_randn(g, m, k))
+    w, ws = ops.quantize_weight(_randn(g, n, taps * k), taps)
+    rows = torch.randint(-1, m, (m, taps), generator=g, device="cuda", dtype=torch.int32)
+    b, r = _randn(g, n), _randn(g, m, n)
+    kw = dict(scale=scales, bias=b, relu=True, gain=b, shift=b, residual_scale=0.7)
+    whole = ops.linear_int8(codes, w, ws, rows=rows, residual=r, **kw)
+    for lo, hi in ((0, 1), (m // 3, m // 3 + 12), (m - 17, m), (m // 2, min(m, m // 2 + 40))):
+        lo = max(lo, 0)
+        assert torch.equal(whole[lo:hi], ops.linear_int8(codes, w, ws, rows=rows[lo:hi], residual=r[lo:hi], **kw)), (lo, hi)
+    _linear_case(ops, m, n, k, taps, "bf16", "fp32", "brgs", m + n, cache=m)

@@ -151,9 +151,15 @@ struct Chunk {
   }
 };
 
-// ---- rows to codes: TPR threads (64 or 256) a row, the row kept in
-// registers (NV chunks of 16 bytes a thread) between the maximum and the
-// codes, so it is read once; NV = 0: longer rows are read twice.
+// ---- rows to codes
+//
+// Two passes over a row, its maximum and its codes, and one read of it: TPR
+// threads (64 or 256) a row keep it in registers (NV chunks of 16 bytes a
+// thread) in between; NV = 0: rows longer than that are read twice.  Bound by
+// memory: 13 056 rows of 512 floats (33.5 MB read and written) 6.6 us, 5.0 TB/s,
+// what a large copy reaches here; 8 192 rows of 4 096 bf16 (101 MB) 18 us;
+// 9 001 rows of 2 047 bf16, whose ends are loaded one by one, 12 to 14 us (55 MB).
+// One row of 512: 1.8 us, the launch.
 template <int TYPE, int TPR, int NV>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeRows a) {
   constexpr int N = Chunk<TYPE>::N;
@@ -210,12 +216,17 @@ void LaunchQuantize(const QuantizeRows& a, hipStream_t s) {
   constexpr int N = Chunk<TYPE>::N;
   const int kp = Int8Padded(a.k);
   const dim3 rows4 = Grid((a.m + 3) / 4), rows1 = Grid(a.m);
-  // a wave a row as long as it fits its registers; with too few rows to fill
-  // the chip so, four waves share the longer ones
+  // A wave a row as long as that takes few registers; of longer rows only where
+  // there are so many that they fill the chip (us in a graph, a wave / four
+  // waves a row): 512 rows of 1024 floats 3.4 / 3.3, 2048 3.7 / 4.4, 8192 6.8 /
+  // 10.2; 2048 rows of 2048 floats 4.6 / 4.8, 4096 6.9 / 8.2; 4096 rows of 2047
+  // bf16 8.8 / 8.5, 8192 13.3 / 14.4; 8192 rows of 4096 bf16 22.2 / 18.0.
+  const long long many = N == 4 ? 1024 : 4096;
   if (kp <= 64 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 1>), rows4, dim3(256), 0, s, a);
   else if (kp <= 64 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 2>), rows4, dim3(256), 0, s, a);
-  else if (kp <= 64 * 4 * N && a.m > 2048) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 4>), rows4, dim3(256), 0, s, a);
-  else if (kp <= 64 * 8 * N && a.m > 2048) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 8>), rows4, dim3(256), 0, s, a);
+  else if (kp <= 64 * 4 * N && a.m > many) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 64, 4>), rows4, dim3(256), 0, s, a);
+  else if (TYPE == kFloat32 && kp <= 64 * 8 * N && a.m > 2 * many)
+    hipLaunchKernelGGL((quantize_rows_kernel<kFloat32, 64, 8>), rows4, dim3(256), 0, s, a);
   else if (kp <= 256 * 2 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 2>), rows1, dim3(256), 0, s, a);
   else if (kp <= 256 * 4 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 4>), rows1, dim3(256), 0, s, a);
   else if (kp <= 256 * 8 * N) hipLaunchKernelGGL((quantize_rows_kernel<TYPE, 256, 8>), rows1, dim3(256), 0, s, a);
@@ -228,6 +239,9 @@ void LaunchQuantize(const QuantizeRows& a, hipStream_t s) {
 // kMapStreams streams it sums the streams' row counts itself, in LDS (at most
 // 16 KB of lengths out of L2, against a launch of its own for the sums);
 // with more, a first launch has written `starts` and the search reads those.
+// Bound by latencies one after another (lengths, sums, search, the stream's
+// numbers, its pages), not by its bytes: one stream of 51 frames 3.7 to 4.3 us,
+// 256 streams 5.4, 4 001 streams and 2 M entries (8 MB) 10.7.
 // Larger workgroups sum more streams: 4 001 streams in one of 256 / 512 / 1024
 // threads, 400 100 rows of 5 entries 10.4 / 9.2 / 10.2 us, 8 002 rows 8.3 / 7.2 /
 // 7.7.
@@ -459,10 +473,15 @@ __global__ __launch_bounds__(THREADS) void frame_map_kernel(FrameMap a) {
 // after lane), so that the sixteen lanes which a 16-byte-a-lane read serves
 // together, four runs of four rows, lie in different banks ((row >> 1) & 3,
 // right for eight neighbouring rows, cost 1.5 times the reads' cycles).
+// A product of 8192 x 4096 x 4096 takes 139 to 145 us (1.9 to 2.0 POP/s): the
+// matrix units are busy 44 % of the cycles, LDS has no bank conflict, L2 serves
+// 86 % of the lines, and the clock gives way under load (codes that are all
+// zero: 116 us).  Deeper rings, four waves of 128 x 128 and reads further ahead
+// of the products changed nothing there.
 constexpr int kPartBytes = 64;
 
 // lane l's 16 bytes at p go to LDS byte `to` + 16 * l (to: the same in all lanes).
-// The compiler does not count these loads: WaitStep does.
+// The compiler does not count these loads: the waits below do.
 __device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "memory");
 }
@@ -498,9 +517,10 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 
 // The 16 values that a lane holds of a 32 x 32 block, rows (i & 3) + 8 * (i >>
 // 2) after its first: through a buffer that begins at the block's first row
-// and ends behind the last row of the matrix, so an access costs one 32-bit
-// add and the hardware's range check leaves out the rows past the end (and
-// the columns past it, whose offset is kOutside).
+// (where rows are mapped, at the matrix's) and ends behind the last row of the
+// matrix, so an access costs one 32-bit add and the hardware's range check
+// leaves out the rows past the end (and rows and columns that are not there,
+// whose offset is kOutside).
 constexpr uint32_t kOutside = 0x80000000u;
 struct BlockRows {
   __amdgpu_buffer_rsrc_t rows;
@@ -1067,8 +1087,9 @@ namespace {
 
 template <int THREADS, int EACH>
 void LaunchMap(const FrameMap& a, hipStream_t s) {
-  // two rows a lane once there are enough rows for it: then fewer workgroups sum the streams
-  const int each = a.cap > 256 * 1024 && a.taps <= 8 ? 2 : 1;
+  // Two rows a lane once there are enough rows for it: fewer workgroups then sum the streams (us in a graph, one / two
+  // rows a lane, 4 001 streams and room for 200 050 rows of 5 entries 7.3 / 9.1, 400 100 8.5 / 9.3, 800 200 12.3 / 11.4).
+  const int each = a.cap > 512 * 1024 && a.taps <= 8 ? 2 : 1;
   const long long grid = (a.cap + each * THREADS - 1) / (each * THREADS);
   if (!EACH && !grid) return;
   const unsigned lds = each * THREADS * a.taps * sizeof(int);
@@ -1103,10 +1124,6 @@ void LaunchTile(const LinearInt8& a, hipStream_t s) {
   hipLaunchKernelGGL(kernel, Grid(tm * tn), dim3(64 * WM * WN), lds, s, a, (int)tm, (int)tn);
 }
 
-}  // namespace
-
-namespace {
-
 // 64 x 64 tiles: the longer K is, the more of it a step (us in a graph, 1 / 2 /
 // 4 parts): 4352 x 512 x 96 5.6 / 5.6 / 7.0, 2048 x 512 x 1024 6.8 / 6.6 / 6.1;
 // four parts take 64 KB of LDS, which more than two tiles a CU miss: 4352 x 512
@@ -1130,6 +1147,7 @@ void LaunchNarrow(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
 
 template <int TYPE>
 void LaunchFused(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
+  // values kept in registers: 1 x 4096 x 4096 6.3 us with room for 4096 of them in the workgroup, 7.2 for 16384
   const bool more = (long long)a.m * a.taps * a.k > kFusedValues / 4;
   if (a.m <= 16 && more) LaunchNarrow<TYPE, 1, 1, 4, kFusedValues>(a, x, s);
   else if (a.m <= 16) LaunchNarrow<TYPE, 1, 1, 4, kFusedValues / 4>(a, x, s);
