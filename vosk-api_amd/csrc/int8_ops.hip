@@ -481,7 +481,8 @@ __global__ __launch_bounds__(THREADS) void frame_map_kernel(FrameMap a) {
 constexpr int kPartBytes = 64;
 
 // lane l's 16 bytes at p go to LDS byte `to` + 16 * l (to: the same in all lanes).
-// The compiler does not count these loads: the waits below do.
+// The compiler does not count these loads: the waits below do.  (Nothing else in
+// these kernels uses m0.)
 __device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "memory");
 }

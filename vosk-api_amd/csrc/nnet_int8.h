@@ -7,9 +7,10 @@
 // times, and its fused stages are bias, ReLU, scale + offset and one bypass,
 // in that order.  The first layer keeps 32 bits: its input is assembled from
 // features and an i-vector, of sizes that one scale a frame does not serve,
-// and its weights are a few per cent of the model's.  A node that a product reads has, next to its ring of floats, a
-// ring of codes and scales, written by a quantisation after the op that
-// computes it; the rings of floats stay what every other op reads.
+// and its weights are a few per cent of the model's.  A node that a product
+// reads has, next to its ring of floats, a ring of codes and scales, written by
+// a quantisation after the op that computes it; the rings of floats stay what
+// every other op reads.
 //
 // Weights have one scale for each output column, activations one for each
 // frame; sums are exact (int8_ops.h), so a stream's log-likelihoods do not
