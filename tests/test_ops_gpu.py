@@ -852,3 +852,80 @@ def test_linear_tiles_of_every_size_agree(ops, m, n, k, taps):
         lo = max(lo, 0)
         assert torch.equal(whole[lo:hi], ops.linear_int8(codes, w, ws, rows=rows[lo:hi], residual=r[lo:hi], **kw)), (lo, hi)
     _linear_case(ops, m, n, k, taps, "bf16", "fp32", "brgs", m + n, cache=m)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k", [(1, 16384), (1, 16385), (2, 8192), (3, 5440), (16, 1024), (17, 960), (32, 512), (31, 528)])
+def test_linear_float_rows_at_the_end_of_one_launch(ops, m, k, t):
+    """16384 values (rows x padded columns) are quantised in the product's launch, more before it."""
+    _linear_case(ops, m, 45, k, 1, t, "fp32", "brg", m + k)
+
+
+@pytest.mark.parametrize("count", [0, 1, 5, 19, 50])
+@pytest.mark.parametrize("k", [30, 600])
+def test_linear_float_rows_through_a_map_up_to_a_count(ops, k, count):
+    g, m, n = _gen(85), 20, 70
+    x = _randn(g, 33, k).bfloat16()
+    w, ws = ops.quantize_weight(_randn(g, n, 2 * k), 2)
+    rows = torch.randint(-1, 33, (m, 2), generator=g, device="cuda", dtype=torch.int32)
+    cnt = torch.tensor([count], dtype=torch.int32, device="cuda")
+    out = torch.full((m, n), 7.0, device="cuda")
+    ops.linear_int8(x, w, ws, rows=rows, count=cnt, out=out)
+    codes, scales = ops.quantize_rows(x)
+    want = ops.linear_int8(codes, w, ws, scale=scales, rows=rows)
+    assert torch.equal(out[:count], want[:count]) and (out[count:] == 7.0).all()
+
+
+@pytest.mark.parametrize("m,n,k,taps", [(4, 30, 64, 1), (40, 300, 320, 2), (70, 600, 512, 1), (300, 1100, 128, 3), (2100, 2000, 256, 2),
+                                        (4200, 2200, 320, 1)])
+def test_linear_absent_rows_add_nothing_to_anything(ops, m, n, k, taps):
+    """The row that stands in for absent ones holds a NaN, and so does every row that no entry names."""
+    g = _gen(86)
+    x = _randn(g, 64, k)
+    x[0, 3], x[1, 0], x[63, k - 1] = float("nan"), float("inf"), float("nan")
+    codes, scales = ops.quantize_rows(x)
+    w, ws = ops.quantize_weight(_randn(g, n, taps * k), taps)
+    b = _randn(g, n)
+    rows = torch.randint(2, 63, (m, taps), generator=g, device="cuda", dtype=torch.int32)
+    rows[::2, 0] = -1
+    rows[1::4, taps - 1] = 64
+    rows[m - 1] = 2**31 - 1
+    y = ops.linear_int8(codes, w, ws, scale=scales, rows=rows, bias=b)
+    assert torch.isfinite(y).all() and torch.equal(y[m - 1], b)
+    if taps == 1:
+        assert torch.equal(y[::2], b.expand(len(y[::2]), n))
+    rows[m // 2, taps - 1] = 63
+    bad = ops.linear_int8(codes, w, ws, scale=scales, rows=rows, bias=b)
+    assert bad[m // 2].isnan().all()
+    bad[m // 2] = y[m // 2]
+    assert torch.equal(bad, y)
+    rows[m // 2, taps - 1] = -1
+    assert torch.equal(ops.linear_int8(x, w, ws, rows=rows, bias=b), ops.linear_int8(codes, w, ws, scale=scales, rows=rows, bias=b))
+
+
+def test_products_on_two_threads(ops):
+    """The C calls of two threads, each on a stream of its own."""
+    import threading
+    g = _gen(87)
+    jobs = []
+    for m, n, k in ((5, 200, 300), (90, 500, 640), (600, 700, 512)):
+        x = _randn(g, m, k)
+        w, ws = ops.quantize_weight(_randn(g, n, k))
+        jobs.append((x, w, ws, ops.linear_int8(x, w, ws)))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(40):
+                for x, w, ws, want in jobs:
+                    if not torch.equal(ops.linear_int8(x, w, ws), want):
+                        bad.append(tuple(x.shape))
+        s.synchronize()
+    ts = [threading.Thread(target=work) for _ in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
