@@ -1501,7 +1501,6 @@ void Engine::BuildInt8(const std::vector<float*>& rings, const std::vector<float
     HIPCHECK(hipMemset(codes[n], 0, bytes));
     HIPCHECK(hipMemset(scales[n], 0, sizeof(float) * (size_t)frames));
   }
-  int* const starts = (int*)DevAlloc(sizeof(int) * ((size_t)jobs + 1));
   for (const Int8Plan::Map& m : int8_.maps) {
     FrameMap f{};
     f.lengths = Upload(std::vector<int>(jobs, m.rows * m.step));
@@ -1512,7 +1511,7 @@ void Engine::BuildInt8(const std::vector<float*>& rings, const std::vector<float
     f.frame_stride = S;
     f.taps = (int)m.offsets.size();
     f.step = m.step;
-    f.starts = starts;
+    f.starts = (int*)DevAlloc(sizeof(int) * ((size_t)jobs + 1));
     f.rows = (int*)DevAlloc(sizeof(int) * (size_t)jobs * m.rows * f.taps);
     f.per_stream = m.rows;
     SetOffsets(&f, m.offsets.data());
@@ -1584,7 +1583,7 @@ void Engine::BuildInt8(const std::vector<float*>& rings, const std::vector<float
 }
 
 long long Engine::NnetLaunches() const {
-  long long n = (long long)(plan_.ops.size() + int8_maps_.size());
+  long long n = (long long)plan_.ops.size() + FrameMapLaunches((int)int8_maps_.size());
   for (const Int8Plan::OpPlan& o : int8_.ops) n += o.quantize;
   return n;
 }
@@ -1592,13 +1591,13 @@ long long Engine::NnetLaunches() const {
 void Engine::LaunchNnet(const NnetBatch& b, hipStream_t s) {
   if (b.njobs == 0) return;
   const DevJob* dj = (const DevJob*)(d_stage_ + (size_t)b.buf * stage_bytes_ + b.o_dj);
-  for (FrameMap m : int8_maps_) {
+  for (FrameMap& m : int8_maps_) {
     m.streams = b.njobs;
     m.first = (const int*)(d_stage_ + (size_t)b.buf * stage_bytes_ + b.o_t);
     m.table = (const int*)(d_stage_ + (size_t)b.buf * stage_bytes_ + b.o_slot);
     m.cap = (long long)b.njobs * m.per_stream;
-    LaunchFrameMap(m, s);
   }
+  LaunchFrameMaps(int8_maps_.data(), (int)int8_maps_.size(), s);
   for (size_t i = 0; i < plan_.ops.size(); i++) {
     NnetOpArgs a = op_args_[i];
     a.M = b.njobs * a.P;

@@ -97,6 +97,10 @@ struct FrameMap {
 // Sets the a->taps offsets and what follows from them and from the pages.
 void SetOffsets(FrameMap* a, const int* offsets);
 void LaunchFrameMap(const FrameMap& a, hipStream_t s);
+// n maps, each with rows and starts of its own, in as few launches as they fit.
+constexpr int kMapsPerLaunch = 8;
+void LaunchFrameMaps(const FrameMap* maps, int n, hipStream_t s);
+inline int FrameMapLaunches(int n) { return (n + kMapsPerLaunch - 1) / kMapsPerLaunch; }
 
 // out[m][n] = epi(sw[n] * sum_j sa[r(m,j)] * sum_k a[r(m,j)][k] * w[n][j * K + k])
 // with r(m, j) = rows[m][j] (rows == nullptr: m, taps 1); an entry outside

@@ -300,7 +300,7 @@ __global__ __launch_bounds__(kStartsThreads) void frame_starts_kernel(FrameMap a
 // already).  A lane makes ROWS rows, 64 apart, of the ROWS * 64 of its wave,
 // their loads in flight together.
 template <int THREADS, int EACH, int ROWS>
-__global__ __launch_bounds__(THREADS) void frame_map_kernel(FrameMap a) {
+__device__ __forceinline__ void map_rows(const FrameMap& a) {
   constexpr bool SUM = EACH > 0;
   constexpr int GAP = EACH > 1 ? EACH : 1 << 30;
   // starts; a gap every EACH so that a thread's lie in other banks than its neighbours'
@@ -457,6 +457,20 @@ __global__ __launch_bounds__(THREADS) void frame_map_kernel(FrameMap a) {
   const long long left = (rows - row0) * a.taps;
   int* const out = a.rows + row0 * a.taps;
   for (int e = lane; e < ROWS * 64 * a.taps && e < left; e += 64) out[e] = turn[e];
+}
+
+template <int THREADS, int EACH, int ROWS>
+__global__ __launch_bounds__(THREADS) void frame_map_kernel(FrameMap a) {
+  map_rows<THREADS, EACH, ROWS>(a);
+}
+
+// several maps in one launch
+struct FrameMaps {
+  FrameMap map[kMapsPerLaunch];
+};
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void frame_maps_kernel(FrameMaps all) {
+  map_rows<THREADS, EACH, 1>(all.map[blockIdx.z]);
 }
 
 // ---- the product
@@ -1109,6 +1123,42 @@ void LaunchFrameMap(const FrameMap& a, hipStream_t s) {
     LaunchMap<kMapManyThreads, kMapStreams / kMapManyThreads>(a, s);
   } else {
     LaunchMap<kMapThreads, 1>(a, s);
+  }
+}
+
+namespace {
+
+template <int THREADS, int EACH>
+void LaunchMaps(const FrameMaps& all, int n, long long cap, int taps, hipStream_t s) {
+  const unsigned lds = THREADS * taps * sizeof(int);
+  auto kernel = frame_maps_kernel<THREADS, EACH>;
+  AskLds((const void*)kernel, lds);
+  dim3 grid = Grid(cap ? (cap + THREADS - 1) / THREADS : 1);
+  grid.z = n;
+  hipLaunchKernelGGL(kernel, grid, dim3(THREADS), lds, s, all);
+}
+
+}  // namespace
+
+void LaunchFrameMaps(const FrameMap* maps, int n, hipStream_t s) {
+  for (; n > 0; maps += kMapsPerLaunch, n -= kMapsPerLaunch) {
+    const int some = n < kMapsPerLaunch ? n : kMapsPerLaunch;
+    FrameMaps all{};
+    long long cap = 0;
+    int taps = 0, streams = 0;
+    for (int i = 0; i < some; i++) {
+      all.map[i] = maps[i];
+      cap = maps[i].cap > cap ? maps[i].cap : cap;
+      taps = maps[i].taps > taps ? maps[i].taps : taps;
+      streams = maps[i].streams > streams ? maps[i].streams : streams;
+    }
+    if (streams > kMapStreams) {
+      for (int i = 0; i < some; i++) LaunchFrameMap(maps[i], s);
+    } else if (streams > kMapThreads) {
+      LaunchMaps<kMapManyThreads, kMapStreams / kMapManyThreads>(all, some, cap, taps, s);
+    } else {
+      LaunchMaps<kMapThreads, 1>(all, some, cap, taps, s);
+    }
   }
 }
 
