@@ -213,3 +213,15 @@ def test_other_front_ends(synth_model_frontend, test_wave):
     _, _, (fp,) = _run(synth_model_frontend, [test_wave[:16000]], "fp32")
     assert e.int8_layers == 24
     assert 0 < _rms(llh - fp) < 0.2 * _rms(fp - fp.mean(0))
+
+
+def test_more_streams_than_threads_of_a_map(synth_model, test_wave):
+    """A pass of 260 jobs: the row maps' other form; every stream as it is alone."""
+    waves = [perturbed_stream(test_wave, i % 3, seconds=1.0 + 0.2 * (i % 3)) for i in range(260)]
+    e, ss, llh = _run(synth_model, waves)
+    e.close()
+    for i in range(3):
+        e, _, alone = _run(synth_model, [waves[i]])
+        e.close()
+        for k in range(i, 260, 3):
+            np.testing.assert_array_equal(llh[k], alone[0], err_msg=str(k))
