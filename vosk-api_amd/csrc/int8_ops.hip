@@ -487,10 +487,10 @@ __global__ __launch_bounds__(THREADS) void frame_maps_kernel(FrameMaps all) {
 // after lane), so that the sixteen lanes which a 16-byte-a-lane read serves
 // together, four runs of four rows, lie in different banks ((row >> 1) & 3,
 // right for eight neighbouring rows, cost 1.5 times the reads' cycles).
-// A product of 8192 x 4096 x 4096 takes 139 to 145 us (1.9 to 2.0 POP/s): the
-// matrix units are busy 44 % of the cycles, LDS has no bank conflict, L2 serves
+// A product of 8192 x 4096 x 4096 takes 131 to 141 us (1.95 to 2.1 POP/s): the
+// matrix units are busy 50 % of the cycles, LDS has no bank conflict, L2 serves
 // 86 % of the lines, and the clock gives way under load (codes that are all
-// zero: 116 us).  Deeper rings, four waves of 128 x 128 and reads further ahead
+// zero: 102 us).  Deeper rings, four waves of 128 x 128 and reads further ahead
 // of the products changed nothing there.
 constexpr int kPartBytes = 64;
 
@@ -675,26 +675,28 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   if (MULTI) __syncthreads();
   const uint32_t to = lds_address(smem) + wave * LOADS * 1024;
   int issued = 0, ipart = 0, ik = 0, itap = 0, ibuf = 0;
-  auto issue = [&] {
+  auto issue_part = [&](int u) {  // part u of the next step
+    const bool last = ik + 1 == kt;  // of the tap
 #pragma unroll
-    for (int u = 0; u < KB; u++) {
-      const bool last = ik + 1 == kt;  // of the tap
-#pragma unroll
-      for (int g = 0; g < LOADS; g++) load_to_lds(p[g], to + (ibuf * KB + u) * PART + g * 1024);
-      if (++ipart >= parts) continue;  // (a step's parts behind the last one are loads of the last one again)
-      ik = last ? 0 : ik + 1;
-      itap += last;
-#pragma unroll
-      for (int g = 0; g < LOADS; g++) {
-        const int r = (wave * LOADS + g) * 16 + lrow;
-        if (MULTI && last && r < TM) p[g] = a.a + (long long)max(srow[itap * TM + r], 0) * a.lda + 16 * chunk;
-        else p[g] += kPartBytes;
-      }
+    for (int g = 0; g < LOADS; g++) load_to_lds(p[g], to + (ibuf * KB + u) * PART + g * 1024);
+    if (u == KB - 1) {
+      issued++;
+      ibuf = ibuf + 1 == ST ? 0 : ibuf + 1;
     }
-    issued++;
-    ibuf = ibuf + 1 == ST ? 0 : ibuf + 1;
+    if (++ipart >= parts) return;  // (a step's parts behind the last one are loads of the last one again)
+    ik = last ? 0 : ik + 1;
+    itap += last;
+#pragma unroll
+    for (int g = 0; g < LOADS; g++) {
+      const int r = (wave * LOADS + g) * 16 + lrow;
+      if (MULTI && last && r < TM) p[g] = a.a + (long long)max(srow[itap * TM + r], 0) * a.lda + 16 * chunk;
+      else p[g] += kPartBytes;
+    }
   };
-  for (int s = 0; s < ST - 1 && s < steps; s++) issue();
+  for (int s = 0; s < ST - 1 && s < steps; s++) {
+#pragma unroll
+    for (int u = 0; u < KB; u++) issue_part(u);
+  }
   for (int i = tid; i < TM * a.taps; i += NT) {  // read behind the first of the loop's barriers
     const int row = MULTI ? srow[i] : row_of(m0 + i, 0);
     sscale[i] = row >= 0 ? a.sa[row] : 0.0f;
@@ -809,7 +811,15 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
     const int behind = issued - s - 1;  // steps in flight after this one
     if (behind >= ST - 2) wait_step<(ST - 2) * KB * LOADS>();
     else wait_last<ST - 3, KB * LOADS>(behind);
-    if (issued < steps) issue();  // into the buffer that every wave left before the barrier
+    // The next step's loads go into the buffer that every wave left before the barrier.  A wave stands still while its
+    // loads are taken: with many blocks a wave they go out between its products (8192 x 4096 x 4096 147 -> 140 us), with
+    // few at once, ahead of them (1999 x 777 x 1001 7.5 against 7.2).
+    constexpr bool BETWEEN = BM * BN >= 8;
+    const bool more = issued < steps;
+    if (!BETWEEN && more) {
+#pragma unroll
+      for (int u = 0; u < KB; u++) issue_part(u);
+    }
     if (BM * BN == 1 && KB >= (MULTI ? 4 : 2) && (!MULTI || k + KB <= kt)) {
       // A wave with one block waits for its reads of LDS: they go ahead of the products (2048 x 512 x 1024 6.3 -> 6.0
       // us, 1999 x 777 x 2 * 1001 12.4 -> 11.8).  With more blocks the products hide them (8192 x 4096 x 4096 1 %
@@ -828,6 +838,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
 #pragma unroll
       for (int u = 0; u < KB; u++) {
         if (s * KB + u >= parts) break;
+        if (BETWEEN && more) issue_part(u);
 #pragma unroll
         for (int i = 2 * u; i < 2 * u + 2; i++) {
           fetch(i);
@@ -1249,7 +1260,7 @@ void LaunchLinearInt8(const LinearInt8& a, hipStream_t s) {
   //   13056 x 512 x 512   13.1 / 11.5 / 15.8
   //   13056 x 4096 x 1024  119 / 82.6 / 94.7
   //   4096 x 4096 x 2048  69.0 / 46.6 / 45.7
-  //   8192 x 4096 x 4096   231 /  160 /  140
+  //   8192 x 4096 x 4096   231 /  160 /  134
   // but short products, which the stores bound, in the smallest:
   //   4352 x 2000 x 192   11.0 / 13.9 / 13.4
   // and the largest, of which a CU holds one, only where the last round of
