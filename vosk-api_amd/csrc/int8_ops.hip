@@ -1187,9 +1187,9 @@ void LaunchTile(const LinearInt8& a, hipStream_t s) {
 }
 
 // 64 x 64 tiles: the longer K is, the more of it a step (us in a graph, 1 / 2 /
-// 4 parts): 4352 x 512 x 96 5.6 / 5.6 / 7.0, 2048 x 512 x 1024 6.8 / 6.6 / 6.1;
+// 4 parts): 4352 x 512 x 96 5.5 / 5.5 / 7.0, 2048 x 512 x 1024 6.8 / 6.3 / 5.9;
 // four parts take 64 KB of LDS, which more than two tiles a CU miss: 4352 x 512
-// x 1024 (544 tiles) 9.1 / 8.6 / 10.5.
+// x 1024 (544 tiles) 9.4 / 9.2 / 10.4.
 template <bool MULTI>
 void LaunchSmallTiles(const LinearInt8& a, long long tiles, hipStream_t s) {
   if (a.k * a.taps < 512) LaunchTile<64, 64, 2, 2, 3, 1, MULTI>(a, s);
@@ -1242,11 +1242,11 @@ void LaunchLinearInt8(const LinearInt8& a, hipStream_t s) {
   if (a.m <= 0 || a.n <= 0) return;
   // Narrow tiles as long as no CU gets two, the smallest first (us in a graph,
   // 16 x 16 / 32 x 16 / 32 x 32 / 64 x 64 tiles, m x n x k):
-  //   16 x 4096 x 4096    5.0 /  5.4 / 5.7 / 11.2
-  //   64 x 4096 x 4096   10.6 / 10.0 / 7.8 / 11.4
-  //   128 x 512 x 512     3.6 /  3.8 / 4.2 /  4.4
-  //   1088 x 96 x 1024    4.5 /  4.1 / 4.5 /  5.4
-  //   1088 x 512 x 512   10.0 / 10.5 / 8.7 /  4.9
+  //   16 x 4096 x 4096    5.1 /  5.7 / 5.8 / 10.4
+  //   64 x 4096 x 4096   10.4 /  9.7 / 7.5 / 10.4
+  //   128 x 512 x 512     3.6 /  3.7 / 4.2 /  4.3
+  //   1088 x 96 x 1024    4.5 /  4.1 / 4.6 /  5.2
+  //   1088 x 512 x 512   10.1 / 10.6 / 8.6 /  4.7
   const QuantizeRows none{};
   auto tiles = [&](int tm, int tn) { return (((long long)a.m + tm - 1) / tm) * (((long long)a.n + tn - 1) / tn); };
   if (tiles(16, 16) <= 256) return LaunchNarrow<-1, 1, 1, 3, 0>(a, none, s);
@@ -1254,21 +1254,21 @@ void LaunchLinearInt8(const LinearInt8& a, hipStream_t s) {
   if (tiles(32, 32) <= 256) return LaunchNarrow<-1, 2, 2, 3, 0>(a, none, s);
   // Else tiles as large as leaves every CU one (us in a graph, 64 x 64 / 128 x
   // 128 / 256 x 256 tiles):
-  //   1999 x 777 x 1001    7.3 /  9.5 / 19.1
-  //   4352 x 512 x 512     6.8 /  7.5 / 13.2
-  //   2048 x 2000 x 1024  13.0 / 11.1 / 20.5
-  //   13056 x 512 x 512   13.1 / 11.5 / 15.8
-  //   13056 x 4096 x 1024  119 / 82.6 / 94.7
-  //   4096 x 4096 x 2048  69.0 / 46.6 / 45.7
-  //   8192 x 4096 x 4096   231 /  160 /  134
+  //   1999 x 777 x 1001    7.4 /  9.8 / 18.1
+  //   4352 x 512 x 512     7.1 /  7.7 / 12.9
+  //   2048 x 2000 x 1024  13.0 / 11.6 / 19.2
+  //   13056 x 512 x 512   13.3 / 11.5 / 15.3
+  //   13056 x 4096 x 1024  117 / 81.0 / 90.7
+  //   4096 x 4096 x 2048  67.3 / 45.9 / 43.3
+  //   8192 x 4096 x 4096   237 /  160 /  135
   // but short products, which the stores bound, in the smallest:
-  //   4352 x 2000 x 192   11.0 / 13.9 / 13.4
+  //   4352 x 2000 x 192   11.1 / 13.8 / 13.3
   // and the largest, of which a CU holds one, only where the last round of
-  // them is nearly full: 5000 x 5000 x 5000 (400 tiles) 176 / 154, but 4864 x
-  // 4096 x 4096 (304) 98.5 / 126.
+  // them is nearly full: 5000 x 5000 x 5000 (400 tiles) 173 / 140, but 4864 x
+  // 4096 x 4096 (304) 99.0 / 114.
   // Several taps hold a second set of accumulators, for which the largest
   // tiles have no registers; theirs gain from 128 x 128 at short K too:
-  //   13056 x 512 x 2 * 96  15.2 / 13.8
+  //   13056 x 512 x 2 * 96  15.3 / 13.9
   const bool wide = tiles(128, 128) >= 256;
   const long long big = tiles(256, 256), rounds = (big + 255) / 256;
   if (a.taps > 1) {
