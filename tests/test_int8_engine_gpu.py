@@ -225,3 +225,46 @@ def test_more_streams_than_threads_of_a_map(synth_model, test_wave):
         e.close()
         for k in range(i, 260, 3):
             np.testing.assert_array_equal(llh[k], alone[0], err_msg=str(k))
+
+
+def _batch_texts(model_dir, waves, monkeypatch):
+    import vosk
+    monkeypatch.setenv("VOSK_BATCH_MODEL_DIR", model_dir)
+    model = vosk.BatchModel()
+    recs = [vosk.BatchRecognizer(model, 16000) for _ in waves]
+    for r, w in zip(recs, waves):
+        r.AcceptWaveform(np.asarray(w, np.float32).astype("<i2").tobytes())
+        r.FinishStream()
+    model.Wait()
+    out = []
+    for r in recs:
+        text = ""
+        while True:
+            res = r.Result()
+            if not res:
+                break
+            text += " " + json.loads(res)["text"]
+        out.append(text.strip())
+    return out
+
+
+def test_batch_model_at_its_own_number_of_streams(synth_model_noep, test_wave, monkeypatch):
+    """600 streams and 2 000 outputs: the log-likelihoods have no ring, so no ring's limit is theirs.  The results are
+    those of a batch model with 4 streams."""
+    import vosk
+    vosk.SetLogLevel(-1)
+    vosk.GpuInit()
+    monkeypatch.setenv("VOSK_AMD_NNET", "int8")
+    monkeypatch.delenv("VOSK_AMD_BATCH_SLOTS", raising=False)
+    waves = [perturbed_stream(test_wave, i, seconds=2.0 + 0.45 * i) for i in range(3)]
+    many = _batch_texts(synth_model_noep, waves, monkeypatch)
+    monkeypatch.setenv("VOSK_AMD_BATCH_SLOTS", "4")
+    few = _batch_texts(synth_model_noep, waves, monkeypatch)
+    assert many == few and all(many), (many, few)
+
+
+def test_streams_past_the_limit_of_a_ring_are_refused_with_the_number(synth_model):
+    """A ring of 512 frames of 512 floats a stream is 1 MiB: 2 047 streams stay below 2^31 bytes."""
+    from vosk import engine
+    with pytest.raises(RuntimeError, match="at most 2047 streams an engine"):
+        engine.Engine(synth_model, frames_per_chunk=51, max_streams=2048, precision="int8")

@@ -372,6 +372,12 @@ Engine::Engine(std::shared_ptr<const ModelData> md, const EngineConfig& cfg) : m
   ring_ = std::max(ring_, Pow2AtLeast(int8_.span));
   sample_ring_ = Pow2AtLeast((long long)cfg_.max_step_samples + 2 * L + o.WindowShift() + 64);
   const int S = cfg_.max_slots;
+  if (cfg_.nnet_int8) {
+    const long long most = int8_.MaxRingRows(plan_) / ring_;
+    if (S > most)
+      VAMD_ERR("8-bit layers: " << S << " streams with rings of " << ring_ << " frames pass 2^31 bytes a ring (at most "
+                                << most << " streams an engine)");
+  }
   std::vector<float*> ring_ptrs(plan_.nodes.size());
   std::vector<int> ring_dims(plan_.nodes.size());
   for (size_t i = 0; i < plan_.nodes.size(); i++) {
@@ -1490,7 +1496,6 @@ void Engine::FinishDecodeBatch(const DecBatch& b) {
 void Engine::BuildInt8(const std::vector<float*>& rings, const std::vector<float*>& vecs) {
   const int S = cfg_.max_slots, jobs = S * jobs_per_slot_;
   const long long frames = (long long)ring_ * S;
-  if (frames > INT_MAX) VAMD_ERR("8-bit layers: more than 2^31 ring rows");
   std::vector<int8_t*> codes(plan_.nodes.size(), nullptr);
   std::vector<float*> scales(plan_.nodes.size(), nullptr);
   for (size_t n = 0; n < plan_.nodes.size(); n++) {
@@ -1560,9 +1565,6 @@ void Engine::BuildInt8(const std::vector<float*>& rings, const std::vector<float
         l.ldout_to = map.taps;
         l.out_rows = frames;
       }
-      if (frames * std::max(l.ldo, l.ldr) * 4 >= (1ll << 31))
-        VAMD_ERR("8-bit layers: a ring of " << frames << " rows of " << std::max(l.ldo, l.ldr)
-                                            << " floats passes 2^31 bytes (fewer streams an engine)");
       int8_args_[i] = l;
     }
     if (o.quantize) {

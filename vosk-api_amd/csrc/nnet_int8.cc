@@ -2,6 +2,7 @@
 #include "nnet_int8.h"
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <limits>
 #include <sstream>
@@ -143,6 +144,19 @@ Int8Plan BuildInt8Plan(const NnetPlan& p) {
     r.span = std::max(r.span, (m.rows - 1) * m.step + *mm.second - *mm.first + 1);
   }
   return r;
+}
+
+long long Int8Plan::MaxRingRows(const NnetPlan& p) const {
+  long long rows = INT_MAX;
+  auto mapped = [&](int node) {
+    if (node >= 0) rows = std::min(rows, ((1ll << 31) - 1) / ((long long)sizeof(float) * p.nodes[node].dim));
+  };
+  for (size_t i = 0; i < ops.size(); i++) {
+    if (!ops[i].product) continue;
+    mapped(p.ops[i].out_node);
+    mapped(ops[i].res_node);
+  }
+  return rows;
 }
 
 std::string Int8Plan::Describe(const NnetPlan& p) const {

@@ -50,6 +50,10 @@ struct Int8Plan {
   std::vector<char> coded;   // per stored node: has a ring of codes
   int products = 0;
   int span = 0;              // frames that one job's maps span at most
+  // Rows of a ring at most: a matrix whose rows a product maps (an output or a
+  // bypass ring; not the log-likelihoods) is smaller than 2^31 bytes, and a
+  // row's number has 31 bits.
+  long long MaxRingRows(const NnetPlan& p) const;
   std::string Describe(const NnetPlan& p) const;
 };
 
