@@ -98,7 +98,9 @@ typedef struct {
     const float *bias;       /* [n], or NULL */
     const float *gain, *shift; /* [n], or both NULL */
     const void *residual;    /* [m][n] of residual_type, rows ldr elements apart, or NULL */
-    void *out;               /* [m][n] of out_type, rows ldo apart; residual itself, or overlapping no input */
+    void *out;               /* [m][n] of out_type, rows ldo apart; overlapping no input, but it may be residual
+                                itself (address, type and stride) where out_to and res_from are both NULL or
+                                the same map; refused where it overlaps residual otherwise */
     const int *out_to;       /* or NULL: output row i goes to row out_to[i * ldout_to] of the out_rows rows of
                                 out; an entry outside is skipped, those inside have to be distinct */
     const int *res_from;     /* or NULL: row i's residual is row res_from[i * ldres_from] of the res_rows rows;

@@ -218,3 +218,23 @@ def test_precision_names():
     from vosk import engine
     with pytest.raises(ValueError, match="precision"):
         engine.Engine("nowhere", precision="int4")
+
+
+# 7 output rows of 9 floats in a matrix of 20 columns and 50 rows
+IN_PLACE = {**LINEAR, "ldo": 20, "residual": P, "ldr": 20}
+
+
+@pytest.mark.parametrize("change", [
+    dict(out_to=P, ldout_to=1, out_rows=50), dict(res_from=P, ldres_from=1, res_rows=50),
+    dict(out_to=P, ldout_to=1, out_rows=50, res_from=P + 4, ldres_from=1, res_rows=50),
+    dict(out_to=P, ldout_to=1, out_rows=50, res_from=P, ldres_from=2, res_rows=50),
+    dict(residual_type=1), dict(out_type=2), dict(ldr=19), dict(ldo=19), dict(ldo=9, ldr=18), dict(residual=P + 4), dict(out=P + 20 * 4),
+    dict(residual=P + 8 * 4), dict(out=P + 8 * 4), dict(residual=P + 12 * 4), dict(residual=P + 26 * 4), dict(residual=P + 20 * 6 * 4 + 32),
+    dict(m=1, residual=P + 4), dict(m=1, ldo=9, out_to=P, out_rows=50, ldr=0),
+    dict(out=P + 49 * 80, residual=P, res_from=P, ldres_from=1, res_rows=50), dict(out=P + 6 * 80 - 4, out_to=P, ldout_to=1, out_rows=9),
+])
+def test_out_that_overlaps_the_residual_otherwise_than_row_by_row_is_refused(lib, change):
+    """One row's residual would be read while another's output is written over it: in place goes row by row, through no
+    maps or through the same map."""
+    assert _call(lib, "vamd_op_linear_int8", Linear, **{**IN_PLACE, **change}) < 0
+    assert "overlap" in _err(lib) and "residual" in _err(lib)

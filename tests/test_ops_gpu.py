@@ -929,3 +929,45 @@ def test_products_on_two_threads(ops):
     for t in ts:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,n,k,taps", [(1, 17, 64, 1), (9, 33, 128, 2), (70, 96, 192, 1), (300, 513, 192, 2), (3000, 2000, 96, 1)])
+def test_linear_in_place_through_one_map(ops, m, n, k, taps, t):
+    """out is the residual and both have the same map; and out is other columns of the residual's rows."""
+    g = _gen(m + n + k)
+    c, s = ops.quantize_rows(_randn(g, 40, k))
+    w, ws = ops.quantize_weight(_randn(g, n, taps * k) / (taps * k) ** 0.5, taps)
+    at = torch.randint(-1, 41, (m, taps), generator=g, device="cuda", dtype=torch.int32)
+    to = (torch.randperm(m + 30, generator=g, device="cuda")[:m].int() - 10).contiguous()
+    a, b = at.cpu().numpy(), to.cpu().numpy()
+    ok = (b >= 0) & (b < m + 5)
+    big = _randn(g, m + 5, 2 * n + 3).to(TYPES[t])
+    res = big[:, :n]
+    before = _np(big)
+    v, size = ref.linear(c.cpu().numpy(), s.cpu().numpy(), a, w.cpu().numpy(), ws.cpu().numpy(), taps,
+                         residual=np.where(ok[:, None], before[np.where(ok, b, 0), :n], 0.0), residual_scale=-1.5)
+    for lo in (0, n + 1):  # in place, and beside it
+        into = big.clone()
+        out = into[:, lo:lo + n]
+        ops.linear_int8(c, w, ws, scale=s, rows=at, residual=into[:, :n], residual_scale=-1.5, out=out, out_rows=to, residual_rows=to)
+        got = _np(into)
+        _check(torch.from_numpy(got[b[ok], lo:lo + n]), v[ok], size[ok], taps, t)
+        got[b[ok], lo:lo + n] = before[b[ok], lo:lo + n]
+        np.testing.assert_array_equal(got, before)
+
+
+def test_linear_out_over_the_residual_otherwise_is_refused(ops):
+    g = _gen(1)
+    x = _randn(g, 50, 64)
+    w, ws = ops.quantize_weight(_randn(g, 32, 64))
+    buf = _randn(g, 51, 70)
+    before = buf.clone()
+    to = torch.arange(50, device="cuda", dtype=torch.int32).flip(0).contiguous()
+    for kw in (dict(out=buf[:50, :32], residual=buf[:50, :32], out_rows=to), dict(out=buf[:50, :32], residual=buf[:50, :32], residual_rows=to),
+               dict(out=buf[:50, :32], residual=buf[:50, :32], out_rows=to, residual_rows=to.clone()),
+               dict(out=buf[:50, :32], residual=buf[:50, 31:63]), dict(out=buf[:50, :32], residual=buf[1:, :32]),
+               dict(out=buf[:50, :32], residual=buf[1:, :32], out_rows=to, residual_rows=to)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.linear_int8(x, w, ws, **kw)
+    assert torch.equal(buf, before)

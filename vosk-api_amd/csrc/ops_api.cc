@@ -4,6 +4,7 @@
 
 #include <climits>
 #include <cmath>
+#include <numeric>
 
 #include "common.h"
 #include "int8_ops.h"
@@ -71,6 +72,23 @@ void CheckRows(const QuantizeRows& a) {
   Want(a.cache_rows >= (a.rows ? 0 : a.m), "quantize_rows: fewer code rows than rows");
 }
 
+// Whether two matrices of rows x n elements share a byte: their spans do, and
+// not as different columns of common rows (in steps of both strides' common
+// divisor each has the columns of one row).
+struct Extent {
+  const void* p;
+  long long rows, ld, bytes;  // ld: bytes from row to row; bytes: of a row
+};
+bool Overlap(const Extent& a, const Extent& b) {
+  if (a.rows <= 0 || b.rows <= 0) return false;
+  const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+  if (pa + (uintptr_t)((a.rows - 1) * a.ld + a.bytes) <= pb || pb + (uintptr_t)((b.rows - 1) * b.ld + b.bytes) <= pa) return false;
+  const long long g = std::gcd(a.rows > 1 ? a.ld : 0, b.rows > 1 ? b.ld : 0);
+  if (g == 0) return true;
+  const long long d = pb >= pa ? (long long)((pb - pa) % (uintptr_t)g) : (g - (long long)((pa - pb) % (uintptr_t)g)) % g;  // b's column
+  return d < a.bytes || d + b.bytes > g;
+}
+
 alignas(16) char kNoWorkspace[16];
 
 void CheckLinear(const LinearInt8& a) {
@@ -101,6 +119,13 @@ void CheckLinear(const LinearInt8& a) {
          "linear_int8: residual has to be below 2^31 bytes where res_from maps its rows");
     Want(a.ldr <= kInt8MaxStride || (a.m == 1 && !a.res_from), "linear_int8: rows of residual may be 2^23 elements apart at most");
     Want(Aligned(a.residual, Bytes(a.res_type)), "linear_int8: residual is not aligned to its elements");
+    // in place, a lane reads the elements that it writes itself: of the same row, whatever maps it
+    const bool same_rows = a.out_to == a.res_from && (!a.out_to || a.m == 1 || a.ldout_to == a.ldres_from);
+    const bool in_place = a.out == a.residual && a.out_type == a.res_type && same_rows &&
+                          (a.ldo == a.ldr || (a.m == 1 && !a.out_to));
+    const long long so = Bytes(a.out_type), sr = Bytes(a.res_type);
+    Want(in_place || !Overlap({a.out, a.out_rows, a.ldo * so, a.n * so}, {a.residual, a.res_rows, a.ldr * sr, a.n * sr}),
+         "linear_int8: out overlaps residual without being it, row by row through the same map");
   }
 }
 

@@ -299,7 +299,9 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     are left as they were (or, where the call makes out, have no value).
 
     out [M, N] may be given, else it is made, of `dtype` (float32).  It may be
-    residual itself; it must not overlap another input.  out_rows (int32 [M]):
+    residual itself, if out_rows and residual_rows are both absent or one and
+    the same tensor; it must not overlap residual otherwise (refused) nor
+    another input.  out_rows (int32 [M]):
     output row i goes to row out_rows[i] of a given out [O, N], skipped outside
     it; entries inside have to be distinct.  residual_rows (int32 [M]): its
     residual is row residual_rows[i] of residual [R, N], none outside it.  (A
