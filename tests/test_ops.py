@@ -238,3 +238,14 @@ def test_out_that_overlaps_the_residual_otherwise_than_row_by_row_is_refused(lib
     maps or through the same map."""
     assert _call(lib, "vamd_op_linear_int8", Linear, **{**IN_PLACE, **change}) < 0
     assert "overlap" in _err(lib) and "residual" in _err(lib)
+
+
+@pytest.mark.parametrize("change", [
+    dict(out_to=P, out_rows=1 << 62, ldo=9), dict(out_to=P, out_rows=(1 << 60) // 9, ldo=18), dict(out_to=P, out_rows=(1 << 62) + 5, ldo=64),
+    dict(out_to=P, out_rows=(1 << 31) // 36 + 1, ldo=9), dict(residual=P, ldr=9, res_from=P, res_rows=1 << 62),
+    dict(residual=P, ldr=64, res_from=P, res_rows=1 << 58), dict(residual=P, ldr=1 << 61, res_from=P, res_rows=8, m=1),
+    dict(out_to=P, out_rows=8, ldo=1 << 61, m=1),
+])
+def test_mapped_matrices_whose_size_passes_64_bits_are_refused(lib, change):
+    assert _call(lib, "vamd_op_linear_int8", Linear, **{**LINEAR, **change}) < 0
+    assert "2^31" in _err(lib)

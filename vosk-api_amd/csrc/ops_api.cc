@@ -43,6 +43,8 @@ void Want(bool ok, const char* what) {
 
 bool Aligned(const void* p, unsigned n) { return ((uintptr_t)p) % n == 0; }
 bool FloatTypeOk(int t) { return t == kFloat32 || t == kFloat16 || t == kBFloat16; }
+// rows * ld * bytes < 2^31, of rows >= 0 and ld >= 1 of any size
+bool Below31Bits(long long rows, long long ld, unsigned bytes) { return rows == 0 || ld <= ((1ll << 31) - 1) / bytes / rows; }
 unsigned Bytes(int t) { return t == kFloat32 ? 4 : 2; }
 
 template <class F>
@@ -108,14 +110,14 @@ void CheckLinear(const LinearInt8& a) {
   Want(!a.rows || a.m == 1 || a.ldrows >= a.taps, "linear_int8: rows of the row map overlap");
   Want(a.ldo >= a.n || (a.m == 1 && !a.out_to), "linear_int8: output rows overlap");
   Want(a.out_rows >= 0 && a.res_rows >= 0, "linear_int8: bad sizes");
-  Want(!a.out_to || a.out_rows * a.ldo * Bytes(a.out_type) < (1ll << 31),
+  Want(!a.out_to || Below31Bits(a.out_rows, a.ldo, Bytes(a.out_type)),
        "linear_int8: out has to be below 2^31 bytes where out_to maps its rows");
   Want(a.ldo <= kInt8MaxStride || (a.m == 1 && !a.out_to), "linear_int8: rows of out may be 2^23 elements apart at most");
   Want(Aligned(a.out, Bytes(a.out_type)), "linear_int8: out is not aligned to its elements");
   if (a.residual) {
     Want(FloatTypeOk(a.res_type), "linear_int8: unknown residual type");
     Want(a.ldr >= a.n || (a.m == 1 && !a.res_from), "linear_int8: residual rows overlap");
-    Want(!a.res_from || a.res_rows * a.ldr * Bytes(a.res_type) < (1ll << 31),
+    Want(!a.res_from || Below31Bits(a.res_rows, a.ldr, Bytes(a.res_type)),
          "linear_int8: residual has to be below 2^31 bytes where res_from maps its rows");
     Want(a.ldr <= kInt8MaxStride || (a.m == 1 && !a.res_from), "linear_int8: rows of residual may be 2^23 elements apart at most");
     Want(Aligned(a.residual, Bytes(a.res_type)), "linear_int8: residual is not aligned to its elements");
