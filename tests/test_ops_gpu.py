@@ -971,3 +971,26 @@ def test_linear_out_over_the_residual_otherwise_is_refused(ops):
         with pytest.raises(ValueError, match="overlap"):
             ops.linear_int8(x, w, ws, **kw)
     assert torch.equal(buf, before)
+
+
+@pytest.mark.parametrize("floats", [False, True])
+@pytest.mark.parametrize("m", [3, 20, 300])
+def test_linear_residual_of_no_rows_adds_nothing(ops, m, floats):
+    """res_rows = 0: no row is read, whatever the map names and wherever the matrix lies."""
+    g = _gen(m)
+    x = _randn(g, m, 64)
+    w, ws = ops.quantize_weight(_randn(g, 40, 64))
+    codes, scales = ops.quantize_rows(x)
+    kw = dict(scale=None if floats else scales)
+    want = ops.linear_int8(x if floats else codes, w, ws, **kw)
+    rows = torch.randint(-2, 5, (m,), generator=g, device="cuda", dtype=torch.int32)
+    got = ops.linear_int8(x if floats else codes, w, ws, residual=torch.zeros(0, 40, device="cuda"), residual_rows=rows, **kw)
+    assert torch.equal(got, want)
+    # the same in C, with an address: that of a matrix of NaN
+    nan = torch.full((8, 40), float("nan"), device="cuda")
+    out, space = torch.zeros_like(want), torch.empty(m * 68, dtype=torch.int8, device="cuda")
+    p = [t.data_ptr() for t in (codes, scales, x, space, w, ws, nan, out, rows)]
+    args = ops._LINEAR(*(0, 0, 0, 0, p[2], p[3]) if floats else (p[0], p[1], 0, 0, 0, 0), p[4], p[5], 0, 0, 0, p[6], p[7], 0, p[8],
+                       m, 0 if floats else 64, 64 if floats else 0, 64, 40, 40, 0, 0, 0, 1, 0, m, 40, 64, 1, 0, 0, 0, 0, 2.0)
+    assert ops._c.vamd_op_linear_int8(0, torch.cuda.current_stream().cuda_stream, args) == 0
+    assert torch.equal(out, want)

@@ -616,9 +616,9 @@ __device__ __forceinline__ void finish_one(const LinearInt8& a, float v, const C
   if (a.gain) y = y * c.gain + c.shift;
   if (a.residual) {
     const int from = a.res_from ? a.res_from[m * a.ldres_from] : m;
-    const bool there = from >= 0 && from < a.res_rows;
-    const float z = load_float(a.residual, a.res_type, (there ? from : 0) * a.ldr + n);
-    y = a.res_scale * (there ? z : 0.0f) + y;
+    // (an absent row is not read: there may be no row at all)
+    const float z = from >= 0 && from < a.res_rows ? load_float(a.residual, a.res_type, from * a.ldr + n) : 0.0f;
+    y = a.res_scale * z + y;
   }
   const int to = a.out_to ? a.out_to[m * a.ldout_to] : m;
   if (to >= 0 && to < a.out_rows) store_float(a.out, a.out_type, to * a.ldo + n, y);
