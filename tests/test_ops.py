@@ -249,3 +249,24 @@ def test_out_that_overlaps_the_residual_otherwise_than_row_by_row_is_refused(lib
 def test_mapped_matrices_whose_size_passes_64_bits_are_refused(lib, change):
     assert _call(lib, "vamd_op_linear_int8", Linear, **{**LINEAR, **change}) < 0
     assert "2^31" in _err(lib)
+
+
+def test_kernels_use_m0_for_loads_to_lds_alone(tmp_path):
+    """load_to_lds sets m0 unknown to the compiler: every instruction of the kernels' assembly that names m0 (or reads it
+    unnamed) is one of its own.  Built with the flags of the library; no packed fp32 instruction either."""
+    pkg = os.path.join(REPO, "vosk-api_amd")
+    made = subprocess.run(["make", "-C", pkg, "-n", "-B", "build/int8_ops.o"], capture_output=True, text=True, check=True).stdout
+    cmd = [ln for ln in made.splitlines() if "-c csrc/int8_ops.hip" in ln][0].split()
+    cmd[cmd.index("-c")] = "-S"
+    cmd[cmd.index("-o") + 1] = str(tmp_path / "a.s")
+    subprocess.run(cmd + ["--cuda-device-only"], cwd=pkg, check=True, capture_output=True)
+    code = [ln.split(";")[0].split("//")[0].strip() for ln in open(tmp_path / "a.s")]
+    code = [ln for ln in code if ln and not ln.startswith(".")]
+    sets = 0
+    for i, ln in enumerate(code):
+        if re.search(r"\bm0\b", ln):
+            assert re.fullmatch(r"s_mov_b32 m0, s\d+", ln), ln
+            assert code[i + 1] == "s_nop 0" and code[i + 2].startswith("global_load_lds_dwordx4 "), code[i:i + 3]
+            sets += 1
+        assert not re.match(r"(v_pk_\w+_f32|[sv]_movrel|v_interp|ds_gws|ds_append|ds_consume|s_sendmsg|buffer_load_\w+.*\blds\b)", ln), ln
+    assert sets == sum(ln.startswith("global_load_lds") for ln in code) > 0

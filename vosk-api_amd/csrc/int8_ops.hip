@@ -495,8 +495,10 @@ __global__ __launch_bounds__(THREADS) void frame_maps_kernel(FrameMaps all) {
 constexpr int kPartBytes = 64;
 
 // lane l's 16 bytes at p go to LDS byte `to` + 16 * l (to: the same in all lanes).
-// The compiler does not count these loads: the waits below do.  (Nothing else in
-// these kernels uses m0.)
+// The compiler does not count these loads: the waits below do.  Nor can it be told
+// that m0 changes (a reserved register: naming it as clobbered is warned against
+// and changes no instruction); it has no use for m0 of its own in these kernels,
+// which a test of their assembly holds it to.
 __device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "memory");
 }
