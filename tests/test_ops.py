@@ -270,3 +270,21 @@ def test_kernels_use_m0_for_loads_to_lds_alone(tmp_path):
             sets += 1
         assert not re.match(r"(v_pk_\w+_f32|[sv]_movrel|v_interp|ds_gws|ds_append|ds_consume|s_sendmsg|buffer_load_\w+.*\blds\b)", ln), ln
     assert sets == sum(ln.startswith("global_load_lds") for ln in code) > 0
+
+
+def test_forward_mode_tangents_are_refused_like_gradients():
+    """A dual tensor has an address and requires no gradient, but its tangent would be lost; under no_grad as well, which
+    is for reverse mode alone."""
+    import torch.autograd.forward_ad as fw
+    from vosk import ops
+    x = torch.ones(3, 4)
+    ops._no_grad(x, None, 1.0)
+    with fw.dual_level():
+        d = fw.make_dual(x, x)
+        ops._no_grad(x, None)
+        for t in (d, d[1:], d * 2):
+            with pytest.raises(ValueError, match="gradient"):
+                ops._no_grad(x, None, t)
+        with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
+            ops._no_grad(d)
+    ops._no_grad(d, x)

@@ -994,3 +994,25 @@ def test_linear_residual_of_no_rows_adds_nothing(ops, m, floats):
                        m, 0 if floats else 64, 64 if floats else 0, 64, 40, 40, 0, 0, 0, 1, 0, m, 40, 64, 1, 0, 0, 0, 0, 2.0)
     assert ops._c.vamd_op_linear_int8(0, torch.cuda.current_stream().cuda_stream, args) == 0
     assert torch.equal(out, want)
+
+
+def test_forward_mode_tangents_are_refused(ops):
+    import torch.autograd.forward_ad as fw
+    g = _gen(2)
+    x = _randn(g, 5, 64)
+    w, ws = ops.quantize_weight(_randn(g, 8, 64))
+    codes, scales = ops.quantize_rows(x)
+    y = _randn(g, 5, 8)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ops.quantize_rows(dual(x)), lambda: ops.quantize_rows(x, codes, dual(scales)), lambda: ops.quantize_weight(dual(x)),
+                     lambda: ops.linear_int8(dual(x), w, ws), lambda: ops.linear_int8(x, w, dual(ws)), lambda: ops.linear_int8(codes, w, ws, scale=dual(scales)),
+                     lambda: ops.linear_int8(x, w, ws, bias=dual(ws)), lambda: ops.linear_int8(x, w, ws, gain=ws, shift=dual(ws)),
+                     lambda: ops.linear_int8(x, w, ws, residual=dual(y)), lambda: ops.linear_int8(x, w, ws, out=dual(y))):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+        ops.linear_int8(x, w, ws)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.quantize_rows(x, codes, scales.clone().requires_grad_())
+    with pytest.raises((ValueError, RuntimeError)):  # (its tensors have no address)
+        torch.func.jvp(lambda a: ops.linear_int8(a, w, ws), (x,), (x,))

@@ -11,8 +11,8 @@ precision="int8")), on tensors of the caller's.  Calls go to the current
 stream of the tensors' device, wait for nothing and may be captured into a
 graph.  A tensor used on another stream than the one it was allocated on has
 to be kept by the caller as torch asks (Tensor.record_stream).  A wrong
-argument raises ValueError before anything is enqueued.  There is no backward:
-tensors that require gradients are refused.
+argument raises ValueError before anything is enqueued.  There is no backward
+and no forward mode: tensors that require gradients or carry tangents are refused.
 
 libvosk.so and torch have to share one HIP runtime, which they do when torch
 is imported first; importing this module after vosk alone raises ImportError.
@@ -24,6 +24,7 @@ import functools
 import struct
 
 import torch
+import torch.autograd.forward_ad as _forward
 
 from . import _c
 
@@ -146,6 +147,10 @@ def _no_grad(*ts):
         for t in ts:
             if getattr(t, "requires_grad", False):
                 _refuse("a tensor requires a gradient: the 8-bit operators have no backward")
+    if _forward._current_level >= 0:  # (no_grad is for reverse mode alone)
+        for t in ts:
+            if isinstance(t, torch.Tensor) and _forward.unpack_dual(t).tangent is not None:
+                _refuse("a tensor has a forward-mode gradient: the 8-bit operators have none")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -202,6 +207,7 @@ def quantize_rows(x, codes=None, scales=None, rows=None, count=None, from_rows=N
             _refuse("codes has to be int8")
         if cols < kb:
             _refuse("codes has to have %d columns" % kb)
+        _no_grad(scales)
         sp = _vector(scales, "scales", _f32, c, dev)
         xr = m
         if from_rows is not None:
