@@ -268,3 +268,12 @@ def test_streams_past_the_limit_of_a_ring_are_refused_with_the_number(synth_mode
     from vosk import engine
     with pytest.raises(RuntimeError, match="at most 2047 streams an engine"):
         engine.Engine(synth_model, frames_per_chunk=51, max_streams=2048, precision="int8")
+
+
+def test_an_empty_environment_variable_is_none(synth_model, monkeypatch):
+    from vosk import engine
+    monkeypatch.setenv("VOSK_AMD_NNET", "")
+    for precision, layers in (("fp32", 0), ("int8", 24)):
+        e = engine.Engine(synth_model, max_streams=1, precision=precision)
+        assert e.int8_layers == layers
+        e.close()

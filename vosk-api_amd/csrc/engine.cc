@@ -330,7 +330,7 @@ Engine::Engine(std::shared_ptr<const ModelData> md, const EngineConfig& cfg) : m
   cfg_.frames_per_chunk = fpc;
   plan_ = BuildNnetPlan(m.nnet, fpc, fss, m.dcb.acoustic_scale);
   if (LogLevel() > 0) VAMD_LOG(plan_.Describe());
-  if (const char* o = getenv("VOSK_AMD_NNET")) {
+  if (const char* o = getenv("VOSK_AMD_NNET"); o && *o) {
     const std::string v(o);
     if (v == "int8") cfg_.nnet_int8 = true;
     else if (v == "fp32") cfg_.nnet_int8 = false;
