@@ -1016,3 +1016,17 @@ def test_forward_mode_tangents_are_refused(ops):
         ops.quantize_rows(x, codes, scales.clone().requires_grad_())
     with pytest.raises((ValueError, RuntimeError)):  # (its tensors have no address)
         torch.func.jvp(lambda a: ops.linear_int8(a, w, ws), (x,), (x,))
+
+
+def test_a_device_that_is_not_there_leaves_no_error_behind(ops):
+    """The call fails and says why; the next launch of the process, whoever's, does not report it again."""
+    x = _randn(_gen(0), 4, 64)
+    c, s = torch.empty(4, 64, dtype=torch.int8, device="cuda"), torch.empty(4, device="cuda")
+    torch.cuda.synchronize()
+    args = ops._ROWS(x.data_ptr(), 0, 0, 0, c.data_ptr(), s.data_ptr(), 4, 64, 4, 64, 0, 0, 4, 0, 64)
+    for device in (torch.cuda.device_count(), -1):
+        assert ops._c.vamd_op_quantize_rows(device, None, args) < 0
+        assert b"HIP error" in ops._c.vamd_last_error()
+        torch.add(x, 1.0)
+        ops.quantize_rows(x)
+    torch.cuda.synchronize()

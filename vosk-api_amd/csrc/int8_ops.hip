@@ -1084,8 +1084,10 @@ __global__ __launch_bounds__(kNarrowThreads) void linear_narrow_kernel(LinearInt
 // more than 64 KB of LDS has to be asked for
 void AskLds(const void* kernel, size_t bytes) {
   if (bytes > 64 * 1024 &&
-      hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess)
+      hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess) {
+    (void)hipGetLastError();
     VAMD_ERR("the device does not give a workgroup " << bytes << " bytes of LDS");
+  }
 }
 
 }  // namespace

@@ -28,7 +28,9 @@ class OnDevice {
     if (changed_) (void)hipSetDevice(before_);
   }
   static void Check(hipError_t e) {
-    if (e != hipSuccess) throw Fatal(std::string("HIP error ") + hipGetErrorString(e));
+    if (e == hipSuccess) return;
+    (void)hipGetLastError();  // told here: the next launch's check, whoever's, does not find it
+    throw Fatal(std::string("HIP error ") + hipGetErrorString(e));
   }
 
  private:
