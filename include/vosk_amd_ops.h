@@ -31,8 +31,11 @@ int vamd_op_code_bytes(int k);
 
 /* Rows of floats to 8-bit codes with a 32-bit scale for each row:
  *   scale = fl32(max |x| / 127), code = x / scale rounded half to even
- * exactly, so code * scale is within scale / 2 of x.  A row of zeros gets
- * scale 0; a row that holds an Inf or a NaN gets scale NaN and codes 0. */
+ * exactly, so code * scale is within scale / 2 of x where scale is a normal
+ * float (max |x| from 127 * 2^-126 on).  A smaller scale is rounded to a
+ * multiple of 2^-149: codes end at -127 and 127 then, and a row whose scale
+ * rounds to 0 (max |x| up to 63 * 2^-149) gets codes 0, as a row of zeros
+ * does.  A row that holds an Inf or a NaN gets scale NaN and codes 0. */
 typedef struct {
     const void *x;           /* rows of k of `type`, ldx elements apart */
     const int *rows;         /* or NULL: row i goes to row rows[i * ldrows] of codes and scales; an entry
@@ -84,8 +87,10 @@ int vamd_op_frame_map(int device, void *stream, const VamdFrameMap *args);
  * With x (and codes and scale NULL) rows of floats take the place of codes:
  * they are quantised as by vamd_op_quantize_rows in the call, which may take a
  * workspace (vamd_op_linear_workspace).  rows then maps the cache_rows rows of
- * x; without it x has m rows.  m is at
- * most 2^30, n and the row strides ldr and ldo at most 2^23. */
+ * x; without it x has m rows.  Where the workspace is not 0 all cache_rows
+ * rows are quantised, however few of them the map names: a large cache is
+ * better kept in codes.  m is at most 2^30, n and the row strides ldr and ldo at
+ * most 2^23. */
 typedef struct {
     const signed char *codes; /* rows of kb bytes, lda apart; 16-byte aligned rows */
     const float *scale;      /* [cache_rows] */

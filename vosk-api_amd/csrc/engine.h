@@ -382,8 +382,8 @@ class Engine {
   bool Step(const std::vector<int>& slots, bool allow_pipeline = true);
   void SetStepSamples(int n) { cfg_.max_step_samples = n; }
   const StageTimes& stage_times() const { return times_; }
+  long long NnetLaunches() const;  // kernels of one pass of the acoustic model
   // layers that run as 8-bit products (0: a 32-bit engine)
-  long long NnetLaunches() const;  // of one pass
   int Int8Layers() const { return cfg_.nnet_int8 ? int8_.products : 0; }
   bool kaldi_order() const { return dec_.kaldi != 0; }  // the decoder's token-passing order
   void ResetStageTimes() { times_ = StageTimes(); }

@@ -169,8 +169,9 @@ def quantize_rows(x, codes=None, scales=None, rows=None, count=None, from_rows=N
 
       scale = fl32(max |x| / 127), code = x / scale rounded half to even,
 
-    decided exactly.  A row of zeros gets scale 0; a row holding an Inf or a
-    NaN gets scale NaN and codes 0.  Returns (codes int8 [M, code_bytes(K)],
+    decided exactly.  A row of zeros gets scale 0 (a row so small that its
+    scale is no normal float as well, or codes that end at +-127); a row holding
+    an Inf or a NaN gets scale NaN and codes 0.  Returns (codes int8 [M, code_bytes(K)],
     scales float32 [M]); columns from K on are zero.
 
     codes and scales may be given (codes [C, >= code_bytes(K)], its rows
@@ -224,7 +225,7 @@ def quantize_weight(w, taps=1):
     """A weight matrix [N, taps * K] (one block of K columns for each spliced
     frame) as linear_int8 takes it: (codes int8 [N, taps * code_bytes(K)],
     scales float32 [N]), one scale for each output column n, the rounding of
-    quantize_rows."""
+    quantize_rows (and its limit: taps * K is at most 131 072)."""
     _on(w, "w")
     if w.dim() != 2 or taps < 1 or w.shape[1] % taps:
         _refuse("w has to be [N, taps * K]")
@@ -299,8 +300,10 @@ def linear_int8(x, weight, weight_scale, *, scale=None, rows=None, count=None, b
     weight: int8 [N, J * code_bytes(K)] in -127 .. 127, weight_scale: float32 [N]
     (quantize_weight).  x is either int8 codes [C, code_bytes(K)] with scale
     float32 [C] (quantize_rows), or float rows [C, K] that are quantised in
-    the call, to the same codes.  rows (int32 [M, J], frame_map) says which
-    rows of x are read; an entry outside [0, C) adds nothing.  Without it row
+    the call, to the same codes (all C rows, but for the smallest calls: float
+    rows that a map reads few of are better quantised before, with from_rows).
+    rows (int32 [M, J], frame_map) says which rows of x are read; an entry
+    outside [0, C) adds nothing.  Without it row
     i reads row i.  count (int32, one element, on the GPU): output rows from there on
     are left as they were (or, where the call makes out, have no value).
 
