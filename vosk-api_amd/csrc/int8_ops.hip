@@ -241,7 +241,7 @@ void LaunchQuantize(const QuantizeRows& a, hipStream_t s) {
 // with more, a first launch has written `starts` and the search reads those.
 // Bound by latencies one after another (lengths, sums, search, the stream's
 // numbers, its pages), not by its bytes: one stream of 51 frames 3.7 to 4.3 us,
-// 256 streams 5.4, 4 001 streams and 2 M entries (8 MB) 10.7.
+// 256 streams 5.2 to 5.8, 4 001 streams and 2 M entries (8 MB) 10.8 to 12.1.
 // Larger workgroups sum more streams: 4 001 streams in one of 256 / 512 / 1024
 // threads, 400 100 rows of 5 entries 10.4 / 9.2 / 10.2 us, 8 002 rows 8.3 / 7.2 /
 // 7.7.
@@ -487,11 +487,13 @@ __global__ __launch_bounds__(THREADS) void frame_maps_kernel(FrameMaps all) {
 // after lane), so that the sixteen lanes which a 16-byte-a-lane read serves
 // together, four runs of four rows, lie in different banks ((row >> 1) & 3,
 // right for eight neighbouring rows, cost 1.5 times the reads' cycles).
-// A product of 8192 x 4096 x 4096 takes 131 to 141 us (1.95 to 2.1 POP/s): the
-// matrix units are busy 50 % of the cycles, LDS has no bank conflict, L2 serves
-// 86 % of the lines, and the clock gives way under load (codes that are all
-// zero: 102 us).  Deeper rings, four waves of 128 x 128 and reads further ahead
-// of the products changed nothing there.
+// A product of 8192 x 4096 x 4096 takes 139 us (2.0 POP/s; in a graph, where a
+// library's bare integer product takes 129 on the same card; 143 on another;
+// 151 between other kernels): the matrix units are busy 50 % of the cycles, LDS
+// has no bank conflict, L2 serves 86 % of the lines, and the clock gives way
+// under load (codes that are all zero: 112 us, the library's 103).  Deeper
+// rings, four waves of 128 x 128 and reads further ahead of the products changed
+// nothing there.
 constexpr int kPartBytes = 64;
 
 // lane l's 16 bytes at p go to LDS byte `to` + 16 * l (to: the same in all lanes).
@@ -1223,11 +1225,16 @@ void LaunchFused(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
 
 }  // namespace
 
-// Each workgroup quantises all rows: one launch up to 16384 values, which a
-// program that calls it from Python gets back (us a call, one launch / two: 1 x
-// 4096 x 4096 7.1 / 11.6, 4 x 4096 x 4096 9.1 / 11.5, 16 x 1024 x 96 8.3 / 11.7)
-// and which costs little in a graph (1 x 4096 x 4096 5.6 / 6.9, 16 x 512 x 512
-// 5.6 / 5.6, 4 x 4096 x 4096 8.6 / 7.7, 32 x 512 x 512 7.7 / 5.7).
+// Each workgroup quantises all rows: one launch up to 16384 values, chosen for
+// the program that calls it from Python and waits for the calls, not the GPU (us
+// a call of bf16 rows, one launch / two: 1 x 4096 x 4096 7.1 / 11.6, 4 x 4096 x
+// 4096 9.1 / 11.5, 16 x 1024 x 96 8.3 / 11.7).  In a graph it gains with one or
+// two rows (bf16 / fp32 rows, one launch against two: 1 x 4096 x 4096 5.6
+// against 7.1 / 6.3 against 7.3, 2 x 512 x 512 4.7 against 5.9 / 4.2 against
+// 5.7), costs little at 16 x 512 x 512 (6.1 against 6.2 / 7.6 against 6.0) and
+// most at the end of the range (4 x 4096 x 4096 9.4 against 8.2 / 11.8 against
+// 7.7, 32 x 512 x 512 8.1 against 6.3 / 10.6 against 6.0): a graph of such calls
+// is better off with quantize_rows and codes.
 bool LinearFloatFused(int m, int k, int taps) { return m <= 32 && (long long)m * k * taps <= kFusedValues; }
 
 void LaunchLinearFloat(const LinearInt8& a, const QuantizeRows& x, hipStream_t s) {
@@ -1260,16 +1267,20 @@ void LaunchLinearInt8(const LinearInt8& a, hipStream_t s) {
   // 128 / 256 x 256 tiles):
   //   1999 x 777 x 1001    7.4 /  9.8 / 18.1
   //   4352 x 512 x 512     7.1 /  7.7 / 12.9
-  //   2048 x 2000 x 1024  13.0 / 11.6 / 19.2
-  //   13056 x 512 x 512   13.3 / 11.5 / 15.3
-  //   13056 x 4096 x 1024  117 / 81.0 / 90.7
-  //   4096 x 4096 x 2048  67.3 / 45.9 / 43.3
-  //   8192 x 4096 x 4096   237 /  160 /  135
+  //   2048 x 2000 x 1024  14.3 / 12.4 / 20.1
+  //   13056 x 512 x 512   16.1 / 12.1 / 15.7
+  //   8192 x 4096 x 1024  87.8 / 54.6 / 55.4
+  //   13056 x 4096 x 1024  135 / 86.2 / 94.2
+  //   4096 x 4096 x 2048  73.7 / 48.9 / 44.7
+  //   16384 x 4096 x 2048  298 /  180 /  161
+  //   8192 x 4096 x 4096   254 /  170 /  143
+  // (K from 2048 on takes the largest; shorter ones would gain from it only with
+  // very many rows, 16384 x 4096 x 1024 113 / 103, 16384 x 4096 x 512 78.7 / 73.5)
   // but short products, which the stores bound, in the smallest:
   //   4352 x 2000 x 192   11.1 / 13.8 / 13.3
   // and the largest, of which a CU holds one, only where the last round of
-  // them is nearly full: 5000 x 5000 x 5000 (400 tiles) 173 / 140, but 4864 x
-  // 4096 x 4096 (304) 99.0 / 114.
+  // them is nearly full: 5000 x 5000 x 5000 (400 tiles) 181 / 149, but 4864 x
+  // 4096 x 4096 (304) 104 / 118.
   // Several taps hold a second set of accumulators, for which the largest
   // tiles have no registers; theirs gain from 128 x 128 at short K too:
   //   13056 x 512 x 2 * 96  15.3 / 13.9
