@@ -41,3 +41,12 @@ def test_a_failing_import_can_be_tried_again(tmp_path):
                "try:\n    import vosk\nexcept OSError as e:\n    print('/nowhere' in str(e), 'vosk' in sys.modules)\n"
                "del os.environ['VOSK_AMD_LIB']\nimport vosk\nprint(hasattr(vosk, 'Model'))", tmp_path)
     assert got == ["True False", "True"]
+
+
+def test_two_threads_import_it(tmp_path):
+    """The second waits until the package is whole."""
+    got = _run("import sys, threading\nseen = []\n"
+               "def go():\n    import vosk\n    seen.append(hasattr(vosk, 'BatchRecognizer'))\n"
+               "sys.setswitchinterval(1e-5)\nts = [threading.Thread(target=go) for _ in range(8)]\n"
+               "[t.start() for t in ts]\n[t.join() for t in ts]\nprint(seen.count(True), len(seen))", tmp_path)
+    assert got == ["8 8"]

@@ -1,21 +1,9 @@
-"""`import vosk` for programs started in this folder: the package in vosk-api_amd/."""
-import importlib.util
+"""`import vosk` for programs started in this folder: this module becomes the package in vosk-api_amd/."""
+import importlib.machinery
 import os
-import sys
 
-
-def _load():
-    folder = os.path.join(os.path.dirname(os.path.abspath(__file__)), "vosk-api_amd", "vosk")
-    spec = importlib.util.spec_from_file_location(__name__, os.path.join(folder, "__init__.py"),
-                                                  submodule_search_locations=[folder])
-    package = importlib.util.module_from_spec(spec)
-    here = sys.modules[__name__]
-    sys.modules[__name__] = package  # what the import statement returns
-    try:
-        spec.loader.exec_module(package)
-    except BaseException:
-        sys.modules[__name__] = here  # (the import statement takes it out)
-        raise
-
-
-_load()
+__path__ = [os.path.join(os.path.dirname(os.path.abspath(__file__)), "vosk-api_amd", "vosk")]
+__file__ = os.path.join(__path__[0], "__init__.py")
+__package__ = __name__
+__spec__.submodule_search_locations = __path__
+exec(importlib.machinery.SourceFileLoader(__name__, __file__).get_code(__name__))
